@@ -1,6 +1,6 @@
 /*
  * trinity_b200 — C ABI of the sm_100a kernel backend for Trinity's fused attention-block operators
- * (Vanilla, PreNorm, QKNorm, KeyFormer, RoCo) and standalone RMSNorm.
+ * (Vanilla, PreNorm, QKNorm, KeyFormer, RoCo) and standalone RMSNorm, and of the 8-bit key/value cache beside them.
  *
  * This is the boundary a binding (ctypes, cgo, JNI ...) talks to.  Plain pointers and sizes only; no
  * torch types.  All pointers are DEVICE pointers unless a name ends in `_host`.  Nothing here
@@ -283,6 +283,112 @@ int trinity_topk(const TrnTopkArgs* a, void* cuda_stream);
  * fp32 accumulation.
  * ---------------------------------------------------------------------------------------------- */
 int trinity_convert(const void* src, void* dst, int64_t n, int dtype16, int to_fp32, void* cuda_stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Key/value cache in 8 bits.  The reference keeps its caches in 16 bits (convert_eval_rms.py:62-108) and has no
+ * counterpart of what follows.
+ *
+ * A cache holds, for every (batch item b, position s in [0,S), kv head h), D e4m3 codes of the key and D of the value,
+ * and one fp32 scale for every `block` consecutive positions of a (b, h), separately for keys and values: the element's
+ * value is code * scale[b, s / block, h].  trinity_cache_append writes scales that are powers of two; a caller that
+ * fills a cache itself may hold any positive scale within [2^-64, 2^120] (and 0 for a block of zeros).
+ * Scale tensors address (b, block j, h) as ptr + b*stride_b + j*stride_s + h*stride_h, ceil(S / block) blocks.
+ * Codes: 16-byte aligned base, strides positive multiples of 16 (dims of extent 1: any stride), d contiguous.
+ *
+ * How many positions a sequence holds stands on the device, one int32 per batch item (`kv_len`), so that a captured
+ * step replays while the sequences grow; with kv_len == NULL every sequence holds `kv_len_all`.  A value outside
+ * [0, S] counts as the nearer end.  Nothing behind a sequence's last position is read into a result, whatever it holds
+ * (NaN codes included), and nothing behind it is written but the new rows of an append.
+ * ---------------------------------------------------------------------------------------------- */
+typedef struct {
+  TrnHeadTensor k, v;             /* e4m3 codes; with block == 0, where an entry point allows it: 16-bit elements */
+  TrnHeadTensor k_scale, v_scale; /* fp32; stride_s is the stride between blocks; unused with block == 0 */
+  int S;                          /* positions a (b, h) has room for */
+  int block;                      /* positions per scale: 16, 32, 64 or 128 */
+} TrnCacheQ8;
+
+/* Append: rows [kv_len[b], kv_len[b] + M) of every (b, h) become the new keys / values (16-bit, (b, i, h, d)); rows that
+ * would fall behind S are dropped.  kv_len counts what the cache holds BEFORE the call and is not changed.
+ * A block's scale is the smallest power of two 2^e with |x| <= 448 * 2^e for its new finite values, -64 <= e <= 120; a
+ * block that already holds positions keeps the larger of its scale and that one, and where the scale grew its older
+ * codes are rewritten (exact but for what falls under the smallest code).  Codes are rounded to nearest even.  An
+ * infinite or NaN element is held as NaN and does not count for the scale.  D is 64 or 128. */
+typedef struct {
+  TrnCacheQ8 cache;
+  TrnHeadTensor k_new, v_new;     /* s in [0,M) */
+  const int32_t* kv_len;          /* device, [B], or NULL */
+  int kv_len_all;
+  int B, M, Hkv, D;
+  int dtype;                      /* of k_new / v_new */
+} TrnCacheAppendArgs;
+int trinity_cache_append(const TrnCacheAppendArgs* a, void* cuda_stream);
+
+/* Read: code * scale, rounded to `dtype`, of positions [0, kv_len[b]) into k_out / v_out; the rest of these is left as
+ * it is.  Hands an 8-bit cache to the operators that take 16-bit ones (exact in bf16 for power-of-two scales). */
+typedef struct {
+  TrnCacheQ8 cache;
+  TrnHeadTensor k_out, v_out;     /* s in [0, min(kv_len[b], S_out)) */
+  int S_out;                      /* positions k_out / v_out have room for; the rest of a longer sequence is not read */
+  const int32_t* kv_len;
+  int kv_len_all;
+  int B, Hkv, D;
+  int dtype;                      /* of k_out / v_out */
+} TrnCacheReadArgs;
+int trinity_cache_read(const TrnCacheReadArgs* a, void* cuda_stream);
+
+/* Attention over the 8-bit cache, kv_len[b] positions each (the new ones included):
+ *   s = scale * q k^T,  causal: query i of M sees positions j <= kv_len[b] - M + i
+ *   o = softmax(s) v;  lse (optional) as in TrnAttnArgs;  a row that sees no position: o = 0, lse = -inf
+ *   weight (optional): weight[b, h, j] = (weight_add ? weight[b, h, j] : 0) + sum over the queries and the query heads
+ *   of kv head h of p_j, for j < kv_len[b]; the rest is left as it is.  It is what trinity_cache_evict selects by.
+ *   Fixed summation order: results are bitwise reproducible.
+ * Any Hq that is a multiple of Hkv, any M >= 1, D 64 or 128; at most 16 queries (M) with `weight`. */
+typedef struct {
+  TrnHeadTensor q;                /* s in [0,M) */
+  TrnCacheQ8 cache;
+  TrnHeadTensor o;
+  float* lse;                     /* fp32 [B, Hq, M] or NULL */
+  float* weight;                  /* fp32 (b, h, j), j contiguous, or NULL */
+  int64_t weight_stride_b, weight_stride_h;
+  int weight_add;
+  const int32_t* kv_len;
+  int kv_len_all;
+  int B, M, Hq, Hkv, D;
+  int dtype;                      /* of q and o */
+  int causal;
+  float scale;
+  void* workspace;                /* 256-byte aligned device scratch of trinity_attention_q8_workspace() bytes; contents need
+                                     not be initialised.  NULL without `weight`: the key range is not divided. */
+  size_t workspace_bytes;
+} TrnAttnQ8Args;
+int trinity_attention_q8(const TrnAttnQ8Args* a, void* cuda_stream);
+/* Scratch for this shape (reads B, M, Hq, Hkv, D, cache.S, causal, and whether `weight` is given). */
+size_t trinity_attention_q8_workspace(const TrnAttnQ8Args* a);
+
+/* Eviction: of the n = kv_len[b] positions of every (b, kv head h) min(n, keep) stay: positions j < first and
+ * j >= n - recent, and of the others those of the largest score, equal scores by the lower position (a NaN score ranks
+ * above every number).  The score of a position is the sum over the Hs / Hkv score heads of kv head h, taken in 64 bits
+ * and rounded to fp32.  What stays moves, in the order it had, to rows [0, min(n, keep)) of ANOTHER cache (the two must
+ * not overlap); its rows behind them are left as they are.
+ * 8-bit caches: a destination block's scale is the largest scale its rows had, their codes are rewritten to it (exact for
+ * power-of-two scales but for what falls under the smallest code).  src.block == 0 and dst.block == 0: both caches hold
+ * 16-bit elements and rows are copied.  src.block must equal dst.block.
+ * idx [B, Hkv, keep] receives the positions, ascending, -1 behind the last; scores_out (optional) their fp32 scores, 0
+ * behind the last; kv_len_out (optional) [B] min(n, keep).  recent + first <= keep; src.S <= 262144; D is 64 or 128. */
+typedef struct {
+  TrnCacheQ8 src, dst;
+  const float* scores;            /* fp32 (b, hs, j), j contiguous */
+  int64_t score_stride_b, score_stride_h;
+  int Hs;                         /* score heads: a multiple of Hkv */
+  int32_t* idx;                   /* [B, Hkv, keep] contiguous */
+  float* scores_out;              /* [B, Hkv, keep] contiguous, or NULL */
+  int32_t* kv_len_out;            /* [B] or NULL */
+  const int32_t* kv_len;
+  int kv_len_all;
+  int B, Hkv, D;
+  int keep, recent, first;
+} TrnCacheEvictArgs;
+int trinity_cache_evict(const TrnCacheEvictArgs* a, void* cuda_stream);
 
 /* ------------------------------------------------------------------------------------------------
  * Whole block, the unit the reference's generated forward() computes (TritonGen.py:590-708):

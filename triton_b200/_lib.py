@@ -29,6 +29,8 @@ EXPORTS = (
     "trinity_clear_kernel_status", "trinity_selftest_wait_timeout",
     "trinity_rmsnorm", "trinity_qkv_project", "trinity_lora", "trinity_gmlp", "trinity_attention", "trinity_attention_workspace",
     "trinity_attn_colstats", "trinity_topk",
+    "trinity_cache_append", "trinity_cache_read", "trinity_attention_q8", "trinity_attention_q8_workspace",
+    "trinity_cache_evict",
     "trinity_attn_block_workspace", "trinity_attn_block", "trinity_attn_block_host",
     "trinity_static_scratch_capacity", "trinity_attn_block_static", "trinity_convert",
 )
@@ -104,6 +106,47 @@ class TrnTopkArgs(C.Structure):
     ]
 
 
+class TrnCacheQ8(C.Structure):
+    _fields_ = [
+        ("k", TrnHeadTensor), ("v", TrnHeadTensor), ("k_scale", TrnHeadTensor), ("v_scale", TrnHeadTensor),
+        ("S", C.c_int), ("block", C.c_int),
+    ]
+
+
+class TrnCacheAppendArgs(C.Structure):
+    _fields_ = [
+        ("cache", TrnCacheQ8), ("k_new", TrnHeadTensor), ("v_new", TrnHeadTensor), ("kv_len", C.c_void_p),
+        ("kv_len_all", C.c_int), ("B", C.c_int), ("M", C.c_int), ("Hkv", C.c_int), ("D", C.c_int), ("dtype", C.c_int),
+    ]
+
+
+class TrnCacheReadArgs(C.Structure):
+    _fields_ = [
+        ("cache", TrnCacheQ8), ("k_out", TrnHeadTensor), ("v_out", TrnHeadTensor), ("S_out", C.c_int),
+        ("kv_len", C.c_void_p), ("kv_len_all", C.c_int), ("B", C.c_int), ("Hkv", C.c_int), ("D", C.c_int),
+        ("dtype", C.c_int),
+    ]
+
+
+class TrnAttnQ8Args(C.Structure):
+    _fields_ = [
+        ("q", TrnHeadTensor), ("cache", TrnCacheQ8), ("o", TrnHeadTensor), ("lse", C.c_void_p), ("weight", C.c_void_p),
+        ("weight_stride_b", C.c_int64), ("weight_stride_h", C.c_int64), ("weight_add", C.c_int),
+        ("kv_len", C.c_void_p), ("kv_len_all", C.c_int), ("B", C.c_int), ("M", C.c_int), ("Hq", C.c_int),
+        ("Hkv", C.c_int), ("D", C.c_int), ("dtype", C.c_int), ("causal", C.c_int), ("scale", C.c_float),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class TrnCacheEvictArgs(C.Structure):
+    _fields_ = [
+        ("src", TrnCacheQ8), ("dst", TrnCacheQ8), ("scores", C.c_void_p), ("score_stride_b", C.c_int64),
+        ("score_stride_h", C.c_int64), ("Hs", C.c_int), ("idx", C.c_void_p), ("scores_out", C.c_void_p),
+        ("kv_len_out", C.c_void_p), ("kv_len", C.c_void_p), ("kv_len_all", C.c_int), ("B", C.c_int), ("Hkv", C.c_int),
+        ("D", C.c_int), ("keep", C.c_int), ("recent", C.c_int), ("first", C.c_int),
+    ]
+
+
 class TrnBlockArgs(C.Structure):
     _fields_ = [
         ("variant", C.c_int), ("dtype", C.c_int),
@@ -160,7 +203,9 @@ def load() -> C.CDLL:
     lib.trinity_last_kernel_status.argtypes = [C.POINTER(C.c_int)]
     for name, typ in (("trinity_rmsnorm", TrnRmsArgs), ("trinity_qkv_project", TrnProjArgs), ("trinity_lora", TrnLoraArgs), ("trinity_gmlp", TrnGmlpArgs),
                       ("trinity_attention", TrnAttnArgs), ("trinity_attn_colstats", TrnColStatsArgs),
-                      ("trinity_topk", TrnTopkArgs), ("trinity_attn_block", TrnBlockArgs),
+                      ("trinity_topk", TrnTopkArgs), ("trinity_cache_append", TrnCacheAppendArgs),
+                      ("trinity_cache_read", TrnCacheReadArgs), ("trinity_attention_q8", TrnAttnQ8Args),
+                      ("trinity_cache_evict", TrnCacheEvictArgs), ("trinity_attn_block", TrnBlockArgs),
                       ("trinity_attn_block_host", TrnBlockHostArgs), ("trinity_attn_block_static", TrnBlockArgs)):
         fn = getattr(lib, name)
         fn.restype = C.c_int
@@ -169,6 +214,8 @@ def load() -> C.CDLL:
     lib.trinity_attn_block_workspace.argtypes = [C.POINTER(TrnBlockArgs)]
     lib.trinity_attention_workspace.restype = C.c_size_t
     lib.trinity_attention_workspace.argtypes = [C.POINTER(TrnAttnArgs)]
+    lib.trinity_attention_q8_workspace.restype = C.c_size_t
+    lib.trinity_attention_q8_workspace.argtypes = [C.POINTER(TrnAttnQ8Args)]
     lib.trinity_clear_kernel_status.restype = C.c_int
     lib.trinity_clear_kernel_status.argtypes = []
     lib.trinity_selftest_wait_timeout.restype = C.c_int

@@ -83,8 +83,10 @@ int get_device_state(DeviceState** out) {
   return TRN_OK;
 }
 
-int make_tmap_16bit(CUtensorMap* out, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
-                    const uint32_t* box) {
+namespace {
+
+int make_tmap(CUtensorMap* out, CUtensorMapDataType type, uint64_t elem, CUtensorMapSwizzle swizzle, const void* base,
+              int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box) {
   if (g_encode == nullptr) {
     int rc = load_encode_fn();
     if (rc != TRN_OK) return rc;
@@ -101,16 +103,29 @@ int make_tmap_16bit(CUtensorMap* out, const void* base, int rank, const uint64_t
     gbox[i] = box[i];
     estride[i] = 1;
     if (i >= 1) {
-      const uint64_t bytes = strides[i] * 2ull;
+      const uint64_t bytes = strides[i] * elem;
       if ((bytes & 15ull) != 0) return TRN_E_ALIGN;
       gstride[i - 1] = bytes;
     }
   }
-  CUresult r = g_encode(out, CU_TENSOR_MAP_DATA_TYPE_UINT16, static_cast<cuuint32_t>(rank), const_cast<void*>(base),
-                        gdim, gstride, gbox, estride, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CUresult r = g_encode(out, type, static_cast<cuuint32_t>(rank), const_cast<void*>(base), gdim, gstride, gbox, estride,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return record_driver_error(r, "cuTensorMapEncodeTiled");
   return TRN_OK;
+}
+
+}  // namespace
+
+int make_tmap_16bit(CUtensorMap* out, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
+                    const uint32_t* box) {
+  return make_tmap(out, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, CU_TENSOR_MAP_SWIZZLE_128B, base, rank, dims, strides, box);
+}
+
+int make_tmap_8bit(CUtensorMap* out, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
+                   const uint32_t* box, bool swizzle128) {
+  return make_tmap(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                   base, rank, dims, strides, box);
 }
 
 int ensure_dyn_smem(const void* kernel, int bytes, int device) {
@@ -327,6 +342,48 @@ int trinity_topk(const TrnTopkArgs* a, void* cuda_stream) {
   int rc = get_device_state(&ds);
   if (rc != TRN_OK) return rc;
   return launch_topk(*a, static_cast<cudaStream_t>(cuda_stream), *ds);
+}
+
+int trinity_cache_append(const TrnCacheAppendArgs* a, void* cuda_stream) {
+  if (a == nullptr) return TRN_E_NULL;
+  int rc = check_cache_append(*a);
+  if (rc != TRN_OK) return rc;
+  DeviceState* ds = nullptr;
+  rc = get_device_state(&ds);
+  if (rc != TRN_OK) return rc;
+  return launch_cache_append(*a, static_cast<cudaStream_t>(cuda_stream));
+}
+
+int trinity_cache_read(const TrnCacheReadArgs* a, void* cuda_stream) {
+  if (a == nullptr) return TRN_E_NULL;
+  int rc = check_cache_read(*a);
+  if (rc != TRN_OK) return rc;
+  DeviceState* ds = nullptr;
+  rc = get_device_state(&ds);
+  if (rc != TRN_OK) return rc;
+  return launch_cache_read(*a, static_cast<cudaStream_t>(cuda_stream));
+}
+
+int trinity_attention_q8(const TrnAttnQ8Args* a, void* cuda_stream) {
+  if (a == nullptr) return TRN_E_NULL;
+  int rc = check_attention_q8(*a);
+  if (rc != TRN_OK) return rc;
+  DeviceState* ds = nullptr;
+  rc = get_device_state(&ds);
+  if (rc != TRN_OK) return rc;
+  return launch_attention_q8(*a, static_cast<cudaStream_t>(cuda_stream), *ds);
+}
+
+size_t trinity_attention_q8_workspace(const TrnAttnQ8Args* a) { return a == nullptr ? 0 : attention_q8_workspace(*a); }
+
+int trinity_cache_evict(const TrnCacheEvictArgs* a, void* cuda_stream) {
+  if (a == nullptr) return TRN_E_NULL;
+  int rc = check_cache_evict(*a);
+  if (rc != TRN_OK) return rc;
+  DeviceState* ds = nullptr;
+  rc = get_device_state(&ds);
+  if (rc != TRN_OK) return rc;
+  return launch_cache_evict(*a, static_cast<cudaStream_t>(cuda_stream), *ds);
 }
 
 int trinity_convert(const void* src, void* dst, int64_t n, int dtype16, int to_fp32, void* cuda_stream) {

@@ -15,19 +15,19 @@ struct HeadMapInfo {
   int pos_s, pos_h, pos_b;
 };
 
-// Tile = `box_rows` positions x 64 head_dim elements of one (b, h).
-inline int make_head_tmap(CUtensorMap* out, HeadMapInfo* info, const TrnHeadTensor& t, int S, int H, int B, int D,
-                          uint32_t box_rows) {
+// dims of a (b, s, h, d) tensor by ascending stride, d first (extents and strides in elements, tile extents)
+inline int order_head_dims(HeadMapInfo* info, const TrnHeadTensor& t, int S, int H, int B, int D, uint32_t box_rows,
+                           uint64_t span_align, uint64_t (&dims)[4], uint64_t (&strides)[4], uint32_t (&box)[4]) {
   if (t.ptr == nullptr) return TRN_E_NULL;
   // dims of extent 1 may carry any stride: give them one that keeps the descriptor valid
   uint64_t ss = static_cast<uint64_t>(t.stride_s), sh = static_cast<uint64_t>(t.stride_h),
            sb = static_cast<uint64_t>(t.stride_b);
-  if (t.stride_s < 0 || t.stride_h < 0 || t.stride_b < 0) return TRN_E_SHAPE;
+  if ((S > 1 && t.stride_s < 0) || (H > 1 && t.stride_h < 0) || (B > 1 && t.stride_b < 0)) return TRN_E_SHAPE;
   uint64_t span = static_cast<uint64_t>(D);
   if (S > 1 && ss * S > span) span = ss * S;
   if (H > 1 && sh * H > span) span = sh * H;
   if (B > 1 && sb * B > span) span = sb * B;
-  span = (span + 7) & ~7ull;
+  span = (span + span_align - 1) & ~(span_align - 1);
   if (S == 1) ss = span;
   if (H == 1) sh = span;
   if (B == 1) sb = span;
@@ -38,15 +38,41 @@ inline int make_head_tmap(CUtensorMap* out, HeadMapInfo* info, const TrnHeadTens
   for (int i = 0; i < 3; ++i)
     for (int j = i + 1; j < 3; ++j)
       if (dm[j].stride < dm[i].stride) { Dim tmp = dm[i]; dm[i] = dm[j]; dm[j] = tmp; }
-  uint64_t dims[4] = {static_cast<uint64_t>(D), dm[0].extent, dm[1].extent, dm[2].extent};
-  uint64_t strides[4] = {1, dm[0].stride, dm[1].stride, dm[2].stride};
-  uint32_t box[4] = {64u, dm[0].box, dm[1].box, dm[2].box};
+  dims[0] = static_cast<uint64_t>(D);
+  strides[0] = 1;
   for (int i = 0; i < 3; ++i) {
+    dims[i + 1] = dm[i].extent;
+    strides[i + 1] = dm[i].stride;
+    box[i + 1] = dm[i].box;
     if (dm[i].which == 0) info->pos_s = i + 1;
     if (dm[i].which == 1) info->pos_h = i + 1;
     if (dm[i].which == 2) info->pos_b = i + 1;
   }
+  return TRN_OK;
+}
+
+// Tile = `box_rows` positions x 64 head_dim elements of one (b, h).
+inline int make_head_tmap(CUtensorMap* out, HeadMapInfo* info, const TrnHeadTensor& t, int S, int H, int B, int D,
+                          uint32_t box_rows) {
+  if (t.ptr == nullptr) return TRN_E_NULL;
+  if (t.stride_s < 0 || t.stride_h < 0 || t.stride_b < 0) return TRN_E_SHAPE;
+  uint64_t dims[4], strides[4];
+  uint32_t box[4];
+  const int rc = order_head_dims(info, t, S, H, B, D, box_rows, 8, dims, strides, box);
+  if (rc != TRN_OK) return rc;
+  box[0] = 64u;
   return make_tmap_16bit(out, t.ptr, 4, dims, strides, box);
+}
+
+// Tile = `box_rows` positions x all D 8-bit codes of one (b, h): rows of 128 or 64 bytes, swizzled over as many bytes
+inline int make_code_tmap(CUtensorMap* out, HeadMapInfo* info, const TrnHeadTensor& t, int S, int H, int B, int D,
+                          uint32_t box_rows) {
+  uint64_t dims[4], strides[4];
+  uint32_t box[4];
+  const int rc = order_head_dims(info, t, S, H, B, D, box_rows, 16, dims, strides, box);
+  if (rc != TRN_OK) return rc;
+  box[0] = static_cast<uint32_t>(D);
+  return make_tmap_8bit(out, t.ptr, 4, dims, strides, box, D == 128);
 }
 
 // load one [rows x 64] tile: head_dim offset d0, position s0 of (b, h)

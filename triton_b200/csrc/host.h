@@ -39,6 +39,10 @@ int get_device_state(DeviceState** out);
 int make_tmap_16bit(CUtensorMap* out, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
                     const uint32_t* box);
 
+// The same over a tensor of bytes; rows of box[0] bytes, swizzled over 128 (swizzle128) or 64 bytes.
+int make_tmap_8bit(CUtensorMap* out, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
+                   const uint32_t* box, bool swizzle128);
+
 // opts a kernel in to `bytes` of dynamic shared memory, once per (kernel, device)
 int ensure_dyn_smem(const void* kernel, int bytes, int device);
 
@@ -106,6 +110,16 @@ extern thread_local int tls_attn_split_override;
 size_t block_workspace_required(const TrnBlockArgs& a);
 int launch_colstats(const TrnColStatsArgs& a, cudaStream_t st, const DeviceState& ds);
 int launch_topk(const TrnTopkArgs& a, cudaStream_t st, const DeviceState& ds);
+// the four operators of the 8-bit cache: check_* judges the arguments (no CUDA call), launch_* relies on it
+int check_cache_append(const TrnCacheAppendArgs& a);
+int check_cache_read(const TrnCacheReadArgs& a);
+int check_cache_evict(const TrnCacheEvictArgs& a);
+int check_attention_q8(const TrnAttnQ8Args& a);
+int launch_cache_append(const TrnCacheAppendArgs& a, cudaStream_t st);
+int launch_cache_read(const TrnCacheReadArgs& a, cudaStream_t st);
+int launch_cache_evict(const TrnCacheEvictArgs& a, cudaStream_t st, const DeviceState& ds);
+int launch_attention_q8(const TrnAttnQ8Args& a, cudaStream_t st, const DeviceState& ds);
+size_t attention_q8_workspace(const TrnAttnQ8Args& a);
 int launch_convert(const void* src, void* dst, long long n, int dtype16, int to_fp32, cudaStream_t st,
                    const DeviceState& ds);
 

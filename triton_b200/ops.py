@@ -321,6 +321,256 @@ class BlockPlan:
         L.check(self._lib.trinity_attn_block_host(C.byref(h), _stream()))
 
 
+class CacheQ8:
+    """A key/value cache of e4m3 codes with one fp32 scale for every ``block`` positions of a kv head (TrnCacheQ8 in
+    include/trinity_b200.h).  ``k``, ``v``: float8_e4m3fn tensors in ``layout`` ("bhsd", "bshd", "hsd", "shd"); ``k_scale``,
+    ``v_scale``: float32 tensors of the same layout without the last dim, blocks in the place of positions, e.g.
+    [B, Hkv, ceil(S / block)] for "bhsd"."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, *, block: int,
+                 layout: str = "bhsd"):
+        if block not in (16, 32, 64, 128):
+            raise ValueError("a scale covers 16, 32, 64 or 128 positions")
+        for t in (k, v):
+            if t.dtype != torch.float8_e4m3fn:
+                raise TypeError(f"an 8-bit cache holds float8_e4m3fn codes, got {t.dtype}")
+        self.k, self.v = as_bshd(k, layout), as_bshd(v, layout)
+        self.k_scale, self.v_scale = (as_bshd(t.unsqueeze(-1), layout).squeeze(-1) for t in (k_scale, v_scale))
+        self.B, self.S, self.Hkv, self.D = self.k.shape
+        self.block = block
+        if self.v.shape != self.k.shape:
+            raise ValueError("keys and values of a cache must have the same shape")
+        for t in (self.k_scale, self.v_scale):
+            if t.dtype != torch.float32 or t.shape != (self.B, -(-self.S // block), self.Hkv):
+                raise ValueError("scales must be float32, one for each batch item, block of positions and kv head")
+
+    @classmethod
+    def empty(cls, B: int, S: int, Hkv: int, D: int, *, block: int = 64, layout: str = "bhsd", device=None) -> "CacheQ8":
+        """A cache that holds nothing yet, room for ``S`` positions of each sequence."""
+        dims = {"b": B, "h": Hkv, "s": S, "d": D}
+        device = torch.device("cuda") if device is None else device
+        if layout not in _LAYOUT_PERM or ("b" not in layout and B != 1):
+            raise ValueError(f"layout {layout!r} does not fit B = {B}")
+        code = [torch.zeros([dims[x] for x in layout], dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+                for _ in range(2)]
+        dims["s"] = -(-S // block)
+        scale = [torch.zeros([dims[x] for x in layout[:-1]], dtype=torch.float32, device=device) for _ in range(2)]
+        return cls(*code, *scale, block=block, layout=layout)
+
+    def tensors(self):
+        return [self.k, self.v, self.k_scale, self.v_scale]
+
+    def c(self) -> L.TrnCacheQ8:
+        return L.TrnCacheQ8(_head_tensor(self.k), _head_tensor(self.v), _head_tensor(self.k_scale),
+                            _head_tensor(self.v_scale), self.S, self.block)
+
+
+def _one_device(*ts: Optional[torch.Tensor]) -> None:
+    ts = [t for t in ts if t is not None]
+    _need_cuda(*ts)
+    if any(t.device != ts[0].device for t in ts):
+        raise ValueError("all tensors of one call must be on the same device")
+
+
+def _set_kv_len(a, kv_len, B: int, room: int) -> list:
+    """Fills kv_len / kv_len_all of an argument struct; a tensor is returned to be kept alive."""
+    if isinstance(kv_len, torch.Tensor):
+        if kv_len.dtype != torch.int32 or kv_len.numel() != B or not kv_len.is_contiguous():
+            raise ValueError("kv_len must be an int or a contiguous int32 tensor with one entry per batch item")
+        a.kv_len = kv_len.data_ptr()
+        return [kv_len]
+    if not 0 <= int(kv_len) <= room:
+        raise ValueError(f"kv_len = {kv_len} does not fit a cache with room for {room} positions")
+    a.kv_len_all = int(kv_len)
+    return []
+
+
+class _BoundCall:
+    """Arguments of one C-ABI call bound once (pointers, strides, workspace), launched many times on the current stream of
+    the tensors' device.  Construction validates and allocates; ``run()`` only launches, so it can be captured in a CUDA graph.
+    The tensors (lengths included) are read and written in place at every run; two runs of ONE plan that overlap on the GPU
+    (different streams) share its workspace and outputs and must be ordered by the caller."""
+
+    def _bind(self, name: str, args, keep) -> None:
+        self._keep = [t for t in keep if t is not None]
+        _one_device(*self._keep)
+        self.device = self._keep[0].device
+        self.args = args
+        self._ref = C.byref(args)
+        self._fn = getattr(L.load(), name)
+
+    def run(self) -> None:
+        if torch.cuda.current_device() == self.device.index:
+            rc = self._fn(self._ref, _stream())
+        else:
+            with torch.cuda.device(self.device):
+                rc = self._fn(self._ref, _stream())
+        if rc != 0:
+            L.check(rc)
+
+
+class CacheAppendPlan(_BoundCall):
+    """Rows [kv_len, kv_len + M) of every sequence of ``cache`` become ``k`` / ``v`` ((b, s, h, d) views of M 16-bit rows);
+    ``kv_len`` (int, or int32 tensor on the device) counts what the cache holds BEFORE the call and is not changed.  Rows
+    that would fall behind the cache's room are dropped.  See trinity_cache_append for the scales."""
+
+    def __init__(self, cache: CacheQ8, k: torch.Tensor, v: torch.Tensor, *, kv_len):
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.stride(3) != 1 or v.stride(3) != 1:
+            raise ValueError("k and v must be (b, s, h, d) views of one shape and dtype with contiguous head_dim")
+        B, M, Hkv, D = k.shape
+        if (B, Hkv, D) != (cache.B, cache.Hkv, cache.D):
+            raise ValueError("k and v do not fit the cache")
+        a = L.TrnCacheAppendArgs()
+        a.cache, a.k_new, a.v_new = cache.c(), _head_tensor(k), _head_tensor(v)
+        a.B, a.M, a.Hkv, a.D, a.dtype = B, M, Hkv, D, _dtype_code(k)
+        keep = _set_kv_len(a, kv_len, B, cache.S - M if not isinstance(kv_len, torch.Tensor) else cache.S)
+        self._bind("trinity_cache_append", a, keep + cache.tensors() + [k, v])
+
+
+class CacheReadPlan(_BoundCall):
+    """code * scale of the first ``kv_len`` positions of every sequence, as 16-bit (b, s, h, d) tensors."""
+
+    def __init__(self, cache: CacheQ8, k_out: torch.Tensor, v_out: torch.Tensor, *, kv_len):
+        if k_out.dim() != 4 or k_out.shape != v_out.shape or k_out.dtype != v_out.dtype:
+            raise ValueError("k_out and v_out must be (b, s, h, d) views of one shape and dtype")
+        if k_out.stride(3) != 1 or v_out.stride(3) != 1:
+            raise ValueError("k_out and v_out need a contiguous head_dim")
+        B, S, Hkv, D = k_out.shape
+        if (B, Hkv, D) != (cache.B, cache.Hkv, cache.D):
+            raise ValueError("k_out and v_out do not fit the cache")
+        a = L.TrnCacheReadArgs()
+        a.cache, a.k_out, a.v_out, a.S_out = cache.c(), _head_tensor(k_out), _head_tensor(v_out), S
+        a.B, a.Hkv, a.D, a.dtype = B, Hkv, D, _dtype_code(k_out)
+        keep = _set_kv_len(a, kv_len, B, min(S, cache.S) if not isinstance(kv_len, torch.Tensor) else S)
+        self._bind("trinity_cache_read", a, keep + cache.tensors() + [k_out, v_out])
+
+
+class AttentionQ8Plan(_BoundCall):
+    """o = softmax(scale * q k^T) v over the first ``kv_len`` positions of an 8-bit cache; causal: query i of M sees positions
+    up to kv_len - M + i; a row that sees nothing is 0.  q, o: (b, s, h, d) views.  ``lse`` [B, Hq, M] fp32 (base 2).
+    ``weight`` [B, Hkv, S or more] fp32 receives every position's attention weight, summed over the queries (at most 16) and
+    the query heads of the kv head (``weight_add``: is increased by it): what CacheEvictPlan selects by.
+    ``workspace``: a uint8 tensor of attention_q8_workspace_bytes(...) bytes; allocated here when not given."""
+
+    def __init__(self, q: torch.Tensor, cache: CacheQ8, o: torch.Tensor, *, kv_len, causal: bool = True,
+                 scale: Optional[float] = None, lse: Optional[torch.Tensor] = None, weight: Optional[torch.Tensor] = None,
+                 weight_add: bool = False, workspace: Optional[torch.Tensor] = None):
+        if q.dim() != 4 or q.shape != o.shape or q.dtype != o.dtype or q.stride(3) != 1 or o.stride(3) != 1:
+            raise ValueError("q and o must be (b, s, h, d) views of one shape and dtype with contiguous head_dim")
+        B, M, Hq, D = q.shape
+        if (B, D) != (cache.B, cache.D) or Hq % cache.Hkv != 0:
+            raise ValueError("q does not fit the cache")
+        a = L.TrnAttnQ8Args()
+        a.q, a.cache, a.o = _head_tensor(q), cache.c(), _head_tensor(o)
+        a.B, a.M, a.Hq, a.Hkv, a.D, a.dtype = B, M, Hq, cache.Hkv, D, _dtype_code(q)
+        a.causal, a.scale = int(causal), default_scale(D) if scale is None else float(scale)
+        if lse is not None:
+            if lse.dtype != torch.float32 or lse.shape != (B, Hq, M) or not lse.is_contiguous():
+                raise ValueError("lse must be a contiguous float32 [B, Hq, M] tensor")
+            a.lse = lse.data_ptr()
+        if weight is not None:
+            if weight.dtype != torch.float32 or weight.dim() != 3 or weight.shape[:2] != (B, cache.Hkv) or \
+                    weight.shape[2] < cache.S or (weight.shape[2] > 1 and weight.stride(2) != 1):
+                raise ValueError("weight must be float32 [B, Hkv, positions of the cache] with contiguous positions")
+            if M > 16:
+                raise ValueError("weight takes at most 16 queries; attn_colstats sums those of a prompt")
+            a.weight, a.weight_stride_b, a.weight_stride_h = weight.data_ptr(), weight.stride(0), weight.stride(1)
+            a.weight_add = int(weight_add)
+        keep = _set_kv_len(a, kv_len, B, cache.S)
+        if workspace is None:
+            nbytes = L.load().trinity_attention_q8_workspace(C.byref(a))
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+        if workspace is not None:
+            if not workspace.is_contiguous():
+                raise ValueError("workspace must be contiguous")
+            a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        self._bind("trinity_attention_q8", a, keep + cache.tensors() + [q, o, lse, weight, workspace])
+
+
+def attention_q8_workspace_bytes(B: int, M: int, Hq: int, Hkv: int, D: int, S: int, *, causal: bool = True,
+                                 weight: bool = False) -> int:
+    """Scratch of trinity_attention_q8 for this shape over a cache with room for S positions."""
+    a = L.TrnAttnQ8Args()
+    a.B, a.M, a.Hq, a.Hkv, a.D, a.cache.S, a.causal = B, M, Hq, Hkv, D, S, int(causal)
+    a.weight = 1 if weight else None
+    return int(L.load().trinity_attention_q8_workspace(C.byref(a)))
+
+
+class CacheEvictPlan(_BoundCall):
+    """Of the ``kv_len`` positions of every (batch item, kv head) the ``keep`` that stay move, in order, from ``src`` to ``dst``:
+    the first ``first``, the last ``recent``, and of the others those of the largest ``scores`` [B, Hs, S or more] fp32 (Hs a
+    multiple of Hkv: the heads of a group are summed; equal scores by the lower position).  ``src``, ``dst``: CacheQ8 of one
+    block size, or (k, v) pairs of 16-bit (b, s, h, d) views of one dtype; they must not overlap.
+    ``idx`` [B, Hkv, keep] int32: the positions kept, ascending, then -1.  ``scores_out`` [B, Hkv, keep] fp32: their scores,
+    then 0 (the accumulators of the cache they moved to).  ``kv_len_out`` [B] int32: min(kv_len, keep)."""
+
+    def __init__(self, src, dst, scores: torch.Tensor, *, kv_len, keep: int, recent: int = 0, first: int = 0,
+                 idx: Optional[torch.Tensor] = None, scores_out: Optional[torch.Tensor] = None,
+                 kv_len_out: Optional[torch.Tensor] = None):
+        a = L.TrnCacheEvictArgs()
+        views = []
+        for cache, name in ((src, "src"), (dst, "dst")):
+            if isinstance(cache, CacheQ8):
+                setattr(a, name, cache.c())
+                views.append((cache.k, cache.v))
+            else:
+                k, v = cache
+                if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.stride(3) != 1 or v.stride(3) != 1:
+                    raise ValueError("a 16-bit cache is a (k, v) pair of (b, s, h, d) views of one shape and dtype")
+                _dtype_code(k)
+                setattr(a, name, L.TrnCacheQ8(_head_tensor(k), _head_tensor(v), _head_tensor(None), _head_tensor(None),
+                                              k.shape[1], 0))
+                views.append((k, v))
+        (k, _), (k_to, _) = views
+        B, S, Hkv, D = k.shape
+        if isinstance(src, CacheQ8) != isinstance(dst, CacheQ8) or a.src.block != a.dst.block or k.dtype != k_to.dtype:
+            raise ValueError("src and dst must be caches of one kind (and block size)")
+        if (k_to.shape[0], k_to.shape[2], k_to.shape[3]) != (B, Hkv, D) or k_to.shape[1] < keep:
+            raise ValueError("dst must have src's batch, heads and head_dim, and room for keep positions")
+        if keep <= 0 or recent < 0 or first < 0 or recent + first > keep:
+            raise ValueError("keep must be positive and hold first + recent positions")
+        if scores.dtype != torch.float32 or scores.dim() != 3 or scores.shape[0] != B or scores.shape[1] % Hkv != 0 or \
+                scores.shape[1] == 0 or scores.shape[2] < S or (scores.shape[2] > 1 and scores.stride(2) != 1):
+            raise ValueError("scores must be float32 [B, a multiple of Hkv heads, positions of src], positions contiguous")
+        idx = torch.empty(B, Hkv, keep, dtype=torch.int32, device=k.device) if idx is None else idx
+        for t, dt, shape in ((idx, torch.int32, (B, Hkv, keep)), (scores_out, torch.float32, (B, Hkv, keep)),
+                             (kv_len_out, torch.int32, (B,))):
+            if t is not None and (t.dtype != dt or t.shape != shape or not t.is_contiguous()):
+                raise ValueError(f"expected a contiguous {dt} tensor of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+        self.idx = idx
+        a.scores, a.score_stride_b, a.score_stride_h, a.Hs = scores.data_ptr(), scores.stride(0), scores.stride(1), scores.shape[1]
+        a.idx, a.scores_out, a.kv_len_out = idx.data_ptr(), _ptr(scores_out), _ptr(kv_len_out)
+        a.B, a.Hkv, a.D, a.keep, a.recent, a.first = B, Hkv, D, keep, recent, first
+        keep_alive = _set_kv_len(a, kv_len, B, S)
+        for cache, pair in zip((src, dst), views):
+            keep_alive += cache.tensors() if isinstance(cache, CacheQ8) else list(pair)
+        self._bind("trinity_cache_evict", a, keep_alive + [scores, idx, scores_out, kv_len_out])
+
+
+def cache_append(cache: CacheQ8, k: torch.Tensor, v: torch.Tensor, *, kv_len) -> None:
+    """One CacheAppendPlan call."""
+    CacheAppendPlan(cache, k, v, kv_len=kv_len).run()
+
+
+def cache_read(cache: CacheQ8, k_out: torch.Tensor, v_out: torch.Tensor, *, kv_len) -> None:
+    """One CacheReadPlan call."""
+    CacheReadPlan(cache, k_out, v_out, kv_len=kv_len).run()
+
+
+def attention_q8(q: torch.Tensor, cache: CacheQ8, o: Optional[torch.Tensor] = None, **kw) -> torch.Tensor:
+    """One AttentionQ8Plan call (its keyword arguments); returns o."""
+    o = torch.empty(q.shape, dtype=q.dtype, device=q.device) if o is None else o
+    AttentionQ8Plan(q, cache, o, **kw).run()
+    return o
+
+
+def cache_evict(src, dst, scores: torch.Tensor, **kw) -> torch.Tensor:
+    """One CacheEvictPlan call (its keyword arguments); returns idx."""
+    plan = CacheEvictPlan(src, dst, scores, **kw)
+    plan.run()
+    return plan.idx
+
+
 def convert(src: torch.Tensor, dst: torch.Tensor) -> torch.Tensor:
     """fp32 -> bf16/fp16 (rounding) or bf16/fp16 -> fp32 (widening) of contiguous tensors of equal numel."""
     _need_cuda(src, dst)

@@ -94,11 +94,11 @@ def test_caches_refused(lib, make, fn, change, code):
     (_attend, "trinity_attention_q8", dict(q__ptr=None), NULL),
     (_attend, "trinity_attention_q8", dict(o__ptr=(1 << 32) + 4), ALIGN),
     (_attend, "trinity_attention_q8", dict(o__stride_h=0), SHAPE),
-    (_attend, "trinity_attention_q8", dict(weight=5 << 32, weight_stride_b=512, weight_stride_h=256), WORKSPACE),
+    (_attend, "trinity_attention_q8", dict(weight=5 << 32, weight_stride_b=512, weight_stride_h=256, cache__S=100000, kv_len_all=100000), WORKSPACE),
     (_attend, "trinity_attention_q8", dict(weight=5 << 32, weight_stride_b=512, weight_stride_h=0), SHAPE),
     (_attend, "trinity_attention_q8", dict(weight=5 << 32, weight_stride_b=512, weight_stride_h=256, M=17), SHAPE),
-    (_attend, "trinity_attention_q8", dict(workspace=(6 << 32) + 16, workspace_bytes=1 << 40, cache__S=100000), WORKSPACE),
-    (_attend, "trinity_attention_q8", dict(workspace=6 << 32, workspace_bytes=100, cache__S=100000), WORKSPACE),
+    (_attend, "trinity_attention_q8", dict(workspace=(6 << 32) + 16, workspace_bytes=1 << 40, cache__S=100000, kv_len_all=100000), WORKSPACE),
+    (_attend, "trinity_attention_q8", dict(workspace=6 << 32, workspace_bytes=100, cache__S=100000, kv_len_all=100000), WORKSPACE),
     (_evict, "trinity_cache_evict", dict(scores=None), NULL),
     (_evict, "trinity_cache_evict", dict(idx=None), NULL),
     (_evict, "trinity_cache_evict", dict(dst__block=64), VARIANT),

@@ -13,12 +13,15 @@
 // fp16's subnormals.  bf16 outputs take P' as one fp16 (error 2^-12 against the output's 2^-9); fp16 outputs take it as
 // hi + lo, since one part alone would err as much as the output's own rounding.
 //
-// This kernel is for few query rows per kv head: a CTA of four warps owns 16 of the M * Hq / Hkv rows of a (b, kv head) and
-// 1 / n_splits of its positions; each warp walks its quarter in chunks of 32 positions through its own ring of TMA
-// tiles.  It is bound by memory (2 * D bytes per position and kv head): the ring keeps 3 x 8 KB per warp in flight, and
-// codes go from shared memory to registers as the 16 bytes a lane needs (the order of the d axis inside a product and of the
-// columns inside the output is free, so the m16n8k16 fragments are picked such that 128-bit reads have no bank conflicts
-// under the TMA swizzle: K lane (g, t) reads 16-byte units 2t and 2t + 1 of key g, V lane (g, t) unit g of keys 2t, 2t + 1).
+// This kernel is for few query rows per kv head: a CTA of four warps owns up to 8 NT of the M * Hq / Hkv rows of a (b, kv head)
+// and 1 / n_splits of its positions; each warp walks its quarter in chunks of 32 positions through its own ring of TMA
+// tiles.  Both products are taken transposed, s^T = k q^T and o^T = v^T p^T, so that positions and head_dim fill the
+// 16-row side of m16n8k16 and eight query rows the 8-column side: a decode step of 4 to 8 heads per kv head wastes
+// little.  p^T becomes an operand with one 8x8 transposition (movmatrix) per 8 positions.  Codes go from shared memory to
+// registers as the 16 bytes a lane needs: the order of the d axis inside a product and of the rows inside the output is
+// free, so the fragments are picked such that the reads have no bank conflicts under the TMA swizzle (k: lane (g, t)
+// reads units 2t and 2t + 1 of positions g, g + 8; v: unit g of positions 2t, 2t + 1).  The running maximum is shared by a
+// row's lanes and only raised when some score passes it by 2^3, so most chunks need no reduction across lanes.
 // Partial results of the splits are merged by a second small kernel, which also sums the per-position weights from the
 // scores kept in the workspace.  Rows, splits and sums are taken in a fixed order: bitwise reproducible.
 //
@@ -37,22 +40,37 @@ namespace {
 constexpr int kQ8Warps = 4;
 constexpr int kQ8Threads = 32 * kQ8Warps;
 constexpr int kQ8Keys = 32;                    // positions per chunk
-constexpr int kQ8Stages = 3;
-constexpr int kQ8Rows = 16;
+constexpr int kQ8Stages = 2;
 constexpr float kQ8PBias = 12.f;               // log2 of the factor P' carries into the product
+constexpr float kQ8Slack = 3.f;                // log2 of how far a score may pass the running maximum (2^15 fits fp16)
 constexpr float kMinVScale = 7.888609052210118e-31f;   // 2^-100: smaller scales (a block of zeros) count as this
-constexpr int kQ8TargetCtas = 2;               // resident CTAs per SM (registers and shared memory)
+constexpr int kQ8MaxCluster = 8;
+constexpr int kQ8Keep = 4;                     // chunks a warp of a cluster takes at most
+constexpr int kQ8TargetCtas = 3;               // resident CTAs per SM (shared memory)
 
-template <int D>
+// rows a CTA takes: 8, 16 or (head_dim 64, where the output leaves registers for it) 32
+__host__ __device__ constexpr int q8_max_tiles(int D) { return D == 64 ? 4 : 2; }
+
+template <int D, int NT>
 struct Q8Smem {
+  static constexpr int kRows = 8 * NT;
   static constexpr int kTile = kQ8Keys * D;                        // bytes of k or v of a chunk
   static constexpr int kWarpRing = kQ8Stages * 2 * kTile;
   static constexpr int kRing = kQ8Warps * kWarpRing;
   static constexpr int kRow = D + 4;                               // o | max, sum  of a warp's partial result
-  static constexpr int kPart = kQ8Warps * kQ8Rows * kRow * 4;      // overlays the ring after the key loop
-  static constexpr int kBody = kRing > kPart ? kRing : kPart;
+  static constexpr int kPart = kQ8Warps * kRows * kRow * 4;        // overlays the ring after the key loop
+  static constexpr int kTPR = kQ8Threads / kRows;                  // threads and columns a thread of the merge
+  static constexpr int kCW = D / kTPR;
+  static constexpr int kMine = kPart;                              // a CTA's merged result, read by its cluster
+  static constexpr int kEnd = kMine + kRows * kRow * 4;
+  static constexpr int kBody = kRing > kEnd ? kRing : kEnd;
   static constexpr int kBars = kBody;
   static constexpr int kTotal = kBars + 128 + 1024;                // + slack to align the base to 1024 bytes
+  // launches of clusters that also sum weights: [warp][row][kKeptPitch] scores.  The pitch spreads a warp's stores (eight
+  // positions of four rows two apart) over all banks.
+  static constexpr int kKept = kBars + 128;
+  static constexpr int kKeptPitch = kQ8Keep * kQ8Keys + 4;
+  static constexpr int kTotalKept = kTotal + kQ8Warps * kRows * kKeptPitch * 4;
 };
 
 struct Q8Params {
@@ -62,13 +80,14 @@ struct Q8Params {
   KvLen len;
   float* lse;
   int B, M, Hq, Hkv, G, R;                     // R = M * G rows per (b, kv head): row r = query r / G, head r % G
-  int tiles;                                   // 16-row tiles per (b, kv head)
+  int tiles, tile_rows;                        // row tiles per (b, kv head), rows of one
   int causal;
   float scale_log2;
   int shift;                                   // log2(block)
-  int n_splits;
-  float* part_o;                               // [n_splits][units][16][D], units = B * Hkv * tiles
-  float2* part_ml;                             // [n_splits][units][16]
+  int ctas;                                    // CTAs the chunks are dealt out to; 0: a CTA per unit, nothing divided
+  float* part_o;                               // [units + ctas][tile_rows][D], units = B * Hkv * tiles
+  float2* part_ml;                             // [units + ctas][tile_rows]; without division [units][tile_rows] or NULL
+  int2* pieces;                                // [units] CTAs of a unit's first and last piece
   float* scores;                               // [B * Hkv][R][pitch], log2 domain, or NULL
   long long pitch;
   float* weight;
@@ -106,465 +125,770 @@ __device__ __forceinline__ int q8_key(int c) {
   else return (c & 4) + ((0x2130 >> ((c & 3) * 4)) & 3) ;
 }
 
-// HILO: P' enters the product as two fp16 parts.
-template <typename T, int D, bool HILO>
-__global__ void __launch_bounds__(kQ8Threads)
-attn_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-               const __grid_constant__ Q8Params p) {
-  using SM = Q8Smem<D>;
-  constexpr int KS = D / 16;                   // k steps of q k^T
-  constexpr int NB = D / 8;                    // 8-column blocks of o
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+// transposes an 8x8 matrix of 16-bit values held two to a lane
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+// log2 and reciprocal of a scale: exact for powers of two
+__device__ __forceinline__ void scale_log_inv(float s, float& lg, float& inv) {
+  const uint32_t u = __float_as_uint(s);
+  if ((u & 0x7fffffu) == 0u && u - (1u << 23) < (252u << 23)) {       // 2^-126 .. 2^125
+    lg = static_cast<float>(static_cast<int>(u >> 23) - 127);
+    inv = __uint_as_float((254u << 23) - u);
+  } else {
+    lg = log2f(s);
+    inv = 1.0f / s;
+  }
+}
+
+// ---- who does what.  A unit is a (b, kv head, row tile) with the chunks its sequence holds (one where it holds none, to write
+// the empty rows; a tile whose rows do not see the last ones skips them).  All units' chunks, in order, are dealt out in equal
+// contiguous shares, so a CTA's share may end one unit and begin others, and a unit lies on CTAs [first, last]: pieces.
+// Each new piece begins a new unit, a new CTA or both, so slot = unit + CTA numbers the pieces' partial results, a
+// unit's side by side.
+__device__ __forceinline__ int last_seen(const Q8Params& p, int n, int r) {      // by row r of a (b, kv head); -1: nothing
+  return p.causal ? max(n - p.M + r / p.G, -1) : n - 1;
+}
+__device__ __forceinline__ int chunks_of(int n) { return max((n + kQ8Keys - 1) / kQ8Keys, 1); }
+// chunks of the sequences before b and of all, for one (kv head, row tile) (a whole warp, same arguments)
+__device__ __forceinline__ int2 chunks_before(const Q8Params& p, int b) {
+  int x = 0, y = 0;
+  for (int i = threadIdx.x & 31; i < p.B; i += 32) {
+    const int c = chunks_of(p.len(i));
+    y += c;
+    if (i < b) x += c;
+  }
+  return make_int2(static_cast<int>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(x))),
+                   static_cast<int>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(y))));
+}
+__device__ __forceinline__ unsigned share_of(const Q8Params& p, int all) {       // chunks of one CTA, at least one a warp
+  return max((static_cast<unsigned>(all) * p.Hkv * p.tiles + p.ctas - 1) / p.ctas, static_cast<unsigned>(kQ8Warps));
+}
+// What a warp of a CTA has to do for one piece of a unit.
+struct Q8Piece {
+  int b, h, n, r0, rows;                       // sequence, kv head, its length; first row and rows of the tile
+  int lim_min, lim_max;                        // last position that the tile's first / last row sees
+  int chunk0, n_chunks;                        // of this warp
+  int loaded;                                  // chunks this warp's ring has taken before: stage and parity go on
+  float* kept;                                 // where row 0 keeps its scores (log2 domain), or NULL
+  long long kept_pitch;
+  int kept_from;                               // the position that lies at kept[0]
+  __device__ __forceinline__ int last_of(const Q8Params& p, int r) const { return r >= rows ? -1 : last_seen(p, n, r0 + r); }
+};
+// the tile's rows and this warp's quarter of chunks [skip, skip + many) of unit (b, h, tile): those that some row sees
+__device__ __forceinline__ Q8Piece piece_of(const Q8Params& p, int b, int h, int tile, int skip, int many, int warp) {
+  Q8Piece w{};
+  w.b = b; w.h = h; w.n = p.len(b);
+  w.r0 = tile * p.tile_rows;
+  w.rows = min(p.tile_rows, p.R - w.r0);
+  w.lim_min = w.last_of(p, 0);
+  w.lim_max = w.last_of(p, w.rows - 1);
+  const int seen = max(min(skip + many, (w.lim_max + kQ8Keys) / kQ8Keys) - skip, 0);
+  w.chunk0 = skip + seen * warp / kQ8Warps;
+  w.n_chunks = skip + seen * (warp + 1) / kQ8Warps - w.chunk0;
+  return w;
+}
+
+// One piece: every warp walks its chunks, then the warps' results are merged.  Thread (row, column group) of the CTA is left
+// with its row's running maximum, sum and CW columns of the unnormalised output.  HILO: P' enters the product as two
+// fp16 parts.  All threads of the CTA; the rings are empty and shared memory is free for the next piece's tiles after a
+// proxy fence and a barrier.
+template <typename T, int D, int NT, bool HILO>
+__device__ __forceinline__ void q8_piece(const Q8Params& p, const CUtensorMap& tm_k, const CUtensorMap& tm_v, const Q8Piece& w,
+                                         uint8_t* gen, uint32_t base, int* nan_from, const Ctl& ctl,
+                                         float (&acc)[Q8Smem<D, NT>::kCW], float& mx, float& tot) {
+  using SM = Q8Smem<D, NT>;
+  constexpr int ROWS = SM::kRows, CW = SM::kCW;
+  constexpr int KS = D / 16;                   // k steps of k q^T
+  constexpr int DT = D / 16;                   // 16-row blocks of o^T
   constexpr int KU = D / 64;                   // 16-byte units a lane reads per key row
-  extern __shared__ uint8_t q8_smem_raw[];
-  __shared__ int nan_from[D];                  // first position whose v code of this column is NaN, in edge chunks
-  __shared__ int s_abort;
-  const uint32_t base = (smem_u32(q8_smem_raw) + 1023u) & ~1023u;
-  uint8_t* gen = q8_smem_raw + (base - smem_u32(q8_smem_raw));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const uint32_t bars = base + SM::kBars + warp * kQ8Stages * 8;
-  Ctl ctl{p.status, &s_abort};
-  if (lane == 0) {
-    for (int s = 0; s < kQ8Stages; ++s) mbar_init(bars + 8 * s, 1);
-    fence_mbar_init();
-  }
-  if (threadIdx.x == 0) s_abort = 0;
-  for (int i = threadIdx.x; i < D; i += kQ8Threads) nan_from[i] = 0x7fffffff;
-  __syncthreads();
-  griddep_wait();                              // q, the codes and the lengths may come from the launch before
-  griddep_launch();
-  if (*reinterpret_cast<volatile int*>(p.status) != 0) return;
-
-  const int split = static_cast<int>(blockIdx.x) % p.n_splits;
-  const int unit = static_cast<int>(blockIdx.x) / p.n_splits;
-  const int tile = unit % p.tiles, bh = unit / p.tiles;
-  const int b = bh / p.Hkv, h = bh % p.Hkv;
-  const int n = p.len(b);
-  const int r0 = tile * kQ8Rows, rows = min(kQ8Rows, p.R - r0);
-  // rows g and g + 8: their last visible position (-1: none)
-  auto last_of = [&](int r) { return r >= rows ? -1 : p.causal ? max(n - p.M + (r0 + r) / p.G, -1) : n - 1; };
-  const int lim_lo = last_of(g), lim_hi = last_of(g + 8);
-  const int lim_min = last_of(0), lim_max = last_of(rows - 1);
-
-  // ---- q fragments as fp16 times 2^(14 - exponent of the row's largest element); k step ks = 4 h + j of lane t holds
-  // d = (KU t + h) 16 + 4 j + {0, 1} in registers 0 / 1 and + {2, 3} in 2 / 3
-  uint32_t qa[KS][4];
-  float c_lo = 0.f, c_hi = 0.f;                // scale * log2 e / row factor
-  {
-    auto row_ptr = [&](int r) {
-      const int rr = r0 + min(r, rows - 1);
-      return static_cast<const T*>(p.q.ptr) + b * p.q.stride_b + static_cast<long long>(rr / p.G) * p.q.stride_s +
-             static_cast<long long>(h * p.G + rr % p.G) * p.q.stride_h + t * KU * 16;
-    };
+  int lim[NT][2];                              // last position seen of this lane's columns: rows 8 nt + 2t, + 1
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const T* src = row_ptr(g + 8 * half);
-      uint4 x[2 * KU];
+  for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int i = 0; i < 2 * KU; ++i) x[i] = *reinterpret_cast<const uint4*>(src + i * 8);
-      float f[KU * 16], amax = 0.f;
-      bool bad = false;
-#pragma unroll
-      for (int i = 0; i < 2 * KU; ++i) {
-        const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 v = Io<T>::unpack2(w[e]);
-          f[i * 8 + 2 * e] = v.x;
-          f[i * 8 + 2 * e + 1] = v.y;
-          bad = bad || !(fabsf(v.x) <= FLT_MAX) || !(fabsf(v.y) <= FLT_MAX);
-          amax = fmaxf(amax, fmaxf(fabsf(v.x), fabsf(v.y)));
-        }
-      }
-      float up = 1.f, down = 1.f;
-      if constexpr (Io<T>::kFmt == 1) {
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        const int e = max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -100);
-        up = exp2_int(14 - min(e, 127));
-        down = exp2_int(min(e, 127) - 14);
-      }
-      bad = (__ballot_sync(0xffffffffu, bad) >> (g * 4)) & 0xfu;
-      // a row with an infinite or NaN element: every score is infinite or NaN, and so is its softmax NaN
-      const float c = bad ? __uint_as_float(0x7fffffffu) : p.scale_log2 * down;
-      if (half == 0) c_lo = c; else c_hi = c;
-      const bool there = g + 8 * half < rows;
-#pragma unroll
-      for (int i = 0; i < KS; ++i) {
-        const int d = (i >> 2) * 16 + (i & 3) * 4;
-        const __half2 a = __floats2half2_rn(f[d] * up, f[d + 1] * up), c2 = __floats2half2_rn(f[d + 2] * up, f[d + 3] * up);
-        qa[i][half] = there ? *reinterpret_cast<const uint32_t*>(&a) : 0u;
-        qa[i][2 + half] = there ? *reinterpret_cast<const uint32_t*>(&c2) : 0u;
-      }
-    }
-  }
-
-  // ---- this warp's chunks: dealt out evenly to the warps of all splits
-  const int total = (lim_max + kQ8Keys) / kQ8Keys;                 // lim_max = -1: none
-  const int n_warps = kQ8Warps * p.n_splits, wi = split * kQ8Warps + warp;
-  const int chunk0 = static_cast<int>(static_cast<long long>(total) * wi / n_warps);
-  const int n_chunks = static_cast<int>(static_cast<long long>(total) * (wi + 1) / n_warps) - chunk0;
+    for (int e = 0; e < 2; ++e) lim[nt][e] = w.last_of(p, 8 * nt + 2 * t + e);
   const uint32_t ring = base + warp * SM::kWarpRing;
   auto k_tile = [&](int s) { return ring + s * 2 * SM::kTile; };
   auto load = [&](int c) {                                         // lane 0
-    const int s = c % kQ8Stages, key0 = (chunk0 + c) * kQ8Keys;
+    const int s = (w.loaded + c) % kQ8Stages, key0 = (w.chunk0 + c) * kQ8Keys;
     mbar_expect_tx(bars + 8 * s, 2 * SM::kTile);
-    tma_load_head_tile(k_tile(s), &tm_k, bars + 8 * s, p.ki, 0, key0, h, b);
-    tma_load_head_tile(k_tile(s) + SM::kTile, &tm_v, bars + 8 * s, p.vi, 0, key0, h, b);
+    tma_load_head_tile(k_tile(s), &tm_k, bars + 8 * s, p.ki, 0, key0, w.h, w.b);
+    tma_load_head_tile(k_tile(s) + SM::kTile, &tm_v, bars + 8 * s, p.vi, 0, key0, w.h, w.b);
   };
   if (lane == 0)
-    for (int c = 0; c < min(kQ8Stages, n_chunks); ++c) load(c);
+    for (int c = 0; c < min(kQ8Stages, w.n_chunks); ++c) load(c);
   // scales of a chunk: two halves of 16 positions (the same block unless block is 16)
   auto scales_of = [&](int c, float (&ks)[2], float (&vs)[2]) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int key = (chunk0 + c) * kQ8Keys + 16 * i;
-      const bool in = c < n_chunks && key <= lim_max;
-      ks[i] = in ? *p.ks.at(b, key >> p.shift, h) : 1.f;
-      const float v = in ? *p.vs.at(b, key >> p.shift, h) : 1.f;
-      vs[i] = v < kMinVScale ? kMinVScale : v;
+      const int key = (w.chunk0 + c) * kQ8Keys + 16 * i;
+      const bool in = c < w.n_chunks && key <= w.lim_max;
+      ks[i] = in ? *p.ks.at(w.b, key >> p.shift, w.h) : 1.f;
+      vs[i] = in ? *p.vs.at(w.b, key >> p.shift, w.h) : 1.f;
     }
   };
-
-  float oacc[NB][4];
-#pragma unroll
-  for (int i = 0; i < NB; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) oacc[i][j] = 0.f;
-  float m_lo = -INFINITY, m_hi = -INFINITY, l_lo = 0.f, l_hi = 0.f;
-  float* sc_lo = nullptr;
-  float* sc_hi = nullptr;
-  if (p.scores != nullptr) {
-    if (g < rows) sc_lo = p.scores + (static_cast<long long>(bh) * p.R + r0 + g) * p.pitch;
-    if (g + 8 < rows) sc_hi = p.scores + (static_cast<long long>(bh) * p.R + r0 + g + 8) * p.pitch;
-  }
   float ks_next[2], vs_next[2];
   scales_of(0, ks_next, vs_next);
+
+  // ---- q as the B operand: fp16 times 2^(14 - exponent of the row's largest element).  Column g of k step 4 u + j holds
+  // d = (KU t + u) 16 + 4 j + {0, 1} in register 0 and + {2, 3} in register 1
+  uint32_t qb[NT][KS][2];
+  float cq[NT][2];                             // scale * log2 e / row factor of this lane's columns
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = 8 * nt + g, rr = w.r0 + min(r, w.rows - 1);
+    const T* src = static_cast<const T*>(p.q.ptr) + w.b * p.q.stride_b + static_cast<long long>(rr / p.G) * p.q.stride_s +
+                   static_cast<long long>(w.h * p.G + rr % p.G) * p.q.stride_h + t * KU * 16;
+    uint4 x[2 * KU];
+#pragma unroll
+    for (int i = 0; i < 2 * KU; ++i) x[i] = *reinterpret_cast<const uint4*>(src + i * 8);
+    float f[KU * 16], amax = 0.f;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 2 * KU; ++i) {
+      const uint32_t xx[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 v = Io<T>::unpack2(xx[e]);
+        f[i * 8 + 2 * e] = v.x;
+        f[i * 8 + 2 * e + 1] = v.y;
+        bad = bad || !(fabsf(v.x) <= FLT_MAX) || !(fabsf(v.y) <= FLT_MAX);
+        amax = fmaxf(amax, fmaxf(fabsf(v.x), fabsf(v.y)));
+      }
+    }
+    float up = 1.f, down = 1.f;
+    if constexpr (Io<T>::kFmt == 1) {
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -100), 127);
+      up = exp2_int(14 - e);
+      down = exp2_int(e - 14);
+    }
+    bad = ((__ballot_sync(0xffffffffu, bad) >> (g * 4)) & 0xfu) != 0u;
+    // a row with an infinite or NaN element: every score is infinite or NaN, and so is its softmax NaN
+    const float c = bad ? __uint_as_float(0x7fffffffu) : p.scale_log2 * down;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) cq[nt][e] = __shfl_sync(0xffffffffu, c, (2 * t + e) * 4);
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      const int d = (i >> 2) * 16 + (i & 3) * 4;
+      qb[nt][i][0] = r < w.rows ? Io<__half>::pack2(f[d] * up, f[d + 1] * up) : 0u;
+      qb[nt][i][1] = r < w.rows ? Io<__half>::pack2(f[d + 2] * up, f[d + 3] * up) : 0u;
+    }
+  }
+
+  float oacc[NT][DT][4];
+  float m_ref[NT][2], l_run[NT][2];
+  float* sc[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) oacc[nt][i][j] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      m_ref[nt][e] = -INFINITY;
+      l_run[nt][e] = 0.f;
+      const int r = 8 * nt + 2 * t + e;
+      sc[nt][e] = w.kept != nullptr && r < w.rows ? w.kept + r * w.kept_pitch - w.kept_from : nullptr;
+    }
+  }
   bool ok = true;
 
-  for (int c = 0; c < n_chunks; ++c) {
-    const int s = c % kQ8Stages, key0 = (chunk0 + c) * kQ8Keys;
-    const float ks[2] = {ks_next[0], ks_next[1]}, vs[2] = {vs_next[0], vs_next[1]};
+  for (int c = 0; c < w.n_chunks; ++c) {
+    const int s = (w.loaded + c) % kQ8Stages, key0 = (w.chunk0 + c) * kQ8Keys;
+    float lv[2], inv[2];
+    const float ks[2] = {ks_next[0], ks_next[1]};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) scale_log_inv(vs_next[i] < kMinVScale ? kMinVScale : vs_next[i], lv[i], inv[i]);
     scales_of(c + 1, ks_next, vs_next);
-    const bool edge = key0 + kQ8Keys - 1 > lim_min;                // some row does not see some position of the chunk
-    ok = mbar_wait(bars + 8 * s, (c / kQ8Stages) & 1, ctl, KST_TIMEOUT_CONSUMER);
+    const bool edge = key0 + kQ8Keys - 1 > w.lim_min;                // some row does not see some position of the chunk
+    ok = mbar_wait(bars + 8 * s, ((w.loaded + c) / kQ8Stages) & 1, ctl, KST_TIMEOUT_CONSUMER);
     ok = __all_sync(0xffffffffu, ok);
     if (!ok) break;
-    // ---- scores of four 8-position blocks
-    float sacc[4][4];
+    // ---- s^T of two blocks of 16 positions; rows g, g + 8 of a block are its positions q8_key(g), 8 + q8_key(g)
+    float st[2][NT][4];
 #pragma unroll
-    for (int nb = 0; nb < 4; ++nb) {
+    for (int i = 0; i < 2; ++i) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sacc[nb][j] = 0.f;
-      const uint32_t row = nb * 8 + q8_key<D>(g);
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int u = 0; u < KU; ++u) {
-        const uint4 w = lds128(k_tile(s) + q8_off<D>(row, KU * t + u));
-        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          mma16816<__half>(sacc[nb], qa[4 * u + j], e4m3x2_to_f16x2(ww[j]), e4m3x2_to_f16x2(ww[j] >> 16));
-      }
+        for (int j = 0; j < 4; ++j) st[i][nt][j] = 0.f;
     }
-    // ---- t = acc * c * ks, t' = t + log2 vs
-    float lv[2], inv[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) { lv[i] = log2f(vs[i]); inv[i] = 1.0f / vs[i]; }
-    float mb_lo = -INFINITY, mb_hi = -INFINITY;
+    for (int u = 0; u < KU; ++u) {
+      uint4 kk[4];
 #pragma unroll
-    for (int nb = 0; nb < 4; ++nb) {
-      const float a_lo = c_lo * ks[nb >> 1], a_hi = c_hi * ks[nb >> 1], l = lv[nb >> 1];
+      for (int i = 0; i < 4; ++i) kk[i] = lds128(k_tile(s) + q8_off<D>(8 * i + q8_key<D>(g), KU * t + u));
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float x = sacc[nb][e] * a_lo, y = sacc[nb][2 + e] * a_hi;
-        const int key = key0 + nb * 8 + q8_key<D>(2 * t + e);
-        // whoever reads the kept scores knows which of them a row sees
-        if (sc_lo != nullptr) sc_lo[key] = x;
-        if (sc_hi != nullptr) sc_hi[key] = y;
-        x += l;
-        y += l;
-        if (edge) {
-          if (key > lim_lo) x = -INFINITY;
-          if (key > lim_hi) y = -INFINITY;
+      for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t lo = j == 0 ? kk[2 * i].x : j == 1 ? kk[2 * i].y : j == 2 ? kk[2 * i].z : kk[2 * i].w;
+          const uint32_t hi = j == 0 ? kk[2 * i + 1].x : j == 1 ? kk[2 * i + 1].y : j == 2 ? kk[2 * i + 1].z : kk[2 * i + 1].w;
+          const uint32_t a0 = e4m3x2_to_f16x2(lo), a1 = e4m3x2_to_f16x2(hi);
+          const uint32_t a2 = e4m3x2_to_f16x2(lo >> 16), a3 = e4m3x2_to_f16x2(hi >> 16);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_f16(st[i][nt], a0, a1, a2, a3, qb[nt][4 * u + j][0], qb[nt][4 * u + j][1]);
         }
-        sacc[nb][e] = x;
-        sacc[nb][2 + e] = y;
-        mb_lo = fmaxf(mb_lo, x);
-        mb_hi = fmaxf(mb_hi, y);
       }
     }
-    mb_lo = fmaxf(mb_lo, __shfl_xor_sync(0xffffffffu, mb_lo, 1)); mb_lo = fmaxf(mb_lo, __shfl_xor_sync(0xffffffffu, mb_lo, 2));
-    mb_hi = fmaxf(mb_hi, __shfl_xor_sync(0xffffffffu, mb_hi, 1)); mb_hi = fmaxf(mb_hi, __shfl_xor_sync(0xffffffffu, mb_hi, 2));
-    const float mn_lo = fmaxf(m_lo, mb_lo), mn_hi = fmaxf(m_hi, mb_hi);
-    if (__any_sync(0xffffffffu, mn_lo > m_lo || mn_hi > m_hi)) {
-      const float al_lo = mn_lo == -INFINITY ? 1.f : ex2_approx(m_lo - mn_lo);
-      const float al_hi = mn_hi == -INFINITY ? 1.f : ex2_approx(m_hi - mn_hi);
-      m_lo = mn_lo; m_hi = mn_hi;
-      l_lo *= al_lo; l_hi *= al_hi;
+    // ---- t = acc * c * ks, t' = t + log2 vs.  Accumulator (2 k + e): position 8 k + q8_key(g) of the block, column 2t + e
+    bool raise = false;
 #pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        oacc[i][0] *= al_lo; oacc[i][1] *= al_lo;
-        oacc[i][2] *= al_hi; oacc[i][3] *= al_hi;
-      }
-    }
-    const float use_lo = (m_lo == -INFINITY ? 0.f : m_lo) - kQ8PBias, use_hi = (m_hi == -INFINITY ? 0.f : m_hi) - kQ8PBias;
-    uint32_t ph[4][2], pl[4][2];
-    float sum_lo = 0.f, sum_hi = 0.f;
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int nb = 0; nb < 4; ++nb) {
-      const float a0 = ex2_approx(sacc[nb][0] - use_lo), a1 = ex2_approx(sacc[nb][1] - use_lo);
-      const float b0 = ex2_approx(sacc[nb][2] - use_hi), b1 = ex2_approx(sacc[nb][3] - use_hi);
-      sum_lo = fmaf(a0 + a1, inv[nb >> 1], sum_lo);
-      sum_hi = fmaf(b0 + b1, inv[nb >> 1], sum_hi);
-      ph[nb][0] = Io<__half>::pack2(a0, a1);
-      ph[nb][1] = Io<__half>::pack2(b0, b1);
-      if constexpr (HILO) {
-        const float2 ra = Io<__half>::unpack2(ph[nb][0]), rb = Io<__half>::unpack2(ph[nb][1]);
-        pl[nb][0] = Io<__half>::pack2(a0 - ra.x, a1 - ra.y);
-        pl[nb][1] = Io<__half>::pack2(b0 - rb.x, b1 - rb.y);
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float a = cq[nt][e] * ks[i];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int key = key0 + 16 * i + 8 * k + q8_key<D>(g);
+            float x = st[i][nt][2 * k + e] * a;
+            // whoever reads the kept scores knows which of them a row sees
+            if (sc[nt][e] != nullptr) sc[nt][e][key] = x;
+            x += lv[i];
+            if (edge && key > lim[nt][e]) x = -INFINITY;
+            st[i][nt][2 * k + e] = x;
+            raise = raise || x > m_ref[nt][e] + kQ8Slack;
+          }
+        }
+    if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float al[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float mx = fmaxf(fmaxf(st[0][nt][e], st[0][nt][2 + e]), fmaxf(st[1][nt][e], st[1][nt][2 + e]));
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+          const float mn = fmaxf(m_ref[nt][e], mx);
+          al[e] = mn == -INFINITY ? 1.f : ex2_approx(m_ref[nt][e] - mn);
+          m_ref[nt][e] = mn;
+          l_run[nt][e] *= al[e];
+        }
+#pragma unroll
+        for (int i = 0; i < DT; ++i) {
+          oacc[nt][i][0] *= al[0]; oacc[nt][i][1] *= al[1];
+          oacc[nt][i][2] *= al[0]; oacc[nt][i][3] *= al[1];
+        }
       }
     }
-    l_lo += sum_lo;
-    l_hi += sum_hi;
-    // ---- o += P' v: two steps of 16 positions.  Column block j of lane g's output holds d = g * (D / 8) + j.
+    // ---- P' = 2^(t' - m'), transposed into the B operand of o^T += v^T P'^T
+    uint32_t ph[2][NT][2], pl[2][NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float use[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) use[e] = kQ8PBias - (m_ref[nt][e] == -INFINITY ? 0.f : m_ref[nt][e]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float a = ex2_approx(st[i][nt][2 * k] + use[0]), c2 = ex2_approx(st[i][nt][2 * k + 1] + use[1]);
+          l_run[nt][0] = fmaf(a, inv[i], l_run[nt][0]);
+          l_run[nt][1] = fmaf(c2, inv[i], l_run[nt][1]);
+          const uint32_t hi = Io<__half>::pack2(a, c2);
+          ph[i][nt][k] = transpose8(hi);
+          if constexpr (HILO) {
+            const float2 r = Io<__half>::unpack2(hi);
+            pl[i][nt][k] = transpose8(Io<__half>::pack2(a - r.x, c2 - r.y));
+          }
+        }
+      }
+    }
+    // ---- rows g, g + 8 of block j of o^T hold d = g * (D / 8) + 2 j, + 1
     const uint32_t vt = k_tile(s) + SM::kTile;
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
-      const uint32_t ah[4] = {ph[2 * kk][0], ph[2 * kk][1], ph[2 * kk + 1][0], ph[2 * kk + 1][1]};
-      uint32_t al[4] = {0u, 0u, 0u, 0u};
-      if constexpr (HILO) {
-        al[0] = pl[2 * kk][0]; al[1] = pl[2 * kk][1]; al[2] = pl[2 * kk + 1][0]; al[3] = pl[2 * kk + 1][1];
-      }
       constexpr int W = D / 32;                // 32-bit words a lane takes of a row: 4 or 2
-      uint32_t v[4][W];                        // rows: positions 2t, 2t + 1 of the step's two blocks
+      uint32_t v[4][W];                        // positions 2t, 2t + 1, 2t + 8, 2t + 9 of the block
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int rr = (2 * kk + (i >> 1)) * 8 + q8_key<D>(2 * t + (i & 1));
         if constexpr (D == 128) {
-          const uint4 w = lds128(vt + q8_off<D>(rr, g));
-          v[i][0] = w.x; v[i][1] = w.y; v[i][2] = w.z; v[i][3] = w.w;
+          const uint4 x = lds128(vt + q8_off<D>(rr, g));
+          v[i][0] = x.x; v[i][1] = x.y; v[i][2] = x.z; v[i][3] = x.w;
         } else {
-          const uint2 w = lds64(vt + q8_off<D>(rr, g >> 1) + (g & 1) * 8);
-          v[i][0] = w.x; v[i][1] = w.y;
+          const uint2 x = lds64(vt + q8_off<D>(rr, g >> 1) + (g & 1) * 8);
+          v[i][0] = x.x; v[i][1] = x.y;
         }
         if (edge) {
           const int key = key0 + rr;
 #pragma unroll
-          for (int w = 0; w < W; ++w) {
-            const uint32_t bad = nan_bytes(v[i][w]);
+          for (int j = 0; j < W; ++j) {
+            const uint32_t bad = nan_bytes(v[i][j]);
             if (bad != 0u) {
-              v[i][w] &= ~bad;
-              if (key <= lim_max)
+              v[i][j] &= ~bad;
+              if (key <= w.lim_max)
                 for (int e = 0; e < 4; ++e)
-                  if ((bad >> (8 * e)) & 1u) atomicMin(&nan_from[g * (D / 8) + 4 * w + e], key);
+                  if ((bad >> (8 * e)) & 1u) atomicMin(&nan_from[g * (D / 8) + 4 * j + e], key);
             }
           }
         }
       }
 #pragma unroll
-      for (int w = 0; w < W; ++w) {
-        // bytes of two positions side by side: (k, k + 1) pairs of column 4 w + e
-        const uint32_t x0 = __byte_perm(v[0][w], v[1][w], 0x5140), x1 = __byte_perm(v[0][w], v[1][w], 0x7362);
-        const uint32_t y0 = __byte_perm(v[2][w], v[3][w], 0x5140), y1 = __byte_perm(v[2][w], v[3][w], 0x7362);
-        const uint32_t b0[4] = {e4m3x2_to_f16x2(x0), e4m3x2_to_f16x2(x0 >> 16), e4m3x2_to_f16x2(x1), e4m3x2_to_f16x2(x1 >> 16)};
-        const uint32_t b1[4] = {e4m3x2_to_f16x2(y0), e4m3x2_to_f16x2(y0 >> 16), e4m3x2_to_f16x2(y1), e4m3x2_to_f16x2(y1 >> 16)};
+      for (int j = 0; j < W; ++j) {
+        // bytes of two positions side by side: (k, k + 1) pairs of d = 4 j + {0, 1}, {2, 3}
+        const uint32_t x0 = __byte_perm(v[0][j], v[1][j], 0x5140), x1 = __byte_perm(v[0][j], v[1][j], 0x7362);
+        const uint32_t y0 = __byte_perm(v[2][j], v[3][j], 0x5140), y1 = __byte_perm(v[2][j], v[3][j], 0x7362);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          mma16816<__half>(oacc[4 * w + e], ah, b0[e], b1[e]);
-          if constexpr (HILO) mma16816<__half>(oacc[4 * w + e], al, b0[e], b1[e]);
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t x = e == 0 ? x0 : x1, y = e == 0 ? y0 : y1;
+          const uint32_t a0 = e4m3x2_to_f16x2(x), a1 = e4m3x2_to_f16x2(x >> 16);
+          const uint32_t a2 = e4m3x2_to_f16x2(y), a3 = e4m3x2_to_f16x2(y >> 16);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma_f16(oacc[nt][2 * j + e], a0, a1, a2, a3, ph[kk][nt][0], ph[kk][nt][1]);
+            if constexpr (HILO) mma_f16(oacc[nt][2 * j + e], a0, a1, a2, a3, pl[kk][nt][0], pl[kk][nt][1]);
+          }
         }
       }
     }
     __syncwarp();                              // every lane has read stage s
-    if (lane == 0 && c + kQ8Stages < n_chunks) load(c + kQ8Stages);
+    if (lane == 0 && c + kQ8Stages < w.n_chunks) load(c + kQ8Stages);
   }
-  l_lo += __shfl_xor_sync(0xffffffffu, l_lo, 1); l_lo += __shfl_xor_sync(0xffffffffu, l_lo, 2);
-  l_hi += __shfl_xor_sync(0xffffffffu, l_hi, 1); l_hi += __shfl_xor_sync(0xffffffffu, l_hi, 2);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) l_run[nt][e] += __shfl_xor_sync(0xffffffffu, l_run[nt][e], o);
   __syncthreads();                             // the partial results take the rings' place
-  if (s_abort) {
-    // a wait ran out: give copies in flight time to land before shared memory is given up
+  if (*ctl.abort) {
+    // a wait ran out: give copies in flight time to land before shared memory is put to another use
     const uint64_t t0 = globaltimer_ns();
     while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
-    return;
   }
-  // ---- the warps' partial results -> shared memory [warp][row][D | max, sum], merged in fixed order.  Block j, column
-  // pair (2t, 2t + 1) of this lane's accumulators: d = 2t * (D / 8) + j and (2t + 1) * (D / 8) + j
+  // ---- the warps' partial results -> shared memory [warp][row][D | max, sum], merged in fixed order
   float* part = reinterpret_cast<float*>(gen);
-  {
-    float* lo = part + (warp * kQ8Rows + g) * SM::kRow;
-    float* hi = lo + 8 * SM::kRow;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+  for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int j = 0; j < NB; j += 4) {
-        const int d = (2 * t + i) * (D / 8) + j;
-        *reinterpret_cast<float4*>(lo + d) = make_float4(oacc[j][i], oacc[j + 1][i], oacc[j + 2][i], oacc[j + 3][i]);
-        *reinterpret_cast<float4*>(hi + d) =
-            make_float4(oacc[j][2 + i], oacc[j + 1][2 + i], oacc[j + 2][2 + i], oacc[j + 3][2 + i]);
-      }
+    for (int e = 0; e < 2; ++e) {
+      float* dst = part + (warp * ROWS + 8 * nt + 2 * t + e) * SM::kRow;
+#pragma unroll
+      for (int j = 0; j < DT; j += 2)
+        *reinterpret_cast<float4*>(dst + g * (D / 8) + 2 * j) =
+            make_float4(oacc[nt][j][e], oacc[nt][j][2 + e], oacc[nt][j + 1][e], oacc[nt][j + 1][2 + e]);
+      if (g == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(m_ref[nt][e], l_run[nt][e]);
     }
-    if (t == 0) {
-      *reinterpret_cast<float2*>(lo + D) = make_float2(m_lo, l_lo);
-      *reinterpret_cast<float2*>(hi + D) = make_float2(m_hi, l_hi);
-    }
-  }
   __syncthreads();
-  constexpr int TPR = kQ8Threads / kQ8Rows, CW = D / TPR;          // threads per row, columns per thread
-  const int row = threadIdx.x / TPR, c0 = (threadIdx.x % TPR) * CW;
-  float mx = -INFINITY, tot = 0.f, acc[CW];
+  const int row = threadIdx.x / SM::kTPR, c0 = (threadIdx.x % SM::kTPR) * CW;
+  mx = -INFINITY;
+  tot = 0.f;
 #pragma unroll
   for (int c = 0; c < CW; ++c) acc[c] = 0.f;
 #pragma unroll
-  for (int w = 0; w < kQ8Warps; ++w) mx = fmaxf(mx, part[(w * kQ8Rows + row) * SM::kRow + D]);
+  for (int i = 0; i < kQ8Warps; ++i) mx = fmaxf(mx, part[(i * ROWS + row) * SM::kRow + D]);
 #pragma unroll
-  for (int w = 0; w < kQ8Warps; ++w) {
-    const float* src = part + (w * kQ8Rows + row) * SM::kRow;
+  for (int i = 0; i < kQ8Warps; ++i) {
+    const float* src = part + (i * ROWS + row) * SM::kRow;
     if (src[D + 1] == 0.f) continue;                               // saw no position of this row
     const float f = ex2_approx(src[D] - mx);
     tot = fmaf(f, src[D + 1], tot);
 #pragma unroll
     for (int c = 0; c < CW; ++c) acc[c] = fmaf(f, src[c0 + c], acc[c]);
   }
-  if (row >= rows) return;
-  const int lim = last_of(row);
+  const int last = w.last_of(p, row);
 #pragma unroll
   for (int c = 0; c < CW; ++c)
-    if (nan_from[c0 + c] <= lim) acc[c] = __uint_as_float(0x7fffffffu);
-  if (p.n_splits > 1) {
-    const long long at = (static_cast<long long>(split) * p.B * p.Hkv * p.tiles + unit) * kQ8Rows + row;
-#pragma unroll
-    for (int c = 0; c < CW; c += 4)
-      *reinterpret_cast<float4*>(p.part_o + at * D + c0 + c) = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
-    if (c0 == 0) p.part_ml[at] = make_float2(mx, tot);
-    return;
+    if (nan_from[c0 + c] <= last) acc[c] = __uint_as_float(0x7fffffffu);
+}
+
+// barriers and the table of NaN columns; then the wait for the launch before this one.  Returns whether an earlier kernel gave up.
+template <int D, int NT>
+__device__ __forceinline__ bool q8_begin(const Q8Params& p, const CUtensorMap& tm_k, const CUtensorMap& tm_v, uint32_t base,
+                                         int* nan_from, int* s_abort) {
+  if ((threadIdx.x & 31) == 0) {
+    for (int s = 0; s < kQ8Stages; ++s) mbar_init(base + Q8Smem<D, NT>::kBars + ((threadIdx.x >> 5) * kQ8Stages + s) * 8, 1);
+    fence_mbar_init();
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
   }
-  const int rr = r0 + row, i = rr / p.G, hq = h * p.G + rr % p.G;
+  if (threadIdx.x == 0) *s_abort = 0;
+  for (int i = threadIdx.x; i < D; i += kQ8Threads) nan_from[i] = 0x7fffffff;
+  __syncthreads();
+  griddep_wait();                              // q, the codes and the lengths may come from the launch before
+  griddep_launch();
+  return *reinterpret_cast<volatile int*>(p.status) != 0;
+}
+
+// CW columns of a finished row, and its log-sum-exp
+template <typename T, int CW>
+__device__ __forceinline__ void q8_store_row(const Q8Params& p, int b, int h, int r, int c0, const float* acc, float mx, float tot) {
+  const int i = r / p.G, hq = h * p.G + r % p.G;
   const float inv = tot == 0.f ? 0.f : 1.0f / tot;
   T* dst = static_cast<T*>(p.o.ptr) + b * p.o.stride_b + static_cast<long long>(i) * p.o.stride_s +
            static_cast<long long>(hq) * p.o.stride_h + c0;
 #pragma unroll
-  for (int c = 0; c < CW; c += 8) {
-    uint4 v;
-    v.x = Io<T>::pack2(acc[c] * inv, acc[c + 1] * inv); v.y = Io<T>::pack2(acc[c + 2] * inv, acc[c + 3] * inv);
-    v.z = Io<T>::pack2(acc[c + 4] * inv, acc[c + 5] * inv); v.w = Io<T>::pack2(acc[c + 6] * inv, acc[c + 7] * inv);
-    *reinterpret_cast<uint4*>(dst + c) = v;
+  for (int c = 0; c < CW; c += 2) *reinterpret_cast<uint32_t*>(dst + c) = Io<T>::pack2(acc[c] * inv, acc[c + 1] * inv);
+  if (c0 == 0 && p.lse != nullptr) p.lse[(static_cast<long long>(b) * p.Hq + hq) * p.M + i] = mx - kQ8PBias + log2f(tot);
+}
+
+// Long caches: each CTA takes its share of all chunks, a piece of a unit after the other.
+template <typename T, int D, int NT, bool HILO>
+__global__ void __launch_bounds__(kQ8Threads)
+attn_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+               const __grid_constant__ Q8Params p) {
+  using SM = Q8Smem<D, NT>;
+  constexpr int ROWS = SM::kRows, CW = SM::kCW;
+  extern __shared__ uint8_t q8_smem_raw[];
+  __shared__ int nan_from[D];                  // first position whose v code of this column is NaN, in edge chunks
+  __shared__ int s_abort;
+  const uint32_t base = (smem_u32(q8_smem_raw) + 1023u) & ~1023u;
+  uint8_t* gen = q8_smem_raw + (base - smem_u32(q8_smem_raw));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Ctl ctl{p.status, &s_abort};
+  if (q8_begin<D, NT>(p, tm_k, tm_v, base, nan_from, &s_abort)) return;
+
+  // ---- this CTA's share: chunks [at, end) of all, beginning `skip` chunks into unit (b, h, tile)
+  const int cta = static_cast<int>(blockIdx.x);
+  int b, h, tile, skip = 0, left;              // left: chunks still to do
+  unsigned share = 1u;
+  if (p.ctas == 0) {
+    tile = cta % p.tiles;
+    h = cta / p.tiles % p.Hkv;
+    b = cta / p.tiles / p.Hkv;
+    left = chunks_of(p.len(b));
+  } else {
+    const int all = chunks_before(p, 0).y;
+    share = share_of(p, all);
+    const unsigned per = p.Hkv * p.tiles, end = static_cast<unsigned>(all) * per;
+    unsigned at = cta * share;
+    if (at >= end) return;
+    left = static_cast<int>(min(end - at, share));
+    // the sequence the share begins in: running sums over 32 sequences at a time
+    b = p.B;
+    for (int b0 = 0; b0 < p.B; b0 += 32) {
+      const unsigned c = b0 + lane < p.B ? chunks_of(p.len(b0 + lane)) * per : 0u;
+      unsigned incl = c;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      const uint32_t past = __ballot_sync(0xffffffffu, incl > at);
+      if (past != 0u) {
+        const int l = __ffs(past) - 1;
+        b = b0 + l;
+        at -= __shfl_sync(0xffffffffu, incl - c, l);
+        break;
+      }
+      at -= __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (b == p.B) return;                      // lengths that change under the kernel: nothing sensible to do, nothing unsafe done
+    const unsigned mine = chunks_of(p.len(b)), u = min(at / mine, per - 1);
+    skip = static_cast<int>(at - u * mine);
+    h = static_cast<int>(u / p.tiles);
+    tile = static_cast<int>(u % p.tiles);
   }
-  if (c0 == 0) {
-    const float lse = mx - kQ8PBias + log2f(tot);
-    if (p.lse != nullptr) p.lse[(static_cast<long long>(b) * p.Hq + hq) * p.M + i] = lse;
-    if (p.part_ml != nullptr) p.part_ml[static_cast<long long>(unit) * kQ8Rows + row] = make_float2(mx, tot);
+  for (int loaded = 0;;) {
+    const int bh = b * p.Hkv + h, unit = bh * p.tiles + tile;
+    const int total = chunks_of(p.len(b)), many = max(min(total - skip, left), 1);
+    Q8Piece w = piece_of(p, b, h, tile, skip, many, warp);
+    w.loaded = loaded;
+    if (p.scores != nullptr) {
+      w.kept = p.scores + (static_cast<long long>(bh) * p.R + w.r0) * p.pitch;
+      w.kept_pitch = p.pitch;
+    }
+    float acc[CW], mx, tot;
+    q8_piece<T, D, NT, HILO>(p, tm_k, tm_v, w, gen, base, nan_from, ctl, acc, mx, tot);
+    if (s_abort) return;
+    const int row = threadIdx.x / SM::kTPR, c0 = (threadIdx.x % SM::kTPR) * CW;
+    if (row < w.rows) {
+      const long long at = static_cast<long long>(unit + (p.ctas > 0 ? cta : 0)) * ROWS + row;
+      if (many < total) {
+#pragma unroll
+        for (int c = 0; c < CW; c += 4)
+          *reinterpret_cast<float4*>(p.part_o + at * D + c0 + c) = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+      } else {
+        q8_store_row<T, CW>(p, b, h, w.r0 + row, c0, acc, mx, tot);
+      }
+      if (c0 == 0 && p.part_ml != nullptr) p.part_ml[at] = make_float2(mx, tot);
+    }
+    if (skip == 0 && threadIdx.x == 0 && p.pieces != nullptr) {    // the unit begins in this share, with `left` chunks of it to go
+      const int rest = total - left;                               // chunks that fall to the CTAs behind
+      p.pieces[unit] = make_int2(p.ctas > 0 ? cta : 0, (p.ctas > 0 ? cta : 0) + (rest > 0 ? (rest + static_cast<int>(share) - 1) / static_cast<int>(share) : 0));
+    }
+    // ---- the next piece of the share begins with the next unit
+    left -= many;
+    if (left <= 0) return;
+    loaded += w.n_chunks;
+    skip = 0;
+    if (++tile == p.tiles) {
+      tile = 0;
+      if (++h == p.Hkv) {
+        h = 0;
+        if (++b == p.B) return;
+      }
+    }
+    fence_proxy_async_smem();                  // the partial results gave way to the next piece's tiles
+    __syncthreads();
+    for (int i = threadIdx.x; i < D; i += kQ8Threads) nan_from[i] = 0x7fffffff;
+    __syncthreads();
   }
 }
 
-// Merge of the splits and weights of the positions.  CTAs [0, merge_ctas): one warp per row; the rest: one thread per
-// position of a (b, kv head), rows in ascending order.
+// Short caches (at most kQ8Keep chunks a warp): a cluster of CTAs per unit, which meet in shared memory, so that one launch
+// does everything, the weights too: each warp keeps its scores on chip until the rows' log-sum-exps are known.
+template <typename T, int D, int NT, bool HILO>
+__global__ void __launch_bounds__(kQ8Threads)
+attn_q8_cluster_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                       const __grid_constant__ Q8Params p, int cluster) {
+  using SM = Q8Smem<D, NT>;
+  constexpr int ROWS = SM::kRows, CW = SM::kCW;
+  extern __shared__ uint8_t q8_smem_raw[];
+  __shared__ int nan_from[D];
+  __shared__ int s_abort;
+  __shared__ float lse_of[ROWS];
+  const uint32_t base = (smem_u32(q8_smem_raw) + 1023u) & ~1023u;
+  uint8_t* gen = q8_smem_raw + (base - smem_u32(q8_smem_raw));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Ctl ctl{p.status, &s_abort};
+  // no CTA leaves before the cluster's last barrier; one that must not work writes nothing
+  const bool dead = q8_begin<D, NT>(p, tm_k, tm_v, base, nan_from, &s_abort);
+  const int rank = static_cast<int>(cluster_ctarank()), unit = static_cast<int>(blockIdx.x) / cluster;
+  const int tile = unit % p.tiles, h = unit / p.tiles % p.Hkv, b = unit / p.tiles / p.Hkv;
+  const int total = chunks_of(p.len(b)), skip = total * rank / cluster;
+  Q8Piece w = piece_of(p, b, h, tile, skip, total * (rank + 1) / cluster - skip, warp);
+  if (dead) w.n_chunks = 0;
+  if (p.weight != nullptr) {
+    w.kept = reinterpret_cast<float*>(gen + SM::kKept) + warp * ROWS * SM::kKeptPitch;
+    w.kept_pitch = SM::kKeptPitch;
+    w.kept_from = w.chunk0 * kQ8Keys;
+  }
+  float acc[CW], mx, tot;
+  q8_piece<T, D, NT, HILO>(p, tm_k, tm_v, w, gen, base, nan_from, ctl, acc, mx, tot);
+  const bool write = !dead && s_abort == 0;
+  float* mine = reinterpret_cast<float*>(gen + SM::kMine);         // [ROWS][kRow], behind the warps' results
+  {
+    const int row = threadIdx.x / SM::kTPR, c0 = (threadIdx.x % SM::kTPR) * CW;
+#pragma unroll
+    for (int c = 0; c < CW; c += 4)
+      *reinterpret_cast<float4*>(mine + row * SM::kRow + c0 + c) = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+    if (c0 == 0) *reinterpret_cast<float2*>(mine + row * SM::kRow + D) = make_float2(mx, tot);
+  }
+  if (cluster > 1) cluster_sync_all(); else __syncthreads();
+  const uint32_t mine_s = base + SM::kMine;
+  // ---- rows rank, rank + cluster, ... : two columns a thread, the ranks' results in ascending order
+  auto ml_of = [&](int r, int i) { return ld_cluster_f2(map_to_rank(mine_s + (r * SM::kRow + D) * 4, static_cast<uint32_t>(i))); };
+  for (int r = rank + cluster * (static_cast<int>(threadIdx.x) / (D / 2)); r < w.rows; r += cluster * (kQ8Threads / (D / 2))) {
+    const int d = (threadIdx.x % (D / 2)) * 2;
+    float2 ml[kQ8MaxCluster], v[kQ8MaxCluster];
+#pragma unroll
+    for (int i = 0; i < kQ8MaxCluster; ++i)
+      if (i < cluster) {
+        ml[i] = ml_of(r, i);
+        v[i] = ld_cluster_f2(map_to_rank(mine_s + (r * SM::kRow + d) * 4, static_cast<uint32_t>(i)));
+      }
+    float m = -INFINITY, sum = 0.f, o[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < kQ8MaxCluster; ++i)
+      if (i < cluster) m = fmaxf(m, ml[i].x);
+#pragma unroll
+    for (int i = 0; i < kQ8MaxCluster; ++i)
+      if (i < cluster && ml[i].y != 0.f) {
+        const float f = ex2_approx(ml[i].x - m);
+        sum = fmaf(f, ml[i].y, sum);
+        o[0] = fmaf(f, v[i].x, o[0]);
+        o[1] = fmaf(f, v[i].y, o[1]);
+      }
+    if (write) q8_store_row<T, 2>(p, b, h, w.r0 + r, d, o, m, sum);
+  }
+  if (p.weight != nullptr) {
+    for (int r = threadIdx.x; r < w.rows; r += kQ8Threads) {
+      float m = -INFINITY, sum = 0.f;
+      for (int i = 0; i < cluster; ++i) m = fmaxf(m, ml_of(r, i).x);
+      for (int i = 0; i < cluster; ++i) {
+        const float2 ml = ml_of(r, i);
+        if (ml.y != 0.f) sum = fmaf(ex2_approx(ml.x - m), ml.y, sum);
+      }
+      lse_of[r] = m - kQ8PBias + log2f(sum);
+    }
+    __syncthreads();
+    // only launched with one row tile per (b, kv head): the rows of the tile are all that see a position
+    float* out = p.weight + b * p.w_sb + h * p.w_sh;
+    for (int i = lane; i < w.n_chunks * kQ8Keys; i += 32) {
+      const int key = w.kept_from + i;
+      if (key >= w.n) break;
+      const int first = p.causal ? max(key - (w.n - p.M), 0) * p.G : 0;
+      float sum = 0.f;
+      for (int r = first; r < w.rows; ++r) sum += ex2_approx(w.kept[r * SM::kKeptPitch + i] - lse_of[r]);
+      if (write) out[key] = p.weight_add ? out[key] + sum : sum;
+    }
+  }
+  if (cluster > 1) cluster_sync_all();                             // no CTA leaves while its results may be read
+}
+
+// Merge of the pieces, and weights of the positions.  CTAs [0, merge_ctas): kQ8JoinThreads / (D / 2) rows of a unit each, two
+// columns a thread; the rest: four positions a thread of a (b, kv head), rows in ascending order.
 constexpr int kQ8JoinThreads = 256;
+constexpr int kQ8JoinWarps = kQ8JoinThreads / 32;
+constexpr int kQ8JoinKeys = 4 * kQ8JoinThreads;
+// maximum and sum of a row over its pieces by one warp; at: the row in the first piece's slot
+__device__ __forceinline__ float2 join_ml(const Q8Params& p, long long at, int here, int lane) {
+  float2 mine = make_float2(-INFINITY, 0.f);   // a lane's pieces lane, lane + 32, ...
+  for (int s = lane; s < here; s += 32) {
+    const float2 ml = p.part_ml[at + static_cast<long long>(s) * p.tile_rows];
+    if (ml.y == 0.f) continue;
+    const float m = fmaxf(mine.x, ml.x);
+    mine.y = (mine.y == 0.f ? 0.f : mine.y * ex2_approx(mine.x - m)) + ml.y * ex2_approx(ml.x - m);
+    mine.x = m;
+  }
+  float m = mine.x;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  float tot = mine.y == 0.f ? 0.f : mine.y * ex2_approx(mine.x - m);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) tot += __shfl_xor_sync(0xffffffffu, tot, o);
+  return make_float2(m, tot);
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kQ8JoinThreads)
 attn_q8_join_kernel(const __grid_constant__ Q8Params p, int merge_ctas, int key_tiles) {
-  extern __shared__ float q8_lse[];            // [R] (weight CTAs)
+  extern __shared__ float q8_join[];           // weight CTAs: [R] log-sum-exps
+  constexpr int ROWS = kQ8JoinThreads / (D / 2);
+  __shared__ float2 all[ROWS];
   griddep_wait();
   griddep_launch();
   if (*reinterpret_cast<volatile int*>(p.status) != 0) return;
-  const long long units = static_cast<long long>(p.B) * p.Hkv * p.tiles;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (static_cast<int>(blockIdx.x) < merge_ctas) {
-    const long long id = static_cast<long long>(blockIdx.x) * (kQ8JoinThreads / 32) + warp;     // (bh, r)
-    if (id >= static_cast<long long>(p.B) * p.Hkv * p.R) return;
-    const int r = static_cast<int>(id % p.R), bh = static_cast<int>(id / p.R);
-    const long long at = (static_cast<long long>(bh) * p.tiles + r / kQ8Rows) * kQ8Rows + r % kQ8Rows;
-    const long long step = units * kQ8Rows;
-    constexpr int VPL = D / 32;
-    float m = -INFINITY, tot = 0.f, acc[VPL];
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) acc[i] = 0.f;
-    for (int s = 0; s < p.n_splits; ++s) m = fmaxf(m, p.part_ml[s * step + at].x);
-    for (int s = 0; s < p.n_splits; ++s) {
-      const float2 ml = p.part_ml[s * step + at];
-      if (ml.y == 0.f) continue;
-      const float w = ex2_approx(ml.x - m);
-      tot = fmaf(w, ml.y, tot);
-      const float* src = p.part_o + (s * step + at) * D + lane * VPL;
-#pragma unroll
-      for (int i = 0; i < VPL; i += 2) {
-        const float2 v = *reinterpret_cast<const float2*>(src + i);
-        acc[i] = fmaf(w, v.x, acc[i]);
-        acc[i + 1] = fmaf(w, v.y, acc[i + 1]);
+    const int groups = p.tile_rows / ROWS;     // tile_rows and ROWS are powers of two; at least one
+    const int unit = static_cast<int>(blockIdx.x) / max(groups, 1), r_first = static_cast<int>(blockIdx.x) % max(groups, 1) * ROWS;
+    const int tile = unit % p.tiles, bh = unit / p.tiles, rows = min(p.tile_rows, p.R - tile * p.tile_rows);
+    if (r_first >= rows) return;
+    const int2 on = p.pieces[unit];
+    const int here = on.y - on.x + 1;
+    if (here == 1) return;                     // written by the one piece itself
+    const long long at = static_cast<long long>(unit + on.x) * p.tile_rows + r_first;
+    if (warp < ROWS && r_first + warp < rows) {
+      const float2 ml = join_ml(p, at + warp, here, lane);
+      if (lane == 0) all[warp] = ml;
+    }
+    __syncthreads();
+    const int r = tid / (D / 2), d = (tid % (D / 2)) * 2;
+    if (r_first + r >= rows) return;
+    const float2 ml = all[r];
+    float acc[2] = {0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < here; ++s) {
+      const long long row = at + r + static_cast<long long>(s) * p.tile_rows;
+      const float2 x = p.part_ml[row];
+      const float2 v = *reinterpret_cast<const float2*>(p.part_o + row * D + d);
+      const float w = x.y == 0.f ? 0.f : ex2_approx(x.x - ml.x);
+      if (x.y != 0.f) {                        // a piece that saw nothing has written zeros or, where v has NaN, nothing to weigh
+        acc[0] = fmaf(w, v.x, acc[0]);
+        acc[1] = fmaf(w, v.y, acc[1]);
       }
     }
-    const int b = bh / p.Hkv, hq = (bh % p.Hkv) * p.G + r % p.G, i = r / p.G;
-    const float inv = tot == 0.f ? 0.f : 1.0f / tot;
-    T* dst = static_cast<T*>(p.o.ptr) + b * p.o.stride_b + static_cast<long long>(i) * p.o.stride_s +
-             static_cast<long long>(hq) * p.o.stride_h + lane * VPL;
-#pragma unroll
-    for (int e = 0; e < VPL; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = Io<T>::pack2(acc[e] * inv, acc[e + 1] * inv);
-    if (lane == 0 && p.lse != nullptr) p.lse[(static_cast<long long>(b) * p.Hq + hq) * p.M + i] = m - kQ8PBias + log2f(tot);
+    q8_store_row<T, 2>(p, bh / p.Hkv, bh % p.Hkv, tile * p.tile_rows + r_first + r, d, acc, ml.x, ml.y);
     return;
   }
   const int id = static_cast<int>(blockIdx.x) - merge_ctas;
   const int bh = id / key_tiles, b = bh / p.Hkv, h = bh % p.Hkv;
   const int n = p.len(b);
-  const int key = (id % key_tiles) * kQ8JoinThreads + static_cast<int>(threadIdx.x);
-  if ((id % key_tiles) * kQ8JoinThreads >= n) return;
-  const long long step = units * kQ8Rows;
-  for (int r = threadIdx.x; r < p.R; r += kQ8JoinThreads) {
-    const long long at = (static_cast<long long>(bh) * p.tiles + r / kQ8Rows) * kQ8Rows + r % kQ8Rows;
-    float m = -INFINITY, tot = 0.f;
-    for (int s = 0; s < p.n_splits; ++s) m = fmaxf(m, p.part_ml[s * step + at].x);
-    for (int s = 0; s < p.n_splits; ++s) {
-      const float2 ml = p.part_ml[s * step + at];
-      if (ml.y != 0.f) tot = fmaf(ex2_approx(ml.x - m), ml.y, tot);
-    }
-    q8_lse[r] = m - kQ8PBias + log2f(tot);
+  const int key0 = (id % key_tiles) * kQ8JoinKeys, key = key0 + 4 * tid;
+  if (key0 >= n) return;
+  for (int r = warp; r < p.R; r += kQ8JoinWarps) {
+    const int unit = bh * p.tiles + r / p.tile_rows;
+    const int2 on = p.pieces[unit];
+    const float2 ml = join_ml(p, static_cast<long long>(unit + on.x) * p.tile_rows + r % p.tile_rows, on.y - on.x + 1, lane);
+    if (lane == 0) q8_join[r] = ml.x - kQ8PBias + log2f(ml.y);
   }
   __syncthreads();
   if (key >= n) return;
-  // causal: position j is seen by the queries i >= j - (n - M)
+  // causal: position j is seen by the queries i >= j - (n - M).  What a row kept of positions that it does not see is not
+  // taken, whatever it is.
   const int first = p.causal ? max(key - (n - p.M), 0) * p.G : 0;
   const float* src = p.scores + static_cast<long long>(bh) * p.R * p.pitch + key;
-  float acc = 0.f;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  const bool edge = key + 3 > last_seen(p, n, first);
 #pragma unroll 4
-  for (int r = first; r < p.R; ++r) acc += ex2_approx(src[r * p.pitch] - q8_lse[r]);
+  for (int r = first; r < p.R; ++r) {
+    const float4 x = *reinterpret_cast<const float4*>(src + r * p.pitch);
+    const float l = q8_join[r];
+    const int seen = edge ? last_seen(p, n, r) - key : 3;
+    acc[0] += ex2_approx(x.x - l);
+    if (seen >= 1) acc[1] += ex2_approx(x.y - l);
+    if (seen >= 2) acc[2] += ex2_approx(x.z - l);
+    if (seen >= 3) acc[3] += ex2_approx(x.w - l);
+  }
   float* w = p.weight + b * p.w_sb + h * p.w_sh + key;
-  *w = p.weight_add ? *w + acc : acc;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (key + e < n) w[e] = p.weight_add ? w[e] + acc[e] : acc[e];
 }
 
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 struct Q8Plan {
-  int tiles, n_splits;
-  size_t ml_off, o_off, score_off, total;
+  int tiles, tile_rows, ctas, cluster;         // cluster > 0: one launch of clusters, no scratch
+  long long units;
+  size_t ml_off, o_off, piece_off, score_off, total;
   long long pitch;
 };
 
-// How many CTAs share a (b, kv head, row tile)'s positions: enough to fill the SMs, at least two chunks a warp
-Q8Plan plan_of(const TrnAttnQ8Args& a, int sm_count, bool splits_allowed) {
+// Short caches: clusters of CTAs, when kQ8Keep chunks a warp suffice with as many CTAs per unit (a power of two) as fill one
+// round of resident CTAs (with weights: if one row tile holds all rows).  Else the chunks are dealt out to one round
+// of resident CTAs, fewer where that would leave a warp without a chunk.
+Q8Plan plan_of(const TrnAttnQ8Args& a, int sm_count, bool divide) {
   Q8Plan w{};
   const int R = a.M * (a.Hq / a.Hkv);
-  w.tiles = (R + kQ8Rows - 1) / kQ8Rows;
-  const long long units = static_cast<long long>(a.B) * a.Hkv * w.tiles;
-  const long long chunks = (static_cast<long long>(a.cache.S) + kQ8Keys - 1) / kQ8Keys;
-  long long ns = static_cast<long long>(sm_count) * kQ8TargetCtas / units;
-  if (ns > chunks / (2 * kQ8Warps)) ns = chunks / (2 * kQ8Warps);
-  w.n_splits = ns < 1 || !splits_allowed ? 1 : static_cast<int>(ns);
+  w.tile_rows = 8;
+  while (w.tile_rows < R && w.tile_rows < 8 * q8_max_tiles(a.D)) w.tile_rows *= 2;
+  w.tiles = (R + w.tile_rows - 1) / w.tile_rows;
+  w.units = static_cast<long long>(a.B) * a.Hkv * w.tiles;
+  const int longest = a.kv_len != nullptr ? a.cache.S : min(max(a.kv_len_all, 1), a.cache.S);
+  const int unit_chunks = (longest - 1) / kQ8Keys + 1;
+  const long long round = static_cast<long long>(sm_count) * kQ8TargetCtas;
+  int cluster = 1;
+  while (cluster < kQ8MaxCluster && 2 * cluster * w.units <= round && 2 * cluster * kQ8Warps <= unit_chunks + kQ8Warps - 1) cluster *= 2;
+  if (unit_chunks <= kQ8Keep * kQ8Warps * cluster && (a.weight == nullptr || w.tiles == 1)) {
+    w.cluster = cluster;
+    return w;
+  }
+  const long long chunks = w.units * unit_chunks;
+  if (chunks > 0x3fffffffLL) divide = false;             // chunk numbers stay in 32 bits
+  w.ctas = divide ? static_cast<int>(min((chunks + kQ8Warps - 1) / kQ8Warps, round)) : 0;
   w.pitch = (a.cache.S + 31LL) / 32 * 32;
+  const size_t slots = static_cast<size_t>(w.units + w.ctas) * w.tile_rows;
   size_t off = 0;
   w.ml_off = off;
-  off += up256(static_cast<size_t>(w.n_splits) * units * kQ8Rows * sizeof(float2));
+  off += up256(slots * sizeof(float2));
   w.o_off = off;
-  if (w.n_splits > 1) off += up256(static_cast<size_t>(w.n_splits) * units * kQ8Rows * a.D * sizeof(float));
+  if (divide) off += up256(slots * a.D * sizeof(float));
+  w.piece_off = off;
+  off += up256(static_cast<size_t>(w.units) * sizeof(int2));
   w.score_off = off;
   if (a.weight != nullptr) off += up256(static_cast<size_t>(a.B) * a.Hkv * R * w.pitch * sizeof(float));
-  w.total = off;
-  if (w.n_splits == 1 && a.weight == nullptr) w.total = 0;
+  w.total = divide || a.weight != nullptr ? off : 0;
   return w;
 }
 
-template <typename T, int D>
-int launch_typed(const TrnAttnQ8Args& a, cudaStream_t st, const DeviceState& ds) {
-  using SM = Q8Smem<D>;
+template <typename T, int D, int NT>
+int launch_tiles(const TrnAttnQ8Args& a, const Q8Plan& w, cudaStream_t st, const DeviceState& ds) {
+  using SM = Q8Smem<D, NT>;
   constexpr bool HILO = Io<T>::kFmt == 0;
-  const Q8Plan w = plan_of(a, kAttnNominalSMs, a.workspace != nullptr);
   Q8Params p{};
   p.q = a.q; p.o = a.o;
   CUtensorMap tm_k, tm_v;
@@ -575,7 +899,7 @@ int launch_typed(const TrnAttnQ8Args& a, cudaStream_t st, const DeviceState& ds)
   p.len = KvLen{a.kv_len, a.kv_len_all, a.cache.S};
   p.lse = a.lse;
   p.B = a.B; p.M = a.M; p.Hq = a.Hq; p.Hkv = a.Hkv; p.G = a.Hq / a.Hkv; p.R = a.M * p.G;
-  p.tiles = w.tiles; p.n_splits = w.n_splits;
+  p.tiles = w.tiles; p.tile_rows = w.tile_rows; p.ctas = w.ctas;
   p.causal = a.causal;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.shift = block_shift(a.cache.block);
@@ -583,26 +907,60 @@ int launch_typed(const TrnAttnQ8Args& a, cudaStream_t st, const DeviceState& ds)
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   if (w.total > 0) {
     p.part_ml = reinterpret_cast<float2*>(ws + w.ml_off);
-    if (w.n_splits > 1) p.part_o = reinterpret_cast<float*>(ws + w.o_off);
+    p.pieces = reinterpret_cast<int2*>(ws + w.piece_off);
+    if (w.ctas > 0) p.part_o = reinterpret_cast<float*>(ws + w.o_off);
     if (a.weight != nullptr) p.scores = reinterpret_cast<float*>(ws + w.score_off);
   }
   p.pitch = w.pitch;
   p.weight = a.weight; p.w_sb = a.weight_stride_b; p.w_sh = a.weight_stride_h; p.weight_add = a.weight_add;
-  const long long units = static_cast<long long>(a.B) * a.Hkv * w.tiles;
-  if (units * w.n_splits > 0x7fffffffLL) return TRN_E_SHAPE;
-  auto kern = attn_q8_kernel<T, D, HILO>;
+  if (w.units * max(w.cluster, 1) + w.ctas > 0x7fffffffLL) return TRN_E_SHAPE;
+  if (w.cluster > 0) {
+    auto kern = attn_q8_cluster_kernel<T, D, NT, HILO>;
+    rc = ensure_dyn_smem(reinterpret_cast<const void*>(kern), SM::kTotalKept, ds.device);
+    if (rc != TRN_OK) return rc;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(w.units * w.cluster), 1, 1);
+    cfg.blockDim = dim3(kQ8Threads, 1, 1);
+    cfg.dynamicSmemBytes = a.weight != nullptr ? SM::kTotalKept : SM::kTotal;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(w.cluster);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    TRN_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tm_k, tm_v, p, w.cluster));
+    return TRN_OK;
+  }
+  auto kern = attn_q8_kernel<T, D, NT, HILO>;
   rc = ensure_dyn_smem(reinterpret_cast<const void*>(kern), SM::kTotal, ds.device);
   if (rc != TRN_OK) return rc;
-  const long long merge = w.n_splits > 1 ? (static_cast<long long>(a.B) * a.Hkv * p.R + 7) / 8 : 0;
+  constexpr int kMergeRows = kQ8JoinThreads / (D / 2);
+  const long long merge = w.ctas > 0 ? w.units * max(w.tile_rows / kMergeRows, 1) : 0;
   const int longest = a.kv_len != nullptr ? a.cache.S : min(max(a.kv_len_all, 0), a.cache.S);
-  const int key_tiles = a.weight != nullptr ? (longest + kQ8JoinThreads - 1) / kQ8JoinThreads : 0;
+  const int key_tiles = a.weight != nullptr ? (longest + kQ8JoinKeys - 1) / kQ8JoinKeys : 0;
   const long long join = merge + static_cast<long long>(a.B) * a.Hkv * key_tiles;
   if (join > 0x7fffffffLL) return TRN_E_SHAPE;
-  TRN_CUDA_TRY(launch_pdl(kern, dim3(static_cast<unsigned>(units * w.n_splits)), dim3(kQ8Threads), SM::kTotal, st, tm_k, tm_v, p));
+  const unsigned grid = static_cast<unsigned>(w.ctas > 0 ? w.ctas : w.units);
+  TRN_CUDA_TRY(launch_pdl(kern, dim3(grid), dim3(kQ8Threads), SM::kTotal, st, tm_k, tm_v, p));
   if (join > 0)
     TRN_CUDA_TRY(launch_pdl(attn_q8_join_kernel<T, D>, dim3(static_cast<unsigned>(join)), dim3(kQ8JoinThreads),
-                            a.weight != nullptr ? p.R * sizeof(float) : 0, st, p, static_cast<int>(merge), max(key_tiles, 1)));
+                            a.weight != nullptr ? p.R * sizeof(float) : 0, st, p, static_cast<int>(merge),
+                            max(key_tiles, 1)));
   return TRN_OK;
+}
+
+template <typename T, int D>
+int launch_typed(const TrnAttnQ8Args& a, cudaStream_t st, const DeviceState& ds) {
+  const Q8Plan w = plan_of(a, kAttnNominalSMs, a.workspace != nullptr);
+  if (w.tile_rows == 8) return launch_tiles<T, D, 1>(a, w, st, ds);
+  if constexpr (q8_max_tiles(D) >= 4) {
+    if (w.tile_rows == 32) return launch_tiles<T, D, 4>(a, w, st, ds);
+  }
+  return launch_tiles<T, D, 2>(a, w, st, ds);
 }
 
 constexpr int kQ8MaxWeightQueries = 16;
@@ -637,7 +995,10 @@ int launch_attention_q8(const TrnAttnQ8Args& a, cudaStream_t st, const DeviceSta
 
 size_t attention_q8_workspace(const TrnAttnQ8Args& a) {
   if (a.B <= 0 || a.M <= 0 || a.Hq <= 0 || a.Hkv <= 0 || a.Hq % a.Hkv != 0 || a.cache.S <= 0 || (a.D != 64 && a.D != 128)) return 0;
-  return plan_of(a, kAttnNominalSMs, true).total;
+  TrnAttnQ8Args full = a;                      // whatever the sequences hold when the call comes
+  full.kv_len = nullptr;
+  full.kv_len_all = a.cache.S;
+  return plan_of(full, kAttnNominalSMs, true).total;
 }
 
 }  // namespace trn

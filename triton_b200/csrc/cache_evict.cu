@@ -18,7 +18,8 @@ namespace {
 
 constexpr int kEvMaxCluster = 8;
 constexpr int kEvMaxN = 262144;
-constexpr int kEvThreads = 512;
+constexpr int kEvThreads = 1024;
+constexpr int kEvAhead = 4;             // positions a thread sums side by side
 constexpr int kEvWarps = kEvThreads / 32;
 constexpr int kEvMoveThreads = 256;
 constexpr int kEvGroup16 = 64;          // destination positions per CTA of a 16-bit move
@@ -80,17 +81,23 @@ evict_select_kernel(const __grid_constant__ EvictParams p, int cluster) {
   }
   // ---- keys of this CTA's slice
   const float* sc = p.scores + b * p.sc_sb + static_cast<long long>(h) * p.group * p.sc_sh + lo;
-  for (int j = tid; j < cnt; j += kEvThreads) {
-    float w;
-    if (p.group == 1) {
-      w = sc[j];
-    } else {
-      double acc = 0.0;
-#pragma unroll 8
-      for (int g = 0; g < p.group; ++g) acc += static_cast<double>(sc[g * p.sc_sh + j]);
-      w = static_cast<float>(acc);
+  if (p.group == 1) {
+    for (int j = tid; j < cnt; j += kEvThreads) ev_keys[j] = order_key(sc[j]);
+  } else {
+    // kEvAhead positions at a time, so that enough loads are under way: a row's sum is one chain of Hs / Hkv adds
+    for (int j0 = tid; j0 < cnt; j0 += kEvAhead * kEvThreads) {
+      double acc[kEvAhead] = {};
+#pragma unroll 4
+      for (int g = 0; g < p.group; ++g) {
+        const float* src = sc + g * p.sc_sh + j0;
+#pragma unroll
+        for (int i = 0; i < kEvAhead; ++i)
+          if (j0 + i * kEvThreads < cnt) acc[i] += static_cast<double>(src[i * kEvThreads]);
+      }
+#pragma unroll
+      for (int i = 0; i < kEvAhead; ++i)
+        if (j0 + i * kEvThreads < cnt) ev_keys[j0 + i * kEvThreads] = order_key(static_cast<float>(acc[i]));
     }
-    ev_keys[j] = order_key(w);
   }
   if (tid < 256) hist[0][tid] = 0u;
   __syncthreads();
@@ -248,7 +255,7 @@ evict_move_kernel(const __grid_constant__ MoveParams p) {
   const int seg = tid % SEG;
   const uint8_t* s0 = static_cast<const uint8_t*>(src.ptr) + (b * src.stride_b + h * src.stride_h) * ELEM + seg * 16;
   uint8_t* d0 = static_cast<uint8_t*>(dst.ptr) + (b * dst.stride_b + h * dst.stride_h) * ELEM + seg * 16;
-#pragma unroll 2
+#pragma unroll 4
   for (int r = tid / SEG; r < g1 - g0; r += ROWS) {
     uint4 c = *reinterpret_cast<const uint4*>(s0 + from[r] * (src.stride_s * ELEM));
     if constexpr (Q8) {
@@ -336,9 +343,10 @@ int launch_cache_evict(const TrnCacheEvictArgs& a, cudaStream_t st, const Device
   const long long rows = static_cast<long long>(a.B) * a.Hkv;
   const int longest = a.kv_len != nullptr ? a.src.S : min(max(a.kv_len_all, 0), a.src.S);
 
-  // a cluster splits long rows while SMs are idle; a slice of 1024 positions is two keys a thread
+  // a cluster pays a barrier among its CTAs for each digit: it splits a row only where its scores are many (and SMs idle)
   int cluster = 1;
-  while (cluster < kEvMaxCluster && longest > 1024 * cluster && rows * cluster * 2 <= 2 * ds.sm_count) cluster *= 2;
+  const long long row_scores = static_cast<long long>(longest) * (a.Hs / a.Hkv);
+  while (cluster < kEvMaxCluster && row_scores > 8192LL * cluster && rows * cluster * 2 <= ds.sm_count) cluster *= 2;
   while (cluster < kEvMaxCluster && longest > 32768 * cluster) cluster *= 2;      // 128 KB of keys at most
   EvictParams p{};
   p.scores = a.scores;

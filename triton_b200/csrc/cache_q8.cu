@@ -48,7 +48,6 @@ cache_append_kernel(const __grid_constant__ AppendParams p) {
   const float s_old = older > 0 ? *slot : 0.f;
 
   uint4 x[VPT];
-  float amax = 0.f;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int v = i * kAppendThreads + static_cast<int>(threadIdx.x);
@@ -57,23 +56,43 @@ cache_append_kernel(const __grid_constant__ AppendParams p) {
     if (row >= older && first + row < end)
       x[i] = *reinterpret_cast<const uint4*>(x0 + (first + row - held) * src.stride_s + seg * 8);
   }
+  // largest magnitude: the bits without the sign order as the values do, two at a time; what is not finite has all
+  // exponent bits set and sends the block through the loop that leaves such elements out
+  __shared__ uint32_t part[kAppendThreads / 32];
+  auto block_max = [&](uint32_t m) {
+    m = max(m & 0xffffu, m >> 16);
+    m = __reduce_max_sync(0xffffffffu, m);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
+    __syncthreads();                                                     // also: every thread has read the old scale
+#pragma unroll
+    for (int i = 0; i < kAppendThreads / 32; ++i) m = max(m, part[i]);
+    return m;
+  };
+  constexpr uint32_t kInf = Io<T>::kFmt == 1 ? 0x7f80u : 0x7c00u;
+  uint32_t top = 0u;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 f = Io<T>::unpack2(w[e]);
-      if (fabsf(f.x) <= FLT_MAX) amax = fmaxf(amax, fabsf(f.x));
-      if (fabsf(f.y) <= FLT_MAX) amax = fmaxf(amax, fabsf(f.y));
-    }
+    top = __vmaxu2(top, __vmaxu2(x[i].x & 0x7fff7fffu, x[i].y & 0x7fff7fffu));
+    top = __vmaxu2(top, __vmaxu2(x[i].z & 0x7fff7fffu, x[i].w & 0x7fff7fffu));
   }
-  __shared__ float part[kAppendThreads / 32];
+  top = block_max(top);
+  const bool all_finite = top < kInf;
+  if (!all_finite) {
+    top = 0u;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = amax;
-  __syncthreads();                                                       // also: every thread has read the old scale
+    for (int i = 0; i < VPT; ++i) {
+      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
 #pragma unroll
-  for (int i = 0; i < kAppendThreads / 32; ++i) amax = fmaxf(amax, part[i]);
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t a = w[e] & 0x7fffu, c = (w[e] >> 16) & 0x7fffu;
+        if (a < kInf) top = max(top, a);
+        if (c < kInf) top = max(top, c);
+      }
+    }
+    __syncthreads();                                                     // part is free again
+    top = block_max(top);
+  }
+  const float amax = Io<T>::unpack2(top).x;
   const float need = exp2_int(scale_exp(amax));
   const bool grew = !(s_old >= need);
   const float s = grew ? need : s_old;
@@ -99,7 +118,7 @@ cache_append_kernel(const __grid_constant__ AppendParams p) {
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        f[e] = fabsf(f[e]) <= FLT_MAX ? f[e] : __uint_as_float(0x7fffffffu);
+        if (!all_finite) f[e] = fabsf(f[e]) <= FLT_MAX ? f[e] : __uint_as_float(0x7fffffffu);
         f[e] = pow2 ? f[e] * inv : __fdiv_rn(f[e], s);
       }
     } else {

@@ -394,17 +394,18 @@ class _BoundCall:
     def _bind(self, name: str, args, keep) -> None:
         self._keep = [t for t in keep if t is not None]
         _one_device(*self._keep)
-        self.device = self._keep[0].device
+        self._index = self._keep[0].device.index
         self.args = args
         self._ref = C.byref(args)
         self._fn = getattr(L.load(), name)
 
     def run(self) -> None:
-        if torch.cuda.current_device() == self.device.index:
-            rc = self._fn(self._ref, _stream())
+        # the raw-handle forms of current_device() and current_stream(): a decode step is a few microseconds of work
+        if torch._C._cuda_getDevice() == self._index:
+            rc = self._fn(self._ref, torch._C._cuda_getCurrentRawStream(self._index))
         else:
-            with torch.cuda.device(self.device):
-                rc = self._fn(self._ref, _stream())
+            with torch.cuda.device(self._index):
+                rc = self._fn(self._ref, torch._C._cuda_getCurrentRawStream(self._index))
         if rc != 0:
             L.check(rc)
 

@@ -28,10 +28,7 @@
 // What must not be seen cannot hurt: scores behind a row's last position are replaced, not weighted, and in the
 // chunks where that happens NaN codes of v are taken as 0 in the product (0 * NaN would poison rows that do not see them) and
 // put back as NaN into the outputs of the rows that do.
-#include <math.h>
-
-#include "attn_common.cuh"
-#include "q8.cuh"
+#include "attn_q8.cuh"
 #include "small_mma.cuh"
 
 namespace trn {
@@ -41,9 +38,7 @@ constexpr int kQ8Warps = 4;
 constexpr int kQ8Threads = 32 * kQ8Warps;
 constexpr int kQ8Keys = 32;                    // positions per chunk
 constexpr int kQ8Stages = 2;
-constexpr float kQ8PBias = 12.f;               // log2 of the factor P' carries into the product
 constexpr float kQ8Slack = 3.f;                // log2 of how far a score may pass the running maximum (2^15 fits fp16)
-constexpr float kMinVScale = 7.888609052210118e-31f;   // 2^-100: smaller scales (a block of zeros) count as this
 constexpr int kQ8MaxCluster = 8;
 constexpr int kQ8Keep = 4;                     // chunks a warp of a cluster takes at most
 constexpr int kQ8TargetCtas = 3;               // resident CTAs per SM (shared memory)
@@ -73,29 +68,6 @@ struct Q8Smem {
   static constexpr int kTotalKept = kTotal + kQ8Warps * kRows * kKeptPitch * 4;
 };
 
-struct Q8Params {
-  TrnHeadTensor q, o;
-  HeadMapInfo ki, vi;
-  ScaleTable ks, vs;
-  KvLen len;
-  float* lse;
-  int B, M, Hq, Hkv, G, R;                     // R = M * G rows per (b, kv head): row r = query r / G, head r % G
-  int tiles, tile_rows;                        // row tiles per (b, kv head), rows of one
-  int causal;
-  float scale_log2;
-  int shift;                                   // log2(block)
-  int ctas;                                    // CTAs the chunks are dealt out to; 0: a CTA per unit, nothing divided
-  float* part_o;                               // [units + ctas][tile_rows][D], units = B * Hkv * tiles
-  float2* part_ml;                             // [units + ctas][tile_rows]; without division [units][tile_rows] or NULL
-  int2* pieces;                                // [units] CTAs of a unit's first and last piece
-  float* scores;                               // [B * Hkv][R][pitch], log2 domain, or NULL
-  long long pitch;
-  float* weight;
-  long long w_sb, w_sh;
-  int weight_add;
-  int* status;
-};
-
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
@@ -105,10 +77,6 @@ __device__ __forceinline__ uint2 lds64(uint32_t a) {
   uint2 v;
   asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
   return v;
-}
-// 0xff in every byte of w that holds a NaN code (0x7f or 0xff)
-__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
-  return ((((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu;
 }
 // byte offset of 16-byte unit u of row r in a tile as TMA wrote it: 128-byte rows with the 128-byte swizzle, 64-byte rows
 // with the 64-byte swizzle
@@ -141,26 +109,11 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-// log2 and reciprocal of a scale: exact for powers of two
-__device__ __forceinline__ void scale_log_inv(float s, float& lg, float& inv) {
-  const uint32_t u = __float_as_uint(s);
-  if ((u & 0x7fffffu) == 0u && u - (1u << 23) < (252u << 23)) {       // 2^-126 .. 2^125
-    lg = static_cast<float>(static_cast<int>(u >> 23) - 127);
-    inv = __uint_as_float((254u << 23) - u);
-  } else {
-    lg = log2f(s);
-    inv = 1.0f / s;
-  }
-}
-
 // ---- who does what.  A unit is a (b, kv head, row tile) with the chunks its sequence holds (one where it holds none, to write
 // the empty rows; a tile whose rows do not see the last ones skips them).  All units' chunks, in order, are dealt out in equal
 // contiguous shares, so a CTA's share may end one unit and begin others, and a unit lies on CTAs [first, last]: pieces.
 // Each new piece begins a new unit, a new CTA or both, so slot = unit + CTA numbers the pieces' partial results, a
 // unit's side by side.
-__device__ __forceinline__ int last_seen(const Q8Params& p, int n, int r) {      // by row r of a (b, kv head); -1: nothing
-  return p.causal ? max(n - p.M + r / p.G, -1) : n - 1;
-}
 __device__ __forceinline__ int chunks_of(int n) { return max((n + kQ8Keys - 1) / kQ8Keys, 1); }
 // chunks of the sequences before b and of all, for one (kv head, row tile) (a whole warp, same arguments)
 __device__ __forceinline__ int2 chunks_before(const Q8Params& p, int b) {
@@ -531,18 +484,6 @@ __device__ __forceinline__ bool q8_begin(const Q8Params& p, const CUtensorMap& t
   return *reinterpret_cast<volatile int*>(p.status) != 0;
 }
 
-// CW columns of a finished row, and its log-sum-exp
-template <typename T, int CW>
-__device__ __forceinline__ void q8_store_row(const Q8Params& p, int b, int h, int r, int c0, const float* acc, float mx, float tot) {
-  const int i = r / p.G, hq = h * p.G + r % p.G;
-  const float inv = tot == 0.f ? 0.f : 1.0f / tot;
-  T* dst = static_cast<T*>(p.o.ptr) + b * p.o.stride_b + static_cast<long long>(i) * p.o.stride_s +
-           static_cast<long long>(hq) * p.o.stride_h + c0;
-#pragma unroll
-  for (int c = 0; c < CW; c += 2) *reinterpret_cast<uint32_t*>(dst + c) = Io<T>::pack2(acc[c] * inv, acc[c + 1] * inv);
-  if (c0 == 0 && p.lse != nullptr) p.lse[(static_cast<long long>(b) * p.Hq + hq) * p.M + i] = mx - kQ8PBias + log2f(tot);
-}
-
 // Long caches: each CTA takes its share of all chunks, a piece of a unit after the other.
 template <typename T, int D, int NT, bool HILO>
 __global__ void __launch_bounds__(kQ8Threads)
@@ -839,8 +780,6 @@ attn_q8_join_kernel(const __grid_constant__ Q8Params p, int merge_ctas, int key_
     if (key + e < n) w[e] = p.weight_add ? w[e] + acc[e] : acc[e];
 }
 
-size_t up256(size_t v) { return (v + 255) / 256 * 256; }
-
 struct Q8Plan {
   int tiles, tile_rows, ctas, cluster;         // cluster > 0: one launch of clusters, no scratch
   long long units;
@@ -889,21 +828,12 @@ template <typename T, int D, int NT>
 int launch_tiles(const TrnAttnQ8Args& a, const Q8Plan& w, cudaStream_t st, const DeviceState& ds) {
   using SM = Q8Smem<D, NT>;
   constexpr bool HILO = Io<T>::kFmt == 0;
-  Q8Params p{};
-  p.q = a.q; p.o = a.o;
+  Q8Params p = q8_params(a, ds);
   CUtensorMap tm_k, tm_v;
   int rc = make_code_tmap(&tm_k, &p.ki, a.cache.k, a.cache.S, a.Hkv, a.B, D, kQ8Keys);
   if (rc == TRN_OK) rc = make_code_tmap(&tm_v, &p.vi, a.cache.v, a.cache.S, a.Hkv, a.B, D, kQ8Keys);
   if (rc != TRN_OK) return rc;
-  p.ks = scale_table(a.cache.k_scale); p.vs = scale_table(a.cache.v_scale);
-  p.len = KvLen{a.kv_len, a.kv_len_all, a.cache.S};
-  p.lse = a.lse;
-  p.B = a.B; p.M = a.M; p.Hq = a.Hq; p.Hkv = a.Hkv; p.G = a.Hq / a.Hkv; p.R = a.M * p.G;
   p.tiles = w.tiles; p.tile_rows = w.tile_rows; p.ctas = w.ctas;
-  p.causal = a.causal;
-  p.scale_log2 = a.scale * 1.4426950408889634f;
-  p.shift = block_shift(a.cache.block);
-  p.status = ds.status;
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   if (w.total > 0) {
     p.part_ml = reinterpret_cast<float2*>(ws + w.ml_off);
@@ -912,7 +842,6 @@ int launch_tiles(const TrnAttnQ8Args& a, const Q8Plan& w, cudaStream_t st, const
     if (a.weight != nullptr) p.scores = reinterpret_cast<float*>(ws + w.score_off);
   }
   p.pitch = w.pitch;
-  p.weight = a.weight; p.w_sb = a.weight_stride_b; p.w_sh = a.weight_stride_h; p.weight_add = a.weight_add;
   if (w.units * max(w.cluster, 1) + w.ctas > 0x7fffffffLL) return TRN_E_SHAPE;
   if (w.cluster > 0) {
     auto kern = attn_q8_cluster_kernel<T, D, NT, HILO>;
@@ -938,18 +867,9 @@ int launch_tiles(const TrnAttnQ8Args& a, const Q8Plan& w, cudaStream_t st, const
   auto kern = attn_q8_kernel<T, D, NT, HILO>;
   rc = ensure_dyn_smem(reinterpret_cast<const void*>(kern), SM::kTotal, ds.device);
   if (rc != TRN_OK) return rc;
-  constexpr int kMergeRows = kQ8JoinThreads / (D / 2);
-  const long long merge = w.ctas > 0 ? w.units * max(w.tile_rows / kMergeRows, 1) : 0;
-  const int longest = a.kv_len != nullptr ? a.cache.S : min(max(a.kv_len_all, 0), a.cache.S);
-  const int key_tiles = a.weight != nullptr ? (longest + kQ8JoinKeys - 1) / kQ8JoinKeys : 0;
-  const long long join = merge + static_cast<long long>(a.B) * a.Hkv * key_tiles;
-  if (join > 0x7fffffffLL) return TRN_E_SHAPE;
   const unsigned grid = static_cast<unsigned>(w.ctas > 0 ? w.ctas : w.units);
   TRN_CUDA_TRY(launch_pdl(kern, dim3(grid), dim3(kQ8Threads), SM::kTotal, st, tm_k, tm_v, p));
-  if (join > 0)
-    TRN_CUDA_TRY(launch_pdl(attn_q8_join_kernel<T, D>, dim3(static_cast<unsigned>(join)), dim3(kQ8JoinThreads),
-                            a.weight != nullptr ? p.R * sizeof(float) : 0, st, p, static_cast<int>(merge),
-                            max(key_tiles, 1)));
+  if (w.ctas > 0 || a.weight != nullptr) return launch_q8_join(p, a, w.ctas > 0, st);
   return TRN_OK;
 }
 
@@ -963,10 +883,31 @@ int launch_typed(const TrnAttnQ8Args& a, cudaStream_t st, const DeviceState& ds)
   return launch_tiles<T, D, 2>(a, w, st, ds);
 }
 
+template <typename T, int D>
+int launch_join(const Q8Params& p, const TrnAttnQ8Args& a, bool merge, cudaStream_t st) {
+  constexpr int kMergeRows = kQ8JoinThreads / (D / 2);
+  const long long units = static_cast<long long>(a.B) * a.Hkv * p.tiles;
+  const long long merge_ctas = merge ? units * max(p.tile_rows / kMergeRows, 1) : 0;
+  const int longest = a.kv_len != nullptr ? a.cache.S : min(max(a.kv_len_all, 0), a.cache.S);
+  const int key_tiles = a.weight != nullptr ? (longest + kQ8JoinKeys - 1) / kQ8JoinKeys : 0;
+  const long long grid = merge_ctas + static_cast<long long>(a.B) * a.Hkv * key_tiles;
+  if (grid > 0x7fffffffLL) return TRN_E_SHAPE;
+  if (grid > 0)
+    TRN_CUDA_TRY(launch_pdl(attn_q8_join_kernel<T, D>, dim3(static_cast<unsigned>(grid)), dim3(kQ8JoinThreads),
+                            a.weight != nullptr ? p.R * sizeof(float) : 0, st, p, static_cast<int>(merge_ctas), max(key_tiles, 1)));
+  return TRN_OK;
+}
+
 constexpr int kQ8MaxWeightQueries = 16;
 constexpr int kQ8MaxWeightRows = 8192;         // their log-sum-exps lie in 32 KB of shared memory
 
 }  // namespace
+
+int launch_q8_join(const Q8Params& p, const TrnAttnQ8Args& a, bool merge, cudaStream_t st) {
+  if (a.dtype == TRN_BF16)
+    return a.D == 128 ? launch_join<__nv_bfloat16, 128>(p, a, merge, st) : launch_join<__nv_bfloat16, 64>(p, a, merge, st);
+  return a.D == 128 ? launch_join<__half, 128>(p, a, merge, st) : launch_join<__half, 64>(p, a, merge, st);
+}
 
 int check_attention_q8(const TrnAttnQ8Args& a) {
   if (a.dtype != TRN_BF16 && a.dtype != TRN_FP16) return TRN_E_DTYPE;
@@ -981,13 +922,16 @@ int check_attention_q8(const TrnAttnQ8Args& a) {
     if (a.M > kQ8MaxWeightQueries || a.M * (a.Hq / a.Hkv) > kQ8MaxWeightRows) return TRN_E_SHAPE;
     if ((a.B > 1 && a.weight_stride_b < 1) || (a.Hkv > 1 && a.weight_stride_h < 1)) return TRN_E_SHAPE;
   }
-  const Q8Plan w = plan_of(a, kAttnNominalSMs, a.workspace != nullptr);
-  if (w.total > 0 && (a.workspace == nullptr || (reinterpret_cast<uintptr_t>(a.workspace) & 255u) != 0 || a.workspace_bytes < w.total))
-    return TRN_E_WORKSPACE;
+  // scratch: needed where weights are summed from kept scores, else optional; what is given has to be right
+  const bool tc = attn_q8_tc_applies(a);
+  const size_t need = tc ? attn_q8_tc_workspace(a) : plan_of(a, kAttnNominalSMs, a.workspace != nullptr).total;
+  if (a.workspace != nullptr && ((reinterpret_cast<uintptr_t>(a.workspace) & 255u) != 0 || a.workspace_bytes < need)) return TRN_E_WORKSPACE;
+  if (a.workspace == nullptr && !tc && need > 0) return TRN_E_WORKSPACE;
   return TRN_OK;
 }
 
 int launch_attention_q8(const TrnAttnQ8Args& a, cudaStream_t st, const DeviceState& ds) {
+  if (attn_q8_tc_applies(a)) return launch_attn_q8_tc(a, st, ds);
   if (a.dtype == TRN_BF16)
     return a.D == 128 ? launch_typed<__nv_bfloat16, 128>(a, st, ds) : launch_typed<__nv_bfloat16, 64>(a, st, ds);
   return a.D == 128 ? launch_typed<__half, 128>(a, st, ds) : launch_typed<__half, 64>(a, st, ds);
@@ -998,7 +942,7 @@ size_t attention_q8_workspace(const TrnAttnQ8Args& a) {
   TrnAttnQ8Args full = a;                      // whatever the sequences hold when the call comes
   full.kv_len = nullptr;
   full.kv_len_all = a.cache.S;
-  return plan_of(full, kAttnNominalSMs, true).total;
+  return attn_q8_tc_applies(full) ? attn_q8_tc_workspace(full) : plan_of(full, kAttnNominalSMs, true).total;
 }
 
 }  // namespace trn

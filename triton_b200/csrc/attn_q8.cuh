@@ -1,0 +1,95 @@
+// Pieces shared by the two kernels of the attention over the 8-bit cache (attn_q8.cu: few query rows per kv head, bound by
+// memory; attn_q8_tc.cu: many, on the tensor cores of the 5th generation) and the merge of their partial results.
+#pragma once
+
+#include <math.h>
+
+#include "attn_common.cuh"
+#include "q8.cuh"
+
+namespace trn {
+
+constexpr float kQ8PBias = 12.f;               // log2 of the factor P' carries into the product
+constexpr float kMinVScale = 7.888609052210118e-31f;   // 2^-100: smaller scales (a block of zeros) count as this
+
+struct Q8Params {
+  TrnHeadTensor q, o;
+  HeadMapInfo ki, vi;
+  ScaleTable ks, vs;
+  KvLen len;
+  float* lse;
+  int B, M, Hq, Hkv, G, R;                     // R = M * G rows per (b, kv head): row r = query r / G, head r % G
+  int tiles, tile_rows;                        // row tiles per (b, kv head), rows of one
+  int causal;
+  float scale_log2;
+  int shift;                                   // log2(block)
+  int ctas;                                    // CTAs the chunks are dealt out to; 0: a CTA per unit, nothing divided
+  float* part_o;                               // [units + ctas][tile_rows][D], units = B * Hkv * tiles
+  float2* part_ml;                             // [units + ctas][tile_rows]; without division [units][tile_rows] or NULL
+  int2* pieces;                                // [units] CTAs of a unit's first and last piece
+  float* scores;                               // [B * Hkv][R][pitch], log2 domain, or NULL
+  long long pitch;
+  float* weight;
+  long long w_sb, w_sh;
+  int weight_add;
+  int* status;
+};
+
+// merge of the pieces (merge: whether there are any) and weights of the positions, by the kernel in attn_q8.cu
+int launch_q8_join(const Q8Params& p, const TrnAttnQ8Args& a, bool merge, cudaStream_t st);
+// many query rows per kv head (attn_q8_tc.cu): whether that kernel takes the call, its scratch, its launch
+bool attn_q8_tc_applies(const TrnAttnQ8Args& a);
+size_t attn_q8_tc_workspace(const TrnAttnQ8Args& a);
+int launch_attn_q8_tc(const TrnAttnQ8Args& a, cudaStream_t st, const DeviceState& ds);
+
+namespace {
+
+__device__ __forceinline__ int last_seen(const Q8Params& p, int n, int r) {      // by row r of a (b, kv head); -1: nothing
+  return p.causal ? max(n - p.M + r / p.G, -1) : n - 1;
+}
+// log2 and reciprocal of a scale: exact for powers of two
+__device__ __forceinline__ void scale_log_inv(float s, float& lg, float& inv) {
+  const uint32_t u = __float_as_uint(s);
+  if ((u & 0x7fffffu) == 0u && u - (1u << 23) < (252u << 23)) {       // 2^-126 .. 2^125
+    lg = static_cast<float>(static_cast<int>(u >> 23) - 127);
+    inv = __uint_as_float((254u << 23) - u);
+  } else {
+    lg = log2f(s);
+    inv = 1.0f / s;
+  }
+}
+// 0xff in every byte of w that holds a NaN code (0x7f or 0xff)
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
+  return ((((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu;
+}
+// CW columns of a finished row, and its log-sum-exp
+template <typename T, int CW>
+__device__ __forceinline__ void q8_store_row(const Q8Params& p, int b, int h, int r, int c0, const float* acc, float mx, float tot) {
+  const int i = r / p.G, hq = h * p.G + r % p.G;
+  const float inv = tot == 0.f ? 0.f : 1.0f / tot;
+  T* dst = static_cast<T*>(p.o.ptr) + b * p.o.stride_b + static_cast<long long>(i) * p.o.stride_s +
+           static_cast<long long>(hq) * p.o.stride_h + c0;
+#pragma unroll
+  for (int c = 0; c < CW; c += 2) *reinterpret_cast<uint32_t*>(dst + c) = Io<T>::pack2(acc[c] * inv, acc[c + 1] * inv);
+  if (c0 == 0 && p.lse != nullptr) p.lse[(static_cast<long long>(b) * p.Hq + hq) * p.M + i] = mx - kQ8PBias + log2f(tot);
+}
+
+inline size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+// the parts of a call's parameters that do not depend on the kernel
+inline Q8Params q8_params(const TrnAttnQ8Args& a, const DeviceState& ds) {
+  Q8Params p{};
+  p.q = a.q; p.o = a.o;
+  p.ks = scale_table(a.cache.k_scale); p.vs = scale_table(a.cache.v_scale);
+  p.len = KvLen{a.kv_len, a.kv_len_all, a.cache.S};
+  p.lse = a.lse;
+  p.B = a.B; p.M = a.M; p.Hq = a.Hq; p.Hkv = a.Hkv; p.G = a.Hq / a.Hkv; p.R = a.M * p.G;
+  p.causal = a.causal;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.shift = block_shift(a.cache.block);
+  p.status = ds.status;
+  p.weight = a.weight; p.w_sb = a.weight_stride_b; p.w_sh = a.weight_stride_h; p.weight_add = a.weight_add;
+  return p;
+}
+
+}  // namespace
+}  // namespace trn

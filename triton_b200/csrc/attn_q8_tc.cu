@@ -1,0 +1,618 @@
+// Attention over the 8-bit key/value cache for many query rows per kv head (prompts, chunks, many heads on one kv head): the
+// mathematics of attn_q8.cu on tcgen05 tensor cores.
+//
+// The M * Hq / Hkv rows of a (b, kv head) are taken in tiles of 128 (row r = query r / G, head r % G, so a tile of a causal
+// call spans few queries); a CTA works on two neighbouring tiles against the same keys, so that one tile's softmax runs
+// while the other's products do.
+//   warps 0-3    convert: fetch the next 128 positions' codes into registers, and when a stage is free write them as fp16
+//                into the 128-byte-swizzled tiles the tensor core reads (exact), with the scales of their 16-position groups
+//   warps 4-7,   softmax of tile 0 / 1, one thread per row: q -> shared memory as fp16 times a power of two; then per block of
+//   warps 8-11   128 positions  t' = s * (c ks) + log2 vs,  P' = 2^(t' - m'), packed to fp16 over s in tensor memory,
+//                l += P' / vs;  o is rescaled only when a row's maximum grew by more than 2^8 since the last time
+//   warp 12      issues S_t = q_t k^T and O_t += P'_t v (P' from tensor memory)
+// The scales cost nothing per score: ks and log2 vs change every 16 columns at most and enter the multiply-add that the
+// softmax makes anyway.  bf16 outputs take P' as one fp16 part, fp16 outputs as hi + lo (see attn_q8.cu).
+// Few CTAs (less than one for each SM): the key blocks are divided among several, merged by the kernel in attn_q8.cu.
+//
+// Algorithmic flops: 4 * D per visible (row, position).
+#include <type_traits>
+
+#include "attn_q8.cuh"
+
+namespace trn {
+namespace {
+
+constexpr int kTcRows = 128, kTcKeys = 128;
+constexpr int kTcThreads = 13 * 32;
+constexpr int kTcMmaWarp = 12;
+constexpr int kTcTmemCols = 512;              // S0 [0,128) S1 [128,256) O0 [256,256+D) O1 [384,384+D)
+constexpr float kTcRescale = 8.0f;            // log2 units a row's maximum may pass the offset in use
+constexpr float kTcPBias = 6.0f;              // P' <= 2^14 with it
+constexpr int kTcMaxSplits = 16;
+
+struct TcParams {
+  Q8Params c;
+  TrnHeadTensor k, v;
+  int pairs, n_splits;
+};
+
+template <int D>
+struct TcSmem {
+  static constexpr int kStages = D == 128 ? 2 : 4;
+  static constexpr int kChunks = D / 64;
+  static constexpr int kChunkBytes = 128 * 128;            // 128 rows x 64 fp16
+  static constexpr int kTile = kChunks * kChunkBytes;
+  static constexpr int kQ = 0;                             // two q tiles
+  static constexpr int kKV = 2 * kTile;
+  static constexpr int kScales = kKV + kStages * 2 * kTile;          // [stage][8 groups] (ks, log2 vs, 1 / vs, -)
+  static constexpr int kNan = kScales + kStages * 8 * 16;            // [D] first position with a NaN code in v
+  static constexpr int kBars = kNan + D * 4;
+  static constexpr int kTotal = kBars + 256 + 1024;
+};
+
+// 16 codes -> 16 fp16: units `first` and `first ^ 1` of the row, in an order in which 8 lanes' stores meet all banks
+__device__ __forceinline__ void expand16(uint32_t tile, uint32_t row, uint32_t unit, bool swap, const uint4& c) {
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+  uint32_t r[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    r[2 * i] = e4m3x2_to_f16x2(w[i]);
+    r[2 * i + 1] = e4m3x2_to_f16x2(w[i] >> 16);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const bool hi = (i != 0) != swap;
+    const uint32_t a = tile + swz128(row, unit + (hi ? 1u : 0u));
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};"
+                 ::"r"(a), "r"(hi ? r[4] : r[0]), "r"(hi ? r[5] : r[1]), "r"(hi ? r[6] : r[2]), "r"(hi ? r[7] : r[3])
+                 : "memory");
+  }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kTcThreads, 1)
+attn_q8_tc_kernel(const __grid_constant__ TcParams tp) {
+  using SM = TcSmem<D>;
+  constexpr int KS = SM::kStages;
+  constexpr bool SPLIT = Io<T>::kFmt == 0;
+  const Q8Params& p = tp.c;
+  extern __shared__ uint8_t tc_smem_raw[];
+  const uint32_t base = (smem_u32(tc_smem_raw) + 1023u) & ~1023u;
+  uint8_t* gen = tc_smem_raw + (base - smem_u32(tc_smem_raw));
+  const uint32_t bars = base + SM::kBars;
+  auto k_full = [&](int s) { return bars + 8u * s; };
+  auto v_full = [&](int s) { return bars + 8u * (KS + s); };
+  auto kv_empty = [&](int s) { return bars + 8u * (2 * KS + s); };
+  auto s_full = [&](int t) { return bars + 8u * (3 * KS + t); };
+  auto pv_done = [&](int t) { return bars + 8u * (3 * KS + 2 + t); };
+  auto q_full = [&](int t) { return bars + 8u * (3 * KS + 4 + t); };
+  // P' becomes ready in two halves (positions 0..63, 64..127), so that P' v starts on the first
+  auto p_ready = [&](int t, int half) { return bars + 8u * (3 * KS + 6 + 2 * t + half); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + SM::kBars + 8 * (3 * KS + 10));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* nan_any = reinterpret_cast<int*>(tmem_slot + 2);
+  int* nan_from = reinterpret_cast<int*>(gen + SM::kNan);
+  float4* scales = reinterpret_cast<float4*>(gen + SM::kScales);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Ctl ctl{p.status, abort_flag};
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < KS; ++s) {
+      mbar_init(k_full(s), 128);
+      mbar_init(v_full(s), 128);
+      mbar_init(kv_empty(s), 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(s_full(t), 1);
+      mbar_init(pv_done(t), 1);
+      mbar_init(q_full(t), 128);
+      mbar_init(p_ready(t, 0), 128);
+      mbar_init(p_ready(t, 1), 128);
+    }
+    *abort_flag = 0;
+    *nan_any = 0;
+    fence_mbar_init();
+  }
+  for (int i = threadIdx.x; i < D; i += kTcThreads) nan_from[i] = 0x7fffffff;
+  if (warp == kTcMmaWarp) {
+    tmem_alloc(smem_u32(tmem_slot), kTcTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+  griddep_wait();                              // q, the codes and the lengths may come from the launch before
+  griddep_launch();
+  const bool dead = *reinterpret_cast<volatile int*>(p.status) != 0;
+
+  // ---- which rows and blocks: late (heavy) pairs of tiles first
+  const int per_split = p.B * p.Hkv * tp.pairs;
+  const int split = static_cast<int>(blockIdx.x) / per_split, cta = static_cast<int>(blockIdx.x) % per_split;
+  const int pair = tp.pairs - 1 - cta / (p.B * p.Hkv), bh = cta % (p.B * p.Hkv);
+  const int b = bh / p.Hkv, h = bh % p.Hkv;
+  const int n = p.len(b);
+  int n_blocks[2], lim_max[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int r0 = (2 * pair + t) * kTcRows;
+    lim_max[t] = r0 < p.R ? last_seen(p, n, min(r0 + kTcRows, p.R) - 1) : -1;
+    n_blocks[t] = (lim_max[t] + kTcKeys) / kTcKeys;
+  }
+  int j0 = 0;
+  if (tp.n_splits > 1) {
+    const int full = max(n_blocks[0], n_blocks[1]);
+    j0 = full * split / tp.n_splits;
+    const int j1 = full * (split + 1) / tp.n_splits;
+    n_blocks[0] = max(0, min(j1, n_blocks[0]) - j0);
+    n_blocks[1] = max(0, min(j1, n_blocks[1]) - j0);
+  }
+  if (dead) n_blocks[0] = n_blocks[1] = 0;
+  const int n_max = max(n_blocks[0], n_blocks[1]);
+  const int first_lim = last_seen(p, n, 2 * pair * kTcRows);       // of the CTA's first row: the least any row sees
+  auto q_s = [&](int t) { return base + SM::kQ + t * SM::kTile; };
+  auto k_s = [&](int s) { return base + SM::kKV + s * 2 * SM::kTile; };
+  auto v_s = [&](int s) { return k_s(s) + SM::kTile; };
+
+  if (warp < 4) {
+    // ------------------------------- convert -------------------------------
+    constexpr int SEG = D / 16, RP = 128 / SEG, NP = 128 / RP;     // lanes per row, rows per pass, passes
+    const int row0 = static_cast<int>(threadIdx.x) / SEG, seg = static_cast<int>(threadIdx.x) % SEG;
+    const uint32_t chunk = static_cast<uint32_t>(seg >> 2) * SM::kChunkBytes, unit = static_cast<uint32_t>(seg & 3) * 2u;
+    const bool swap = seg >= 4;
+    const uint8_t* kb = static_cast<const uint8_t*>(tp.k.ptr) + b * tp.k.stride_b + h * tp.k.stride_h + seg * 16;
+    const uint8_t* vb = static_cast<const uint8_t*>(tp.v.ptr) + b * tp.v.stride_b + h * tp.v.stride_h + seg * 16;
+    uint4 kr[NP], vr[NP];
+    float ks = 1.f, vs = 1.f;
+    auto fetch = [&](uint4 (&r)[NP], const uint8_t* src, long long stride, int j) {
+      const int kv0 = (j0 + j) * kTcKeys;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const int key = kv0 + i * RP + row0;
+        r[i] = make_uint4(0u, 0u, 0u, 0u);                         // behind the sequence: zeros, whatever lies there
+        if (key < n) r[i] = *reinterpret_cast<const uint4*>(src + key * stride);
+      }
+    };
+    auto fetch_scales = [&](int j) {
+      const int key = (j0 + j) * kTcKeys + 16 * static_cast<int>(threadIdx.x);
+      if (threadIdx.x < 8) {
+        ks = key < n ? *p.ks.at(b, key >> p.shift, h) : 1.f;
+        vs = key < n ? *p.vs.at(b, key >> p.shift, h) : 1.f;
+      }
+    };
+    if (n_max > 0) {
+      fetch_scales(0);
+      fetch(kr, kb, tp.k.stride_s, 0);
+      fetch(vr, vb, tp.v.stride_s, 0);
+    }
+    for (int j = 0; j < n_max; ++j) {
+      const int st = j % KS, kv0 = (j0 + j) * kTcKeys;
+      bool ok = mbar_wait(kv_empty(st), ((j / KS) & 1) ^ 1u, ctl, KST_TIMEOUT_PRODUCER);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if (threadIdx.x < 8) {
+        float lg, inv;
+        scale_log_inv(vs < kMinVScale ? kMinVScale : vs, lg, inv);
+        scales[st * 8 + threadIdx.x] = make_float4(ks, lg, inv, 0.f);
+      }
+#pragma unroll
+      for (int i = 0; i < NP; ++i) expand16(k_s(st) + chunk, i * RP + row0, unit, swap, kr[i]);
+      fence_proxy_async_smem();
+      mbar_arrive(k_full(st));
+      if (j + 1 < n_max) {
+        fetch_scales(j + 1);
+        fetch(kr, kb, tp.k.stride_s, j + 1);
+      }
+      if (kv0 + kTcKeys - 1 > first_lim) {
+        // some row does not see some position: NaN codes of v count as 0 in the product, their first positions are kept
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t bad = nan_bytes(w[e]);
+            if (bad != 0u) {
+              w[e] &= ~bad;
+              *nan_any = 1;
+              for (int c = 0; c < 4; ++c)
+                if ((bad >> (8 * c)) & 1u) atomicMin(&nan_from[seg * 16 + 4 * e + c], kv0 + i * RP + row0);
+            }
+          }
+          vr[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NP; ++i) expand16(v_s(st) + chunk, i * RP + row0, unit, swap, vr[i]);
+      fence_proxy_async_smem();
+      mbar_arrive(v_full(st));
+      if (j + 1 < n_max) fetch(vr, vb, tp.v.stride_s, j + 1);
+    }
+  } else if (warp == kTcMmaWarp) {
+    // ------------------------------- MMA issuer -------------------------------
+    constexpr uint32_t idesc_qk = make_idesc_f16(0, 0, 0, kTcRows, kTcKeys);
+    constexpr uint32_t idesc_pv = make_idesc_f16(0, 0, 1, kTcRows, D);
+    bool ok = true;
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+      ok = mbar_wait(bar, parity, ctl, KST_TIMEOUT_MMA);
+      ok = __all_sync(0xffffffffu, ok);
+      return ok;
+    };
+    auto issue_qk = [&](int t, int j) {
+      tc_fence_after();
+      if (lane == 0) {
+        const int st = j % KS;
+        const uint64_t qd = make_smem_desc(q_s(t), 0, 1024), kd = make_smem_desc(k_s(st), 0, 1024);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint64_t off = static_cast<uint64_t>(((kk >> 2) * SM::kChunkBytes + (kk & 3) * 32) >> 4);
+          umma_ss(tmem + t * kTcKeys, qd + off, kd + off, idesc_qk, kk != 0 ? 1u : 0u);
+        }
+        umma_commit(s_full(t));
+      }
+      __syncwarp();
+    };
+    if (n_max > 0 && wait(k_full(0), 0)) {
+      for (int t = 0; t < 2 && ok; ++t)
+        if (n_blocks[t] > 0 && wait(q_full(t), 0)) issue_qk(t, 0);
+    }
+    for (int j = 0; j < n_max && ok; ++j) {
+      const int st = j % KS;
+      bool next = false;
+      for (int t = 0; t < 2 && ok; ++t) {
+        if (j >= n_blocks[t]) continue;
+        if (!wait(v_full(st), (j / KS) & 1)) break;
+        const uint64_t vd = make_smem_desc(v_s(st), SM::kChunkBytes, 1024);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          if (!wait(p_ready(t, half), j & 1)) break;
+          tc_fence_after();
+          if (lane == 0) {
+            // P'_t lies over S_t, per 32 columns [hi of 32 positions | lo of the same], 16 columns each; one MMA takes 16
+            // positions = 8 columns
+#pragma unroll
+            for (int k4 = 0; k4 < kTcKeys / 32; ++k4) {
+              const int kk = half * (kTcKeys / 32) + k4;
+              const uint32_t a = tmem + t * kTcKeys + (kk >> 1) * 32 + (kk & 1) * 8;
+              const uint32_t o = tmem + 2 * kTcKeys + t * 128;
+              const uint64_t bd = vd + static_cast<uint64_t>((kk * 2048) >> 4);
+              umma_ts(o, a, bd, idesc_pv, (j | kk) != 0 ? 1u : 0u);
+              if constexpr (SPLIT) umma_ts(o, a + 16, bd, idesc_pv, 1u);
+            }
+            if (half == 1) umma_commit(pv_done(t));
+          }
+          __syncwarp();
+        }
+        if (!ok) break;
+        if (j + 1 < n_blocks[t]) {
+          if (!next && !wait(k_full((j + 1) % KS), ((j + 1) / KS) & 1)) break;
+          next = true;
+          issue_qk(t, j + 1);
+        }
+      }
+      if (!ok) break;
+      if (lane == 0) umma_commit(kv_empty(st));
+      __syncwarp();
+    }
+  } else {
+    // ------------------------------- softmax / epilogue -------------------------------
+    const int t = (warp - 4) >> 2, quad = warp & 3;
+    const int lrow = quad * 32 + lane;
+    const int r = (2 * pair + t) * kTcRows + lrow;
+    const bool there = r < p.R;
+    const int nb = n_blocks[t];
+    const int limit = there ? last_seen(p, n, r) : -1;
+    const int limit_min = last_seen(p, n, min((2 * pair + t) * kTcRows, p.R - 1));
+    const bool warp_active = (2 * pair + t) * kTcRows + quad * 32 < p.R;       // else it only keeps the barriers going
+    const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+    const uint32_t s_tmem = tmem + t * kTcKeys + lanes, o_tmem = tmem + 2 * kTcKeys + t * 128 + lanes;
+    bool ok = true;
+    float c_row = 0.f;
+    // ---- q row -> fp16 times 2^(14 - exponent of its largest element), swizzled
+    if (nb > 0) {
+      const T* src = static_cast<const T*>(p.q.ptr) + b * p.q.stride_b + static_cast<long long>(min(r, p.R - 1) / p.G) * p.q.stride_s +
+                     static_cast<long long>(h * p.G + min(r, p.R - 1) % p.G) * p.q.stride_h;
+      uint32_t top = 0u;                       // largest magnitude by its bits: 0x7f80 (bf16) / 0x7c00 (fp16) and up is not finite
+      for (int i = 0; i < D; i += 8) {
+        const uint4 x = *reinterpret_cast<const uint4*>(src + i);
+        top = __vmaxu2(top, __vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu));
+        top = __vmaxu2(top, __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
+      }
+      top = max(top & 0xffffu, top >> 16);
+      float up = 1.f, down = 1.f;
+      if constexpr (Io<T>::kFmt == 1) {
+        const int e = min(max(static_cast<int>(top >> 7) - 127, -100), 127);
+        up = exp2_int(14 - e);
+        down = exp2_int(e - 14);
+      }
+      // a row with an infinite or NaN element: every score is infinite or NaN, and so is its softmax NaN
+      c_row = top >= (Io<T>::kFmt == 1 ? 0x7f80u : 0x7c00u) ? __uint_as_float(0x7fffffffu) : p.scale_log2 * down;
+#pragma unroll 4
+      for (int u = 0; u < D / 8; ++u) {
+        const uint4 x = *reinterpret_cast<const uint4*>(src + u * 8);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        uint32_t f[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 g = Io<T>::unpack2(w[e]);
+          f[e] = there ? Io<__half>::pack2(g.x * up, g.y * up) : 0u;
+        }
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};"
+                     ::"r"(q_s(t) + (u >> 3) * SM::kChunkBytes + swz128(lrow, u & 7)), "r"(f[0]), "r"(f[1]), "r"(f[2]), "r"(f[3])
+                     : "memory");
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(q_full(t));
+    }
+    float m_run = -INFINITY, l_run = 0.f;
+    uint32_t x[32];
+    for (int j = 0; j < nb; ++j) {
+      const int st = j % KS, kv0 = (j0 + j) * kTcKeys;
+      ok = mbar_wait(k_full(st), (j / KS) & 1, ctl, KST_TIMEOUT_CONSUMER);       // the block's scales
+      if (ok) ok = mbar_wait(s_full(t), j & 1, ctl, KST_TIMEOUT_CONSUMER);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      if (!warp_active) {
+        mbar_arrive(p_ready(t, 0));
+        mbar_arrive(p_ready(t, 1));
+        continue;
+      }
+      const float4* sc = scales + st * 8;
+      const bool masked = kv0 + kTcKeys - 1 > limit_min;
+      // ---- pass 1: the block's maximum of t'
+      float mb = -INFINITY;
+#pragma unroll 1
+      for (int c = 0; c < kTcKeys / 32; ++c) {
+        tmem_ld32(s_tmem + c * 32, x);
+        tmem_wait_ld();
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          float m0 = -INFINITY;
+          if (masked) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (kv0 + c * 32 + hf * 16 + i <= limit) m0 = fmaxf(m0, __uint_as_float(x[hf * 16 + i]));
+          } else {
+            float m1 = fmaxf(__uint_as_float(x[hf * 16 + 0]), __uint_as_float(x[hf * 16 + 1]));
+            m0 = fmaxf(__uint_as_float(x[hf * 16 + 2]), __uint_as_float(x[hf * 16 + 3]));
+#pragma unroll
+            for (int i = 4; i < 16; i += 4) {
+              m0 = fmax3(m0, __uint_as_float(x[hf * 16 + i]), __uint_as_float(x[hf * 16 + i + 1]));
+              m1 = fmax3(m1, __uint_as_float(x[hf * 16 + i + 2]), __uint_as_float(x[hf * 16 + i + 3]));
+            }
+            m0 = fmaxf(m0, m1);
+          }
+          const float4 f = sc[c * 2 + hf];
+          if (m0 != -INFINITY) mb = fmaxf(mb, fmaf(m0, c_row * f.x, f.y));
+        }
+      }
+      const float m_new = mb - kTcPBias;
+      const bool grow = m_new - m_run > kTcRescale;                // first block: m_run = -inf
+      float alpha = 1.0f;
+      if (grow) {
+        alpha = ex2_approx(m_run - m_new);                         // 0 on the first block
+        m_run = m_new;
+        l_run *= alpha;
+      }
+      // S_t(j) was produced after P'_t(j-1) v (MMAs run in issue order), so O_t is quiescent here
+      if (j > 0 && __any_sync(0xffffffffu, grow)) {
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          tmem_ld32(o_tmem + c * 32, x);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * alpha);
+          tmem_st32(o_tmem + c * 32, x);
+        }
+      }
+      // ---- pass 2: P' = 2^(t' - m'), written over S (hi | lo per 32 columns); compiled twice, without and with masks
+      auto pass2 = [&](auto masked_tag) {
+        constexpr bool kMasked = decltype(masked_tag)::value;
+        auto chunk_p = [&](const uint32_t (&src)[32], int c, uint32_t (&pk)[SPLIT ? 32 : 16]) {
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            const float4 f = sc[c * 2 + hf];
+            const float a = c_row * f.x, d = f.y - m_run;
+            const float2 a2 = make_float2(a, a), d2 = make_float2(d, d);
+            float2 pp[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              pp[i] = __ffma2_rn(make_float2(__uint_as_float(src[hf * 16 + 2 * i]), __uint_as_float(src[hf * 16 + 2 * i + 1])), a2, d2);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) pp[i] = make_float2(ex2_approx(pp[i].x), ex2_approx(pp[i].y));
+            if constexpr (kMasked) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int key = kv0 + c * 32 + hf * 16 + 2 * i;
+                if (key > limit) pp[i].x = 0.f;
+                if (key + 1 > limit) pp[i].y = 0.f;
+              }
+            }
+            float2 sum = pp[0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) sum = __fadd2_rn(sum, pp[i]);
+            l_run = fmaf(sum.x + sum.y, f.z, l_run);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) pk[hf * 8 + i] = Io<__half>::pack2(pp[i].x, pp[i].y);
+            if constexpr (SPLIT) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float2 lo = __ffma2_rn(Io<__half>::unpack2(pk[hf * 8 + i]), make_float2(-1.f, -1.f), pp[i]);
+                pk[16 + hf * 8 + i] = Io<__half>::pack2(lo.x, lo.y);
+              }
+            }
+          }
+        };
+        auto store_p = [&](int c, uint32_t (&pk)[SPLIT ? 32 : 16]) {
+          if constexpr (SPLIT) tmem_st32(s_tmem + c * 32, *reinterpret_cast<uint32_t(*)[32]>(pk));
+          else tmem_st16(s_tmem + c * 32, *reinterpret_cast<uint32_t(*)[16]>(pk));
+        };
+        // two register buffers: the next columns are on their way while these are worked on
+        uint32_t y[32];
+        tmem_ld32(s_tmem, x);
+        tmem_wait_ld();
+#pragma unroll 1
+        for (int c = 0; c < kTcKeys / 32; c += 2) {
+          uint32_t pk[SPLIT ? 32 : 16];
+          tmem_ld32(s_tmem + (c + 1) * 32, y);
+          chunk_p(x, c, pk);
+          store_p(c, pk);
+          tmem_wait_ld();
+          if (c + 2 < kTcKeys / 32) tmem_ld32(s_tmem + (c + 2) * 32, x);
+          chunk_p(y, c + 1, pk);
+          store_p(c + 1, pk);
+          if (c == 0) {                                            // the first half of P' is written
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(p_ready(t, 0));
+          }
+          tmem_wait_ld();
+        }
+      };
+      if (masked) pass2(std::true_type{});
+      else pass2(std::false_type{});
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(p_ready(t, 1));
+    }
+    // ---- epilogue.  A row without a block (or without a visible position) has l = 0: o = 0, lse = -inf
+    if (ok && nb > 0 && warp_active) {
+      ok = mbar_wait(pv_done(t), (nb - 1) & 1, ctl, KST_TIMEOUT_CONSUMER);
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+    }
+    if (ok && !dead && warp_active) {
+      const int tile = 2 * pair + t;
+      const long long slot = static_cast<long long>(bh * p.tiles + tile) * tp.n_splits + split;
+      const bool parts = tp.n_splits > 1, any_nan = *reinterpret_cast<volatile int*>(nan_any) != 0;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        if (nb > 0) {
+          tmem_ld32(o_tmem + c * 32, x);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) x[i] = 0u;
+        }
+        if (any_nan) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (nan_from[c * 32 + i] <= limit) x[i] = 0x7fffffffu;
+        }
+        if (!there) continue;
+        if (parts) {
+          float* dst = p.part_o + (slot * kTcRows + lrow) * D + c * 32;
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<float4*>(dst + i) = make_float4(__uint_as_float(x[i]), __uint_as_float(x[i + 1]),
+                                                              __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
+        } else {
+          const int hq = h * p.G + r % p.G;
+          const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;
+          T* dst = static_cast<T*>(p.o.ptr) + b * p.o.stride_b + static_cast<long long>(r / p.G) * p.o.stride_s +
+                   static_cast<long long>(hq) * p.o.stride_h + c * 32;
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            uint4 v;
+            v.x = Io<T>::pack2(__uint_as_float(x[i]) * inv, __uint_as_float(x[i + 1]) * inv);
+            v.y = Io<T>::pack2(__uint_as_float(x[i + 2]) * inv, __uint_as_float(x[i + 3]) * inv);
+            v.z = Io<T>::pack2(__uint_as_float(x[i + 4]) * inv, __uint_as_float(x[i + 5]) * inv);
+            v.w = Io<T>::pack2(__uint_as_float(x[i + 6]) * inv, __uint_as_float(x[i + 7]) * inv);
+            *reinterpret_cast<uint4*>(dst + i) = v;
+          }
+        }
+      }
+      if (there) {
+        if (parts) p.part_ml[slot * kTcRows + lrow] = make_float2(m_run + kQ8PBias, l_run);    // in the merge's convention
+        else if (p.lse != nullptr)
+          p.lse[(static_cast<long long>(b) * p.Hq + h * p.G + r % p.G) * p.M + r / p.G] = m_run + log2f(l_run);
+      }
+      if (parts && split == 0 && lrow == 0) {
+        const int u = bh * p.tiles + tile;                         // its pieces' slots begin at u * n_splits
+        p.pieces[u] = make_int2(u * (tp.n_splits - 1), u * (tp.n_splits - 1) + tp.n_splits - 1);
+      }
+      tc_fence_before();
+    }
+  }
+
+  // ------------------------------- teardown -------------------------------
+  __syncthreads();
+  if (*abort_flag) {                           // a wait ran out: time for the products under way to end
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+    __syncthreads();
+  }
+  if (warp == kTcMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTcTmemCols);
+  }
+}
+
+struct TcPlan {
+  int tiles, pairs, n_splits;
+  size_t ml_off, o_off, piece_off, total;
+};
+
+// key blocks divided among CTAs while that fills SMs, at least two blocks each
+TcPlan tc_plan(const TrnAttnQ8Args& a) {
+  TcPlan w{};
+  const int R = a.M * (a.Hq / a.Hkv);
+  w.tiles = (R + kTcRows - 1) / kTcRows;
+  w.pairs = (w.tiles + 1) / 2;
+  const long long ctas = static_cast<long long>(a.B) * a.Hkv * w.pairs;
+  const int longest = a.kv_len != nullptr ? a.cache.S : min(max(a.kv_len_all, 1), a.cache.S);
+  const long long blocks = (longest - 1) / kTcKeys + 1;
+  w.n_splits = static_cast<int>(max(min(min(kAttnNominalSMs / ctas, blocks / 2), static_cast<long long>(kTcMaxSplits)), 1LL));
+  if (w.n_splits == 1) return w;
+  const size_t rows = static_cast<size_t>(a.B) * a.Hkv * w.tiles * w.n_splits * kTcRows;
+  w.ml_off = 0;
+  w.o_off = up256(rows * sizeof(float2));
+  w.piece_off = w.o_off + up256(rows * a.D * sizeof(float));
+  w.total = w.piece_off + up256(static_cast<size_t>(a.B) * a.Hkv * w.tiles * sizeof(int2));
+  return w;
+}
+
+template <typename T, int D>
+int launch_typed(const TrnAttnQ8Args& a, cudaStream_t st, const DeviceState& ds) {
+  using SM = TcSmem<D>;
+  TcPlan w = tc_plan(a);
+  if (a.workspace == nullptr) w.n_splits = 1;
+  TcParams tp{};
+  tp.c = q8_params(a, ds);
+  tp.k = a.cache.k;
+  tp.v = a.cache.v;
+  tp.pairs = w.pairs;
+  tp.n_splits = w.n_splits;
+  tp.c.tiles = w.tiles;
+  tp.c.tile_rows = kTcRows;
+  if (w.n_splits > 1) {
+    uint8_t* ws = static_cast<uint8_t*>(a.workspace);
+    tp.c.part_ml = reinterpret_cast<float2*>(ws + w.ml_off);
+    tp.c.part_o = reinterpret_cast<float*>(ws + w.o_off);
+    tp.c.pieces = reinterpret_cast<int2*>(ws + w.piece_off);
+  }
+  const long long grid = static_cast<long long>(a.B) * a.Hkv * w.pairs * w.n_splits;
+  if (grid > 0x7fffffffLL || static_cast<long long>(a.B) * a.Hkv * w.tiles * w.n_splits > 0x7fffffffLL) return TRN_E_SHAPE;
+  auto kern = attn_q8_tc_kernel<T, D>;
+  const int rc = ensure_dyn_smem(reinterpret_cast<const void*>(kern), SM::kTotal, ds.device);
+  if (rc != TRN_OK) return rc;
+  TRN_CUDA_TRY(launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(kTcThreads), SM::kTotal, st, tp));
+  return w.n_splits > 1 ? launch_q8_join(tp.c, a, true, st) : TRN_OK;
+}
+
+}  // namespace
+
+// More than 32 rows per kv head, and no weights (those are summed from scores that attn_q8.cu keeps)
+bool attn_q8_tc_applies(const TrnAttnQ8Args& a) {
+  return a.weight == nullptr && static_cast<long long>(a.M) * (a.Hq / a.Hkv) > 32;
+}
+
+size_t attn_q8_tc_workspace(const TrnAttnQ8Args& a) { return tc_plan(a).total; }
+
+int launch_attn_q8_tc(const TrnAttnQ8Args& a, cudaStream_t st, const DeviceState& ds) {
+  if (a.dtype == TRN_BF16)
+    return a.D == 128 ? launch_typed<__nv_bfloat16, 128>(a, st, ds) : launch_typed<__nv_bfloat16, 64>(a, st, ds);
+  return a.D == 128 ? launch_typed<__half, 128>(a, st, ds) : launch_typed<__half, 64>(a, st, ds);
+}
+
+}  // namespace trn

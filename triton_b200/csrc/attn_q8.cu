@@ -68,22 +68,10 @@ struct Q8Smem {
   static constexpr int kTotalKept = kTotal + kQ8Warps * kRows * kKeptPitch * 4;
 };
 
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-  return v;
-}
 __device__ __forceinline__ uint2 lds64(uint32_t a) {
   uint2 v;
   asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
   return v;
-}
-// byte offset of 16-byte unit u of row r in a tile as TMA wrote it: 128-byte rows with the 128-byte swizzle, 64-byte rows
-// with the 64-byte swizzle
-template <int D>
-__device__ __forceinline__ uint32_t q8_off(uint32_t r, uint32_t u) {
-  if constexpr (D == 128) return r * 128u + ((u ^ (r & 7u)) << 4);
-  else return r * 64u + ((u ^ ((r >> 1) & 3u)) << 4);
 }
 // which row of an 8-row block column c of a score block is.  64-byte rows: a quad's even columns 0, 2, 4, 6 and the lane
 // groups' neighbours have to meet different halves of a 128-byte line, hence 0 3 1 2 4 7 5 6

@@ -47,6 +47,18 @@ namespace {
 __device__ __forceinline__ int last_seen(const Q8Params& p, int n, int r) {      // by row r of a (b, kv head); -1: nothing
   return p.causal ? max(n - p.M + r / p.G, -1) : n - 1;
 }
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+// byte offset of 16-byte unit u of row r in a tile as TMA wrote it: 128-byte rows with the 128-byte swizzle, 64-byte rows
+// with the 64-byte swizzle
+template <int D>
+__device__ __forceinline__ uint32_t q8_off(uint32_t r, uint32_t u) {
+  if constexpr (D == 128) return r * 128u + ((u ^ (r & 7u)) << 4);
+  else return r * 64u + ((u ^ ((r >> 1) & 3u)) << 4);
+}
 // log2 and reciprocal of a scale: exact for powers of two
 __device__ __forceinline__ void scale_log_inv(float s, float& lg, float& inv) {
   const uint32_t u = __float_as_uint(s);

@@ -4,12 +4,14 @@
 // The M * Hq / Hkv rows of a (b, kv head) are taken in tiles of 128 (row r = query r / G, head r % G, so a tile of a causal
 // call spans few queries); a CTA works on two neighbouring tiles against the same keys, so that one tile's softmax runs
 // while the other's products do.
-//   warps 0-3    convert: fetch the next 128 positions' codes into registers, and when a stage is free write them as fp16
-//                into the 128-byte-swizzled tiles the tensor core reads (exact), with the scales of their 16-position groups
+//   warps 0-2    convert: TMA brings the next 128 positions' codes to a raw tile; when a stage is free they are written as
+//                fp16 (exact) into the 128-byte-swizzled tiles the tensor core reads, with the scales of their 16-position
+//                groups.  (Codes fetched to registers instead made the proxy fence that publishes a tile wait for the
+//                fetches under way: 633 us against see below for a prompt chunk.)
 //   warps 4-7,   softmax of tile 0 / 1, one thread per row: q -> shared memory as fp16 times a power of two; then per block of
 //   warps 8-11   128 positions  t' = s * (c ks) + log2 vs,  P' = 2^(t' - m'), packed to fp16 over s in tensor memory,
 //                l += P' / vs;  o is rescaled only when a row's maximum grew by more than 2^8 since the last time
-//   warp 12      issues S_t = q_t k^T and O_t += P'_t v (P' from tensor memory)
+//   warp 3       issues S_t = q_t k^T and O_t += P'_t v (P' from tensor memory)
 // The scales cost nothing per score: ks and log2 vs change every 16 columns at most and enter the multiply-add that the
 // softmax makes anyway.  bf16 outputs take P' as one fp16 part, fp16 outputs as hi + lo (see attn_q8.cu).
 // Few CTAs (less than one for each SM): the key blocks are divided among several, merged by the kernel in attn_q8.cu.
@@ -23,8 +25,10 @@ namespace trn {
 namespace {
 
 constexpr int kTcRows = 128, kTcKeys = 128;
-constexpr int kTcThreads = 13 * 32;
-constexpr int kTcMmaWarp = 12;
+constexpr int kTcThreads = 12 * 32;
+constexpr int kTcConvert = 96;                // threads that convert: warps 0-2
+constexpr int kTcMmaWarp = 3;
+static_assert(kTcConvert == 32 * kTcMmaWarp && kTcThreads == 32 * (kTcMmaWarp + 1 + 8), "warps: convert, MMA, softmax from warp 4");
 constexpr int kTcTmemCols = 512;              // S0 [0,128) S1 [128,256) O0 [256,256+D) O1 [384,384+D)
 constexpr float kTcRescale = 8.0f;            // log2 units a row's maximum may pass the offset in use
 constexpr float kTcPBias = 6.0f;              // P' <= 2^14 with it
@@ -32,7 +36,6 @@ constexpr int kTcMaxSplits = 16;
 
 struct TcParams {
   Q8Params c;
-  TrnHeadTensor k, v;
   int pairs, n_splits;
 };
 
@@ -44,7 +47,9 @@ struct TcSmem {
   static constexpr int kTile = kChunks * kChunkBytes;
   static constexpr int kQ = 0;                             // two q tiles
   static constexpr int kKV = 2 * kTile;
-  static constexpr int kScales = kKV + kStages * 2 * kTile;          // [stage][8 groups] (ks, log2 vs, 1 / vs, -)
+  static constexpr int kRaw = kKV + kStages * 2 * kTile;             // codes of k, codes of v
+  static constexpr int kRawTile = 128 * D;
+  static constexpr int kScales = kRaw + 2 * kRawTile;         // [stage][8 groups] (ks, log2 vs, 1 / vs, -)
   static constexpr int kNan = kScales + kStages * 8 * 16;            // [D] first position with a NaN code in v
   static constexpr int kBars = kNan + D * 4;
   static constexpr int kTotal = kBars + 256 + 1024;
@@ -69,9 +74,22 @@ __device__ __forceinline__ void expand16(uint32_t tile, uint32_t row, uint32_t u
   }
 }
 
-template <typename T, int D>
+// 32 lanes x 16 consecutive 32-bit columns of tensor memory
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+// GRP: positions that share a scale within the kernel, 16 or (blocks of 32 and more) 32
+template <typename T, int D, int GRP>
 __global__ void __launch_bounds__(kTcThreads, 1)
-attn_q8_tc_kernel(const __grid_constant__ TcParams tp) {
+attn_q8_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                  const __grid_constant__ TcParams tp) {
   using SM = TcSmem<D>;
   constexpr int KS = SM::kStages;
   constexpr bool SPLIT = Io<T>::kFmt == 0;
@@ -88,7 +106,9 @@ attn_q8_tc_kernel(const __grid_constant__ TcParams tp) {
   auto q_full = [&](int t) { return bars + 8u * (3 * KS + 4 + t); };
   // P' becomes ready in two halves (positions 0..63, 64..127), so that P' v starts on the first
   auto p_ready = [&](int t, int half) { return bars + 8u * (3 * KS + 6 + 2 * t + half); };
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + SM::kBars + 8 * (3 * KS + 10));
+  auto raw_full = [&](int kv) { return bars + 8u * (3 * KS + 10 + kv); };
+  auto raw_empty = [&](int kv) { return bars + 8u * (3 * KS + 12 + kv); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + SM::kBars + 8 * (3 * KS + 14));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* nan_any = reinterpret_cast<int*>(tmem_slot + 2);
   int* nan_from = reinterpret_cast<int*>(gen + SM::kNan);
@@ -98,14 +118,16 @@ attn_q8_tc_kernel(const __grid_constant__ TcParams tp) {
   const Ctl ctl{p.status, abort_flag};
   if (threadIdx.x == 0) {
     for (int s = 0; s < KS; ++s) {
-      mbar_init(k_full(s), 128);
-      mbar_init(v_full(s), 128);
+      mbar_init(k_full(s), kTcConvert);
+      mbar_init(v_full(s), kTcConvert);
       mbar_init(kv_empty(s), 1);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(s_full(t), 1);
       mbar_init(pv_done(t), 1);
       mbar_init(q_full(t), 128);
+      mbar_init(raw_full(t), 1);
+      mbar_init(raw_empty(t), kTcConvert);
       mbar_init(p_ready(t, 0), 128);
       mbar_init(p_ready(t, 1), 128);
     }
@@ -154,24 +176,15 @@ attn_q8_tc_kernel(const __grid_constant__ TcParams tp) {
   auto k_s = [&](int s) { return base + SM::kKV + s * 2 * SM::kTile; };
   auto v_s = [&](int s) { return k_s(s) + SM::kTile; };
 
-  if (warp < 4) {
+  if (warp < kTcConvert / 32) {
     // ------------------------------- convert -------------------------------
-    constexpr int SEG = D / 16, RP = 128 / SEG, NP = 128 / RP;     // lanes per row, rows per pass, passes
-    const int row0 = static_cast<int>(threadIdx.x) / SEG, seg = static_cast<int>(threadIdx.x) % SEG;
-    const uint32_t chunk = static_cast<uint32_t>(seg >> 2) * SM::kChunkBytes, unit = static_cast<uint32_t>(seg & 3) * 2u;
-    const bool swap = seg >= 4;
-    const uint8_t* kb = static_cast<const uint8_t*>(tp.k.ptr) + b * tp.k.stride_b + h * tp.k.stride_h + seg * 16;
-    const uint8_t* vb = static_cast<const uint8_t*>(tp.v.ptr) + b * tp.v.stride_b + h * tp.v.stride_h + seg * 16;
-    uint4 kr[NP], vr[NP];
+    constexpr int SEG = D / 16, UNITS = kTcKeys * SEG;             // 16-byte units of a row, of a raw tile
+    constexpr int PER = 4;                                         // units a thread has in hand
     float ks = 1.f, vs = 1.f;
-    auto fetch = [&](uint4 (&r)[NP], const uint8_t* src, long long stride, int j) {
-      const int kv0 = (j0 + j) * kTcKeys;
-#pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        const int key = kv0 + i * RP + row0;
-        r[i] = make_uint4(0u, 0u, 0u, 0u);                         // behind the sequence: zeros, whatever lies there
-        if (key < n) r[i] = *reinterpret_cast<const uint4*>(src + key * stride);
-      }
+    auto bring = [&](int kv, int j) {                              // thread 0
+      mbar_expect_tx(raw_full(kv), SM::kRawTile);
+      tma_load_head_tile(base + SM::kRaw + kv * SM::kRawTile, kv == 0 ? &tm_k : &tm_v, raw_full(kv), kv == 0 ? p.ki : p.vi, 0,
+                         (j0 + j) * kTcKeys, h, b);
     };
     auto fetch_scales = [&](int j) {
       const int key = (j0 + j) * kTcKeys + 16 * static_cast<int>(threadIdx.x);
@@ -180,14 +193,57 @@ attn_q8_tc_kernel(const __grid_constant__ TcParams tp) {
         vs = key < n ? *p.vs.at(b, key >> p.shift, h) : 1.f;
       }
     };
+    // raw tile kv of block j -> fp16 tile at dst; edge: some row does not see some position of the block
+    auto convert = [&](int kv, uint32_t dst, int kv0, bool edge) {
+      const uint32_t raw = base + SM::kRaw + kv * SM::kRawTile;
+#pragma unroll 1
+      for (int u0 = static_cast<int>(threadIdx.x); u0 < UNITS; u0 += PER * kTcConvert) {
+        uint4 c[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const uint32_t u = min(u0 + i * kTcConvert, UNITS - 1);
+          c[i] = lds128(raw + q8_off<D>(u / SEG, u % SEG));
+        }
+        if (edge && kv == 1) {
+          // v behind the sequence counts as 0 whatever lies there, and so do NaN codes, whose first positions are kept
+#pragma unroll
+          for (int i = 0; i < PER; ++i) {
+            const int u = min(u0 + i * kTcConvert, UNITS - 1), key = kv0 + u / SEG;
+            uint32_t w[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if (key >= n) w[e] = 0u;
+              const uint32_t bad = nan_bytes(w[e]);
+              if (bad != 0u) {
+                w[e] &= ~bad;
+                *nan_any = 1;
+                for (int x = 0; x < 4; ++x)
+                  if ((bad >> (8 * x)) & 1u) atomicMin(&nan_from[u % SEG * 16 + 4 * e + x], key);
+              }
+            }
+            c[i] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const uint32_t u = u0 + i * kTcConvert, seg = u % SEG;
+          if (u < UNITS) expand16(dst + (seg >> 2) * SM::kChunkBytes, u / SEG, (seg & 3) * 2, seg >= 4, c[i]);
+        }
+      }
+      fence_proxy_async_smem();
+    };
     if (n_max > 0) {
+      if (threadIdx.x == 0) {
+        bring(0, 0);
+        bring(1, 0);
+      }
       fetch_scales(0);
-      fetch(kr, kb, tp.k.stride_s, 0);
-      fetch(vr, vb, tp.v.stride_s, 0);
     }
     for (int j = 0; j < n_max; ++j) {
       const int st = j % KS, kv0 = (j0 + j) * kTcKeys;
-      bool ok = mbar_wait(kv_empty(st), ((j / KS) & 1) ^ 1u, ctl, KST_TIMEOUT_PRODUCER);
+      const bool edge = kv0 + kTcKeys - 1 > first_lim;
+      bool ok = mbar_wait(raw_full(0), j & 1, ctl, KST_TIMEOUT_PRODUCER);
+      if (ok) ok = mbar_wait(kv_empty(st), ((j / KS) & 1) ^ 1u, ctl, KST_TIMEOUT_PRODUCER);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       if (threadIdx.x < 8) {
@@ -195,37 +251,22 @@ attn_q8_tc_kernel(const __grid_constant__ TcParams tp) {
         scale_log_inv(vs < kMinVScale ? kMinVScale : vs, lg, inv);
         scales[st * 8 + threadIdx.x] = make_float4(ks, lg, inv, 0.f);
       }
-#pragma unroll
-      for (int i = 0; i < NP; ++i) expand16(k_s(st) + chunk, i * RP + row0, unit, swap, kr[i]);
-      fence_proxy_async_smem();
+      convert(0, k_s(st), kv0, edge);
       mbar_arrive(k_full(st));
-      if (j + 1 < n_max) {
-        fetch_scales(j + 1);
-        fetch(kr, kb, tp.k.stride_s, j + 1);
-      }
-      if (kv0 + kTcKeys - 1 > first_lim) {
-        // some row does not see some position: NaN codes of v count as 0 in the product, their first positions are kept
-#pragma unroll
-        for (int i = 0; i < NP; ++i) {
-          uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t bad = nan_bytes(w[e]);
-            if (bad != 0u) {
-              w[e] &= ~bad;
-              *nan_any = 1;
-              for (int c = 0; c < 4; ++c)
-                if ((bad >> (8 * c)) & 1u) atomicMin(&nan_from[seg * 16 + 4 * e + c], kv0 + i * RP + row0);
-            }
-          }
-          vr[i] = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < NP; ++i) expand16(v_s(st) + chunk, i * RP + row0, unit, swap, vr[i]);
-      fence_proxy_async_smem();
+      if (j + 1 < n_max) fetch_scales(j + 1);
+      // every converting thread is done with the raw tile: the next block's codes may take its place.  (After a wait that ran
+      // out a warp leaves the loop; named barriers count threads, so the others must not wait for it: they meet in
+      // mbarriers only.)
+      mbar_arrive(raw_empty(0));
+      if (threadIdx.x == 0 && j + 1 < n_max && mbar_wait(raw_empty(0), j & 1, ctl, KST_TIMEOUT_PRODUCER)) bring(0, j + 1);
+      ok = mbar_wait(raw_full(1), j & 1, ctl, KST_TIMEOUT_PRODUCER);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      convert(1, v_s(st), kv0, edge);
       mbar_arrive(v_full(st));
-      if (j + 1 < n_max) fetch(vr, vb, tp.v.stride_s, j + 1);
+      mbar_arrive(raw_empty(1));
+      if (threadIdx.x == 0 && j + 1 < n_max && mbar_wait(raw_empty(1), j & 1, ctl, KST_TIMEOUT_PRODUCER)) bring(1, j + 1);
+      __syncwarp();
     }
   } else if (warp == kTcMmaWarp) {
     // ------------------------------- MMA issuer -------------------------------
@@ -307,37 +348,42 @@ attn_q8_tc_kernel(const __grid_constant__ TcParams tp) {
     const uint32_t s_tmem = tmem + t * kTcKeys + lanes, o_tmem = tmem + 2 * kTcKeys + t * 128 + lanes;
     bool ok = true;
     float c_row = 0.f;
-    // ---- q row -> fp16 times 2^(14 - exponent of its largest element), swizzled
+    // ---- q rows -> fp16 times 2^(14 - exponent of a row's largest element), swizzled.  D / 8 lanes take a row, so that a
+    // warp reads whole lines (a row per thread: 8 us more for each CTA); lane L ends up with row L's factor.
     if (nb > 0) {
-      const T* src = static_cast<const T*>(p.q.ptr) + b * p.q.stride_b + static_cast<long long>(min(r, p.R - 1) / p.G) * p.q.stride_s +
-                     static_cast<long long>(h * p.G + min(r, p.R - 1) % p.G) * p.q.stride_h;
-      uint32_t top = 0u;                       // largest magnitude by its bits: 0x7f80 (bf16) / 0x7c00 (fp16) and up is not finite
-      for (int i = 0; i < D; i += 8) {
-        const uint4 x = *reinterpret_cast<const uint4*>(src + i);
-        top = __vmaxu2(top, __vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu));
-        top = __vmaxu2(top, __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
-      }
-      top = max(top & 0xffffu, top >> 16);
-      float up = 1.f, down = 1.f;
-      if constexpr (Io<T>::kFmt == 1) {
-        const int e = min(max(static_cast<int>(top >> 7) - 127, -100), 127);
-        up = exp2_int(14 - e);
-        down = exp2_int(e - 14);
-      }
-      // a row with an infinite or NaN element: every score is infinite or NaN, and so is its softmax NaN
-      c_row = top >= (Io<T>::kFmt == 1 ? 0x7f80u : 0x7c00u) ? __uint_as_float(0x7fffffffu) : p.scale_log2 * down;
+      constexpr int LPR = D / 8, RPI = 32 / LPR;                   // lanes per row, rows per iteration
+      const int sub = lane / LPR, u = lane % LPR;
 #pragma unroll 4
-      for (int u = 0; u < D / 8; ++u) {
-        const uint4 x = *reinterpret_cast<const uint4*>(src + u * 8);
+      for (int it = 0; it < 32 / RPI; ++it) {
+        const int lr = quad * 32 + it * RPI + sub, rr = (2 * pair + t) * kTcRows + lr;
+        uint4 x = make_uint4(0u, 0u, 0u, 0u);
+        if (rr < p.R)
+          x = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q.ptr) + b * p.q.stride_b + static_cast<long long>(rr / p.G) * p.q.stride_s +
+                                              static_cast<long long>(h * p.G + rr % p.G) * p.q.stride_h + u * 8);
+        // largest magnitude by its bits: 0x7f80 (bf16) / 0x7c00 (fp16) and up is not finite
+        uint32_t top = __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
+        top = max(top & 0xffffu, top >> 16);
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        float up = 1.f, down = 1.f;
+        if constexpr (Io<T>::kFmt == 1) {
+          const int e = min(max(static_cast<int>(top >> 7) - 127, -100), 127);
+          up = exp2_int(14 - e);
+          down = exp2_int(e - 14);
+        }
+        // a row with an infinite or NaN element: every score is infinite or NaN, and so is its softmax NaN
+        const float c = top >= (Io<T>::kFmt == 1 ? 0x7f80u : 0x7c00u) ? __uint_as_float(0x7fffffffu) : p.scale_log2 * down;
+        const float mine = __shfl_sync(0xffffffffu, c, (lane % RPI) * LPR);
+        if (lane / RPI == it) c_row = mine;
         const uint32_t w[4] = {x.x, x.y, x.z, x.w};
         uint32_t f[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float2 g = Io<T>::unpack2(w[e]);
-          f[e] = there ? Io<__half>::pack2(g.x * up, g.y * up) : 0u;
+          f[e] = Io<__half>::pack2(g.x * up, g.y * up);
         }
         asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};"
-                     ::"r"(q_s(t) + (u >> 3) * SM::kChunkBytes + swz128(lrow, u & 7)), "r"(f[0]), "r"(f[1]), "r"(f[2]), "r"(f[3])
+                     ::"r"(q_s(t) + (u >> 3) * SM::kChunkBytes + swz128(lr, u & 7)), "r"(f[0]), "r"(f[1]), "r"(f[2]), "r"(f[3])
                      : "memory");
       }
       fence_proxy_async_smem();
@@ -361,29 +407,29 @@ attn_q8_tc_kernel(const __grid_constant__ TcParams tp) {
       const bool masked = kv0 + kTcKeys - 1 > limit_min;
       // ---- pass 1: the block's maximum of t'
       float mb = -INFINITY;
-#pragma unroll 1
+#pragma unroll
       for (int c = 0; c < kTcKeys / 32; ++c) {
         tmem_ld32(s_tmem + c * 32, x);
         tmem_wait_ld();
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
+        for (int g0 = 0; g0 < 32; g0 += GRP) {
           float m0 = -INFINITY;
           if (masked) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (kv0 + c * 32 + hf * 16 + i <= limit) m0 = fmaxf(m0, __uint_as_float(x[hf * 16 + i]));
+            for (int i = 0; i < GRP; ++i)
+              if (kv0 + c * 32 + g0 + i <= limit) m0 = fmaxf(m0, __uint_as_float(x[g0 + i]));
           } else {
-            float m1 = fmaxf(__uint_as_float(x[hf * 16 + 0]), __uint_as_float(x[hf * 16 + 1]));
-            m0 = fmaxf(__uint_as_float(x[hf * 16 + 2]), __uint_as_float(x[hf * 16 + 3]));
+            float m1 = fmaxf(__uint_as_float(x[g0]), __uint_as_float(x[g0 + 1]));
+            m0 = fmaxf(__uint_as_float(x[g0 + 2]), __uint_as_float(x[g0 + 3]));
 #pragma unroll
-            for (int i = 4; i < 16; i += 4) {
-              m0 = fmax3(m0, __uint_as_float(x[hf * 16 + i]), __uint_as_float(x[hf * 16 + i + 1]));
-              m1 = fmax3(m1, __uint_as_float(x[hf * 16 + i + 2]), __uint_as_float(x[hf * 16 + i + 3]));
+            for (int i = 4; i < GRP; i += 4) {
+              m0 = fmax3(m0, __uint_as_float(x[g0 + i]), __uint_as_float(x[g0 + i + 1]));
+              m1 = fmax3(m1, __uint_as_float(x[g0 + i + 2]), __uint_as_float(x[g0 + i + 3]));
             }
             m0 = fmaxf(m0, m1);
           }
-          const float4 f = sc[c * 2 + hf];
-          if (m0 != -INFINITY) mb = fmaxf(mb, fmaf(m0, c_row * f.x, f.y));
+          const float4 f = sc[c * 2 + g0 / 16];
+          if (!masked || m0 != -INFINITY) mb = fmaxf(mb, fmaf(m0, c_row * f.x, f.y));
         }
       }
       const float m_new = mb - kTcPBias;
@@ -397,48 +443,51 @@ attn_q8_tc_kernel(const __grid_constant__ TcParams tp) {
       // S_t(j) was produced after P'_t(j-1) v (MMAs run in issue order), so O_t is quiescent here
       if (j > 0 && __any_sync(0xffffffffu, grow)) {
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          tmem_ld32(o_tmem + c * 32, x);
+        for (int c = 0; c < D / 16; ++c) {
+          uint32_t y[16];
+          tmem_ld16(o_tmem + c * 16, y);
           tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * alpha);
-          tmem_st32(o_tmem + c * 32, x);
+          for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * alpha);
+          tmem_st16(o_tmem + c * 16, y);
         }
       }
       // ---- pass 2: P' = 2^(t' - m'), written over S (hi | lo per 32 columns); compiled twice, without and with masks
       auto pass2 = [&](auto masked_tag) {
         constexpr bool kMasked = decltype(masked_tag)::value;
         auto chunk_p = [&](const uint32_t (&src)[32], int c, uint32_t (&pk)[SPLIT ? 32 : 16]) {
+          float2 sum;
+          float4 f;
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            const float4 f = sc[c * 2 + hf];
+          for (int i0 = 0; i0 < 16; i0 += 8) {                     // pairs of columns, eight at a time
+            if (GRP == 16 || i0 == 0) f = sc[c * 2 + i0 / 8];
             const float a = c_row * f.x, d = f.y - m_run;
             const float2 a2 = make_float2(a, a), d2 = make_float2(d, d);
             float2 pp[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-              pp[i] = __ffma2_rn(make_float2(__uint_as_float(src[hf * 16 + 2 * i]), __uint_as_float(src[hf * 16 + 2 * i + 1])), a2, d2);
+              pp[i] = __ffma2_rn(make_float2(__uint_as_float(src[2 * (i0 + i)]), __uint_as_float(src[2 * (i0 + i) + 1])), a2, d2);
 #pragma unroll
             for (int i = 0; i < 8; ++i) pp[i] = make_float2(ex2_approx(pp[i].x), ex2_approx(pp[i].y));
             if constexpr (kMasked) {
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
-                const int key = kv0 + c * 32 + hf * 16 + 2 * i;
+                const int key = kv0 + c * 32 + 2 * (i0 + i);
                 if (key > limit) pp[i].x = 0.f;
                 if (key + 1 > limit) pp[i].y = 0.f;
               }
             }
-            float2 sum = pp[0];
+            sum = GRP == 16 || i0 == 0 ? pp[0] : __fadd2_rn(sum, pp[0]);
 #pragma unroll
             for (int i = 1; i < 8; ++i) sum = __fadd2_rn(sum, pp[i]);
-            l_run = fmaf(sum.x + sum.y, f.z, l_run);
+            if (GRP == 16 || i0 == 8) l_run = fmaf(sum.x + sum.y, f.z, l_run);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) pk[hf * 8 + i] = Io<__half>::pack2(pp[i].x, pp[i].y);
+            for (int i = 0; i < 8; ++i) pk[i0 + i] = Io<__half>::pack2(pp[i].x, pp[i].y);
             if constexpr (SPLIT) {
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
-                const float2 lo = __ffma2_rn(Io<__half>::unpack2(pk[hf * 8 + i]), make_float2(-1.f, -1.f), pp[i]);
-                pk[16 + hf * 8 + i] = Io<__half>::pack2(lo.x, lo.y);
+                const float2 lo = __ffma2_rn(Io<__half>::unpack2(pk[i0 + i]), make_float2(-1.f, -1.f), pp[i]);
+                pk[16 + i0 + i] = Io<__half>::pack2(lo.x, lo.y);
               }
             }
           }
@@ -572,15 +621,13 @@ TcPlan tc_plan(const TrnAttnQ8Args& a) {
   return w;
 }
 
-template <typename T, int D>
-int launch_typed(const TrnAttnQ8Args& a, cudaStream_t st, const DeviceState& ds) {
+template <typename T, int D, int GRP>
+int launch_grp(const TrnAttnQ8Args& a, cudaStream_t st, const DeviceState& ds) {
   using SM = TcSmem<D>;
   TcPlan w = tc_plan(a);
   if (a.workspace == nullptr) w.n_splits = 1;
   TcParams tp{};
   tp.c = q8_params(a, ds);
-  tp.k = a.cache.k;
-  tp.v = a.cache.v;
   tp.pairs = w.pairs;
   tp.n_splits = w.n_splits;
   tp.c.tiles = w.tiles;
@@ -593,11 +640,20 @@ int launch_typed(const TrnAttnQ8Args& a, cudaStream_t st, const DeviceState& ds)
   }
   const long long grid = static_cast<long long>(a.B) * a.Hkv * w.pairs * w.n_splits;
   if (grid > 0x7fffffffLL || static_cast<long long>(a.B) * a.Hkv * w.tiles * w.n_splits > 0x7fffffffLL) return TRN_E_SHAPE;
-  auto kern = attn_q8_tc_kernel<T, D>;
-  const int rc = ensure_dyn_smem(reinterpret_cast<const void*>(kern), SM::kTotal, ds.device);
+  CUtensorMap tm_k, tm_v;
+  int rc = make_code_tmap(&tm_k, &tp.c.ki, a.cache.k, a.cache.S, a.Hkv, a.B, D, kTcKeys);
+  if (rc == TRN_OK) rc = make_code_tmap(&tm_v, &tp.c.vi, a.cache.v, a.cache.S, a.Hkv, a.B, D, kTcKeys);
   if (rc != TRN_OK) return rc;
-  TRN_CUDA_TRY(launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(kTcThreads), SM::kTotal, st, tp));
+  auto kern = attn_q8_tc_kernel<T, D, GRP>;
+  rc = ensure_dyn_smem(reinterpret_cast<const void*>(kern), SM::kTotal, ds.device);
+  if (rc != TRN_OK) return rc;
+  TRN_CUDA_TRY(launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(kTcThreads), SM::kTotal, st, tm_k, tm_v, tp));
   return w.n_splits > 1 ? launch_q8_join(tp.c, a, true, st) : TRN_OK;
+}
+
+template <typename T, int D>
+int launch_typed(const TrnAttnQ8Args& a, cudaStream_t st, const DeviceState& ds) {
+  return a.cache.block == 16 ? launch_grp<T, D, 16>(a, st, ds) : launch_grp<T, D, 32>(a, st, ds);
 }
 
 }  // namespace

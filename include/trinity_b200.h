@@ -387,8 +387,13 @@ typedef struct {
   int kv_len_all;
   int B, Hkv, D;
   int keep, recent, first;
+  void* workspace;                /* optional device scratch of trinity_cache_evict_workspace() bytes: lets the whole GPU sum
+                                     the score heads of long rows.  NULL: summed by the CTAs that select (same result) */
+  size_t workspace_bytes;
 } TrnCacheEvictArgs;
 int trinity_cache_evict(const TrnCacheEvictArgs* a, void* cuda_stream);
+/* Scratch for this shape (reads B, Hs, Hkv, src.S); 0: none is used. */
+size_t trinity_cache_evict_workspace(const TrnCacheEvictArgs* a);
 
 /* ------------------------------------------------------------------------------------------------
  * Whole block, the unit the reference's generated forward() computes (TritonGen.py:590-708):

@@ -30,7 +30,7 @@ EXPORTS = (
     "trinity_rmsnorm", "trinity_qkv_project", "trinity_lora", "trinity_gmlp", "trinity_attention", "trinity_attention_workspace",
     "trinity_attn_colstats", "trinity_topk",
     "trinity_cache_append", "trinity_cache_read", "trinity_attention_q8", "trinity_attention_q8_workspace",
-    "trinity_cache_evict",
+    "trinity_cache_evict", "trinity_cache_evict_workspace",
     "trinity_attn_block_workspace", "trinity_attn_block", "trinity_attn_block_host",
     "trinity_static_scratch_capacity", "trinity_attn_block_static", "trinity_convert",
 )
@@ -143,7 +143,8 @@ class TrnCacheEvictArgs(C.Structure):
         ("src", TrnCacheQ8), ("dst", TrnCacheQ8), ("scores", C.c_void_p), ("score_stride_b", C.c_int64),
         ("score_stride_h", C.c_int64), ("Hs", C.c_int), ("idx", C.c_void_p), ("scores_out", C.c_void_p),
         ("kv_len_out", C.c_void_p), ("kv_len", C.c_void_p), ("kv_len_all", C.c_int), ("B", C.c_int), ("Hkv", C.c_int),
-        ("D", C.c_int), ("keep", C.c_int), ("recent", C.c_int), ("first", C.c_int),
+        ("D", C.c_int), ("keep", C.c_int), ("recent", C.c_int), ("first", C.c_int), ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t),
     ]
 
 
@@ -216,6 +217,8 @@ def load() -> C.CDLL:
     lib.trinity_attention_workspace.argtypes = [C.POINTER(TrnAttnArgs)]
     lib.trinity_attention_q8_workspace.restype = C.c_size_t
     lib.trinity_attention_q8_workspace.argtypes = [C.POINTER(TrnAttnQ8Args)]
+    lib.trinity_cache_evict_workspace.restype = C.c_size_t
+    lib.trinity_cache_evict_workspace.argtypes = [C.POINTER(TrnCacheEvictArgs)]
     lib.trinity_clear_kernel_status.restype = C.c_int
     lib.trinity_clear_kernel_status.argtypes = []
     lib.trinity_selftest_wait_timeout.restype = C.c_int

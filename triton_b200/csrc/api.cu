@@ -376,6 +376,8 @@ int trinity_attention_q8(const TrnAttnQ8Args* a, void* cuda_stream) {
 
 size_t trinity_attention_q8_workspace(const TrnAttnQ8Args* a) { return a == nullptr ? 0 : attention_q8_workspace(*a); }
 
+size_t trinity_cache_evict_workspace(const TrnCacheEvictArgs* a) { return a == nullptr ? 0 : cache_evict_workspace(*a); }
+
 int trinity_cache_evict(const TrnCacheEvictArgs* a, void* cuda_stream) {
   if (a == nullptr) return TRN_E_NULL;
   int rc = check_cache_evict(*a);

@@ -52,13 +52,31 @@ __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
   return v;
 }
 
+// Long rows with many score heads: the heads' sums by the whole GPU first.  (Widening to 64 bits runs at a few lanes per
+// clock: two clusters of 8 CTAs took 30 us for 71 heads of 32768 positions.)
+constexpr int kEvSumThreads = 128;
+__global__ void __launch_bounds__(kEvSumThreads)
+evict_sum_kernel(const float* __restrict__ scores, long long sc_sb, long long sc_sh, int group, KvLen len, int Hkv, int S, float* __restrict__ out) {
+  griddep_wait();
+  griddep_launch();
+  const int tiles = (S + kEvSumThreads - 1) / kEvSumThreads;
+  const int row = static_cast<int>(blockIdx.x) / tiles, j = static_cast<int>(blockIdx.x) % tiles * kEvSumThreads + static_cast<int>(threadIdx.x);
+  const int b = row / Hkv, h = row % Hkv;
+  if (j >= len(b)) return;
+  const float* src = scores + b * sc_sb + static_cast<long long>(h) * group * sc_sh + j;
+  double acc = 0.0;
+#pragma unroll 16
+  for (int g = 0; g < group; ++g) acc += static_cast<double>(src[g * sc_sh]);
+  out[static_cast<long long>(row) * S + j] = static_cast<float>(acc);
+}
+
 __global__ void __launch_bounds__(kEvThreads)
 evict_select_kernel(const __grid_constant__ EvictParams p, int cluster) {
   extern __shared__ __align__(16) uint32_t ev_keys[];          // [slice]
   // Three histograms in turn, so that one cluster barrier a pass is enough: pass i clears the one of pass i + 1, which the
   // other CTAs last read in pass i - 2, before the barrier of pass i - 1.
   __shared__ uint32_t hist[3][256];
-  __shared__ uint32_t warp_sum[8];
+  __shared__ uint32_t sum_of[256];
   __shared__ uint32_t found[3];                                // bin of the last kept key, keys above that bin, keys in it
   __shared__ uint32_t warp_gt[kEvWarps], warp_eq[kEvWarps];
   __shared__ uint32_t cta_cnt[2];
@@ -87,7 +105,7 @@ evict_select_kernel(const __grid_constant__ EvictParams p, int cluster) {
     // kEvAhead positions at a time, so that enough loads are under way: a row's sum is one chain of Hs / Hkv adds
     for (int j0 = tid; j0 < cnt; j0 += kEvAhead * kEvThreads) {
       double acc[kEvAhead] = {};
-#pragma unroll 4
+#pragma unroll 6
       for (int g = 0; g < p.group; ++g) {
         const float* src = sc + g * p.sc_sh + j0;
 #pragma unroll
@@ -116,31 +134,45 @@ evict_select_kernel(const __grid_constant__ EvictParams p, int cluster) {
       if (shift == 32 || (k >> shift) == prefix) atomicAdd(&hist[buf][(k >> ns) & 255u], 1u);
     }
     if (tid < 256) hist[buf == 2 ? 0 : buf + 1][tid] = 0u;
-    if (cluster > 1) cluster_sync_all(); else __syncthreads();
-    // bins from the largest: thread t owns bin 255 - t
-    uint32_t c = 0u;
-    if (tid < 256) {
-      if (cluster > 1) {
-        const uint32_t a = smem_u32(&hist[buf][255 - tid]);
-        for (int r = 0; r < cluster; ++r) c += ld_cluster_u32(map_to_rank(a, static_cast<uint32_t>(r)));
-      } else {
-        c = hist[buf][255 - tid];
-      }
-    }
-    uint32_t incl = c;
+    const uint32_t* bins = hist[buf];
+    if (cluster > 1) {
+      cluster_sync_all();
+      if (tid < 256) {
+        const uint32_t a = smem_u32(&hist[buf][tid]);
+        uint32_t c = 0u;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
+        for (int r = 0; r < kEvMaxCluster; ++r)
+          if (r < cluster) c += ld_cluster_u32(map_to_rank(a, static_cast<uint32_t>(r)));
+        sum_of[tid] = c;
+      }
+      bins = sum_of;
     }
-    if (warp < 8 && lane == 31) warp_sum[warp] = incl;
     __syncthreads();
-    if (tid < 256) {
-      for (int i = 0; i < warp; ++i) incl += warp_sum[i];
-      if (incl >= need && incl - c < need) {                   // exactly one bin holds the last kept key
-        found[0] = static_cast<uint32_t>(255 - tid);
-        found[1] = incl - c;
-        found[2] = c;
+    if (warp == 0) {
+      // lane L owns bins 255 - 8 L ... 248 - 8 L, from the largest
+      uint32_t c[8], mine = 0u;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        c[i] = bins[255 - 8 * lane - i];
+        mine += c[i];
+      }
+      uint32_t incl = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      uint32_t above = incl - mine;
+      if (above < need && incl >= need) {                      // the last kept key is in one of this lane's bins
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (above < need && above + c[i] >= need) {
+            found[0] = static_cast<uint32_t>(255 - 8 * lane - i);
+            found[1] = above;
+            found[2] = c[i];
+          }
+          above += c[i];
+        }
       }
     }
     __syncthreads();
@@ -149,7 +181,6 @@ evict_select_kernel(const __grid_constant__ EvictParams p, int cluster) {
     have = found[2];
     shift = ns;
     buf = buf == 2 ? 0 : buf + 1;
-    __syncthreads();                                           // found and warp_sum are free for the next pass
   }
   // kept: key >> shift above prefix, or equal to it and among the first `need` of those.  need == have: all of them.
   // ---- counts per warp (each owns a contiguous piece of the slice), then per CTA and cluster
@@ -281,6 +312,9 @@ void byte_range(const TrnHeadTensor& t, int B, int S, int H, int D, int elem, ui
   *hi = *lo + static_cast<uintptr_t>(((B - 1) * t.stride_b + (S - 1) * t.stride_s + (H - 1) * t.stride_h + D) * elem);
 }
 
+// whether the score heads are summed by a launch of their own: many scores a row, and scratch for the sums
+bool evict_sums_first(const TrnCacheEvictArgs& a) { return a.workspace != nullptr && cache_evict_workspace(a) > 0; }
+
 template <int RB, bool Q8>
 int launch_move(const MoveParams& p, unsigned grid, cudaStream_t st) {
   TRN_CUDA_TRY(launch_pdl(evict_move_kernel<RB, Q8>, dim3(grid), dim3(kEvMoveThreads), 0, st, p));
@@ -289,7 +323,16 @@ int launch_move(const MoveParams& p, unsigned grid, cudaStream_t st) {
 
 }  // namespace
 
+// below about 32 K scores a row the launch costs more than the sums
+size_t cache_evict_workspace(const TrnCacheEvictArgs& a) {
+  if (a.B <= 0 || a.Hkv <= 0 || a.Hs <= a.Hkv || a.Hs % a.Hkv != 0 || a.src.S <= 0) return 0;
+  if (static_cast<long long>(a.src.S) * (a.Hs / a.Hkv) <= 32768) return 0;
+  return static_cast<size_t>(a.B) * a.Hkv * a.src.S * sizeof(float);
+}
+
 int check_cache_evict(const TrnCacheEvictArgs& a) {
+  if (a.workspace != nullptr && ((reinterpret_cast<uintptr_t>(a.workspace) & 3u) != 0 || a.workspace_bytes < cache_evict_workspace(a)))
+    return TRN_E_WORKSPACE;
   if (a.scores == nullptr || a.idx == nullptr) return TRN_E_NULL;
   if (a.src.block != a.dst.block) return TRN_E_VARIANT;
   if (a.B <= 0 || a.Hkv <= 0 || a.Hs <= 0 || a.Hs % a.Hkv != 0) return TRN_E_SHAPE;
@@ -343,15 +386,22 @@ int launch_cache_evict(const TrnCacheEvictArgs& a, cudaStream_t st, const Device
   const long long rows = static_cast<long long>(a.B) * a.Hkv;
   const int longest = a.kv_len != nullptr ? a.src.S : min(max(a.kv_len_all, 0), a.src.S);
 
+  const int group = a.Hs / a.Hkv;
+  const bool sum_first = evict_sums_first(a);
   // a cluster pays a barrier among its CTAs for each digit: it splits a row only where its scores are many (and SMs idle)
   int cluster = 1;
-  const long long row_scores = static_cast<long long>(longest) * (a.Hs / a.Hkv);
+  const long long row_scores = static_cast<long long>(longest) * (sum_first ? 1 : group);
   while (cluster < kEvMaxCluster && row_scores > 8192LL * cluster && rows * cluster * 2 <= ds.sm_count) cluster *= 2;
   while (cluster < kEvMaxCluster && longest > 32768 * cluster) cluster *= 2;      // 128 KB of keys at most
   EvictParams p{};
   p.scores = a.scores;
   p.sc_sb = a.score_stride_b; p.sc_sh = a.score_stride_h;
-  p.group = a.Hs / a.Hkv;
+  p.group = group;
+  if (sum_first) {
+    p.scores = static_cast<const float*>(a.workspace);
+    p.sc_sb = static_cast<long long>(a.Hkv) * a.src.S; p.sc_sh = a.src.S;
+    p.group = 1;
+  }
   p.idx = a.idx; p.scores_out = a.scores_out; p.len_out = a.kv_len_out;
   p.len = KvLen{a.kv_len, a.kv_len_all, a.src.S};
   p.Hkv = a.Hkv; p.keep = a.keep; p.recent = a.recent; p.first = a.first;
@@ -377,6 +427,13 @@ int launch_cache_evict(const TrnCacheEvictArgs& a, cudaStream_t st, const Device
   const size_t smem = static_cast<size_t>(p.slice) * sizeof(uint32_t);
   const int rc = ensure_dyn_smem(reinterpret_cast<const void*>(evict_select_kernel), 32768 * 4, ds.device);
   if (rc != TRN_OK) return rc;
+  if (sum_first) {
+    const long long sum_grid = rows * ((a.src.S + kEvSumThreads - 1) / kEvSumThreads);
+    if (sum_grid > 0x7fffffffLL) return TRN_E_SHAPE;
+    TRN_CUDA_TRY(launch_pdl(evict_sum_kernel, dim3(static_cast<unsigned>(sum_grid)), dim3(kEvSumThreads), 0, st, a.scores,
+                            static_cast<long long>(a.score_stride_b), static_cast<long long>(a.score_stride_h), group, p.len, a.Hkv,
+                            a.src.S, static_cast<float*>(a.workspace)));
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(rows * cluster), 1, 1);
   cfg.blockDim = dim3(kEvThreads, 1, 1);

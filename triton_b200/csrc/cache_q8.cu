@@ -77,12 +77,24 @@ cache_append_kernel(const __grid_constant__ AppendParams p) {
   }
   top = block_max(top);
   const bool all_finite = top < kInf;
+  // the paths below that few blocks take are rolled loops that read the rows again: unrolled over the pieces in registers,
+  // they were most of the kernel's code, and every CTA waited for it to be fetched (prompts: 32 us against 24)
+  auto again = [&](int i, uint32_t (&w)[4], int& row, int& seg) {
+    const int v = i * kAppendThreads + static_cast<int>(threadIdx.x);
+    row = v / SEG;
+    seg = v % SEG;
+    if (row < older || first + row >= end) return false;
+    const uint4 y = *reinterpret_cast<const uint4*>(x0 + (first + row - held) * src.stride_s + seg * 8);
+    w[0] = y.x; w[1] = y.y; w[2] = y.z; w[3] = y.w;
+    return true;
+  };
   if (!all_finite) {
     top = 0u;
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < VPT; ++i) {
-      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
+      uint32_t w[4];
+      int row, seg;
+      if (!again(i, w, row, seg)) continue;
       for (int e = 0; e < 4; ++e) {
         const uint32_t a = w[e] & 0x7fffu, c = (w[e] >> 16) & 0x7fffu;
         if (a < kInf) top = max(top, a);
@@ -97,44 +109,50 @@ cache_append_kernel(const __grid_constant__ AppendParams p) {
   const bool grew = !(s_old >= need);
   const float s = grew ? need : s_old;
   if (threadIdx.x == 0 && (grew || older == 0)) *slot = s;
+  auto put = [&](int row, int seg, const float (&f)[8]) {
+    uint2 r;
+    r.x = f32_to_e4m3x2(f[0], f[1]) | (f32_to_e4m3x2(f[2], f[3]) << 16);
+    r.y = f32_to_e4m3x2(f[4], f[5]) | (f32_to_e4m3x2(f[6], f[7]) << 16);
+    *reinterpret_cast<uint2*>(c0 + row * code.stride_s + seg * 8) = r;
+  };
+  if (older > 0 && grew) {                                               // older codes move to the larger scale
+    const float ratio = s_old / s;
+#pragma unroll 1
+    for (int v = static_cast<int>(threadIdx.x); v < older * SEG; v += kAppendThreads) {
+      const int row = v / SEG, seg = v % SEG;
+      const uint2 c = *reinterpret_cast<const uint2*>(c0 + row * code.stride_s + seg * 8);
+      const float2 a0 = e4m3x2_to_f32(c.x & 0xffffu), a1 = e4m3x2_to_f32(c.x >> 16);
+      const float2 a2 = e4m3x2_to_f32(c.y & 0xffffu), a3 = e4m3x2_to_f32(c.y >> 16);
+      put(row, seg, {a0.x * ratio, a0.y * ratio, a1.x * ratio, a1.y * ratio, a2.x * ratio, a2.y * ratio, a3.x * ratio, a3.y * ratio});
+    }
+  }
   // a power of two has an exact reciprocal; a foreign scale (a cache the caller filled) divides
-  const bool pow2 = (__float_as_uint(s) & 0x7fffffu) == 0u;
-  const float inv = 1.0f / s;
-  const float ratio = s_old / s;
+  if (all_finite && (__float_as_uint(s) & 0x7fffffu) == 0u) {
+    const float inv = 1.0f / s;
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const int v = i * kAppendThreads + static_cast<int>(threadIdx.x);
-    const int row = v / SEG, seg = v % SEG;
-    if (first + row >= end) continue;
-    uint2* dst = reinterpret_cast<uint2*>(c0 + row * code.stride_s + seg * 8);
-    float f[8];
-    if (row >= older) {
-      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+    for (int i = 0; i < VPT; ++i) {
+      const int v = i * kAppendThreads + static_cast<int>(threadIdx.x);
+      const int row = v / SEG, seg = v % SEG;
+      if (row < older || first + row >= end) continue;
+      const float2 a0 = Io<T>::unpack2(x[i].x), a1 = Io<T>::unpack2(x[i].y), a2 = Io<T>::unpack2(x[i].z), a3 = Io<T>::unpack2(x[i].w);
+      put(row, seg, {a0.x * inv, a0.y * inv, a1.x * inv, a1.y * inv, a2.x * inv, a2.y * inv, a3.x * inv, a3.y * inv});
+    }
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < VPT; ++i) {
+      uint32_t w[4];
+      int row, seg;
+      if (!again(i, w, row, seg)) continue;
+      float f[8];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float2 g = Io<T>::unpack2(w[e]);
         f[2 * e] = g.x;
         f[2 * e + 1] = g.y;
       }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (!all_finite) f[e] = fabsf(f[e]) <= FLT_MAX ? f[e] : __uint_as_float(0x7fffffffu);
-        f[e] = pow2 ? f[e] * inv : __fdiv_rn(f[e], s);
-      }
-    } else {
-      if (!grew) continue;
-      const uint2 c = *dst;
-      const uint32_t w[2] = {c.x, c.y};
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float2 a = e4m3x2_to_f32(w[e] & 0xffffu), g = e4m3x2_to_f32(w[e] >> 16);
-        f[4 * e] = a.x * ratio; f[4 * e + 1] = a.y * ratio; f[4 * e + 2] = g.x * ratio; f[4 * e + 3] = g.y * ratio;
-      }
+      for (int e = 0; e < 8; ++e) f[e] = fabsf(f[e]) <= FLT_MAX ? __fdiv_rn(f[e], s) : __uint_as_float(0x7fffffffu);
+      put(row, seg, f);
     }
-    uint2 r;
-    r.x = f32_to_e4m3x2(f[0], f[1]) | (f32_to_e4m3x2(f[2], f[3]) << 16);
-    r.y = f32_to_e4m3x2(f[4], f[5]) | (f32_to_e4m3x2(f[6], f[7]) << 16);
-    *dst = r;
   }
 }
 
@@ -147,11 +165,13 @@ struct ReadParams {
   int Hkv, shift, tiles;
 };
 
-// One CTA per (b, h, tile of positions, keys or values); a thread turns 16 codes into 32 bytes
+// One CTA per (b, h, tile of positions, keys or values); a thread turns 8 codes into 16 bytes, kReadAhead rows at a time: every
+// load and store of a warp covers whole lines
+constexpr int kReadAhead = 4;
 template <typename T, int D>
 __global__ void __launch_bounds__(kReadThreads)
 cache_read_kernel(const __grid_constant__ ReadParams p) {
-  constexpr int SEG = D / 16, ROWS = kReadThreads / SEG, PER = 2;       // PER rows in flight for each thread
+  constexpr int SEG = D / 8, ROWS = kReadThreads / SEG;
   griddep_wait();
   griddep_launch();
   int u = static_cast<int>(blockIdx.x);
@@ -162,34 +182,28 @@ cache_read_kernel(const __grid_constant__ ReadParams p) {
   const int h = u % p.Hkv, b = u / p.Hkv;
   const int n = p.len(b);
   const TrnHeadTensor dst = p.dst[kv], code = p.code[kv];
-  const int seg = static_cast<int>(threadIdx.x) % SEG;
-  const uint8_t* c0 = static_cast<const uint8_t*>(code.ptr) + b * code.stride_b + h * code.stride_h + seg * 16;
-  T* y0 = static_cast<T*>(dst.ptr) + b * dst.stride_b + h * dst.stride_h + seg * 16;
-  uint4 c[PER];
-  float s[PER];
+  const int seg = static_cast<int>(threadIdx.x) % SEG, row0 = tile * kReadAhead * ROWS + static_cast<int>(threadIdx.x) / SEG;
+  const uint8_t* c0 = static_cast<const uint8_t*>(code.ptr) + b * code.stride_b + h * code.stride_h + seg * 8;
+  T* y0 = static_cast<T*>(dst.ptr) + b * dst.stride_b + h * dst.stride_h + seg * 8;
+  uint2 c[kReadAhead];
+  float s[kReadAhead];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int row = (tile * PER + i) * ROWS + static_cast<int>(threadIdx.x) / SEG;
+  for (int i = 0; i < kReadAhead; ++i) {
+    const int row = row0 + i * ROWS;
     if (row < n) {
-      c[i] = *reinterpret_cast<const uint4*>(c0 + row * code.stride_s);
+      c[i] = *reinterpret_cast<const uint2*>(c0 + row * code.stride_s);
       s[i] = *p.scale[kv].at(b, row >> p.shift, h);
     }
   }
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int row = (tile * PER + i) * ROWS + static_cast<int>(threadIdx.x) / SEG;
+  for (int i = 0; i < kReadAhead; ++i) {
+    const int row = row0 + i * ROWS;
     if (row >= n) continue;
-    const uint32_t w[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
-    uint32_t r[8];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 a = e4m3x2_to_f32(w[e] & 0xffffu), g = e4m3x2_to_f32(w[e] >> 16);
-      r[2 * e] = Io<T>::pack2(a.x * s[i], a.y * s[i]);
-      r[2 * e + 1] = Io<T>::pack2(g.x * s[i], g.y * s[i]);
-    }
-    uint4* y = reinterpret_cast<uint4*>(y0 + row * dst.stride_s);
-    y[0] = make_uint4(r[0], r[1], r[2], r[3]);
-    y[1] = make_uint4(r[4], r[5], r[6], r[7]);
+    const float2 a0 = e4m3x2_to_f32(c[i].x & 0xffffu), a1 = e4m3x2_to_f32(c[i].x >> 16);
+    const float2 a2 = e4m3x2_to_f32(c[i].y & 0xffffu), a3 = e4m3x2_to_f32(c[i].y >> 16);
+    *reinterpret_cast<uint4*>(y0 + row * dst.stride_s) =
+        make_uint4(Io<T>::pack2(a0.x * s[i], a0.y * s[i]), Io<T>::pack2(a1.x * s[i], a1.y * s[i]),
+                   Io<T>::pack2(a2.x * s[i], a2.y * s[i]), Io<T>::pack2(a3.x * s[i], a3.y * s[i]));
   }
 }
 
@@ -209,7 +223,7 @@ int append_typed(const TrnCacheAppendArgs& a, const AppendParams& p, unsigned gr
 
 template <typename T, int D>
 int read_typed(const TrnCacheReadArgs& a, ReadParams& p, cudaStream_t st) {
-  constexpr int kRows = 2 * kReadThreads / (D / 16);
+  constexpr int kRows = kReadAhead * kReadThreads / (D / 8);
   const int room = p.len.S, longest = a.kv_len != nullptr ? room : min(max(a.kv_len_all, 0), room);
   p.tiles = (longest + kRows - 1) / kRows;
   const long long grid = 2LL * a.B * a.Hkv * p.tiles;

@@ -119,6 +119,7 @@ int launch_cache_append(const TrnCacheAppendArgs& a, cudaStream_t st);
 int launch_cache_read(const TrnCacheReadArgs& a, cudaStream_t st);
 int launch_cache_evict(const TrnCacheEvictArgs& a, cudaStream_t st, const DeviceState& ds);
 int launch_attention_q8(const TrnAttnQ8Args& a, cudaStream_t st, const DeviceState& ds);
+size_t cache_evict_workspace(const TrnCacheEvictArgs& a);
 size_t attention_q8_workspace(const TrnAttnQ8Args& a);
 int launch_convert(const void* src, void* dst, long long n, int dtype16, int to_fp32, cudaStream_t st,
                    const DeviceState& ds);

@@ -503,11 +503,12 @@ class CacheEvictPlan(_BoundCall):
     multiple of Hkv: the heads of a group are summed; equal scores by the lower position).  ``src``, ``dst``: CacheQ8 of one
     block size, or (k, v) pairs of 16-bit (b, s, h, d) views of one dtype; they must not overlap.
     ``idx`` [B, Hkv, keep] int32: the positions kept, ascending, then -1.  ``scores_out`` [B, Hkv, keep] fp32: their scores,
-    then 0 (the accumulators of the cache they moved to).  ``kv_len_out`` [B] int32: min(kv_len, keep)."""
+    then 0 (the accumulators of the cache they moved to).  ``kv_len_out`` [B] int32: min(kv_len, keep).  ``workspace``: a uint8
+    tensor for the sums of long rows with several score heads (see trinity_cache_evict_workspace); allocated when not given."""
 
     def __init__(self, src, dst, scores: torch.Tensor, *, kv_len, keep: int, recent: int = 0, first: int = 0,
                  idx: Optional[torch.Tensor] = None, scores_out: Optional[torch.Tensor] = None,
-                 kv_len_out: Optional[torch.Tensor] = None):
+                 kv_len_out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None):
         a = L.TrnCacheEvictArgs()
         views = []
         for cache, name in ((src, "src"), (dst, "dst")):
@@ -545,7 +546,14 @@ class CacheEvictPlan(_BoundCall):
         keep_alive = _set_kv_len(a, kv_len, B, S)
         for cache, pair in zip((src, dst), views):
             keep_alive += cache.tensors() if isinstance(cache, CacheQ8) else list(pair)
-        self._bind("trinity_cache_evict", a, keep_alive + [scores, idx, scores_out, kv_len_out])
+        if workspace is None:
+            nbytes = L.load().trinity_cache_evict_workspace(C.byref(a))
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=k.device) if nbytes else None
+        if workspace is not None:
+            if not workspace.is_contiguous():
+                raise ValueError("workspace must be contiguous")
+            a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        self._bind("trinity_cache_evict", a, keep_alive + [scores, idx, scores_out, kv_len_out, workspace])
 
 
 def cache_append(cache: CacheQ8, k: torch.Tensor, v: torch.Tensor, *, kv_len) -> None:

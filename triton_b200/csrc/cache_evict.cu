@@ -53,21 +53,33 @@ __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
 }
 
 // Long rows with many score heads: the heads' sums by the whole GPU first.  (Widening to 64 bits runs at a few lanes per
-// clock: two clusters of 8 CTAs took 30 us for 71 heads of 32768 positions.)
-constexpr int kEvSumThreads = 128;
-__global__ void __launch_bounds__(kEvSumThreads)
+// clock: two clusters of 8 CTAs took 30 us for 71 heads of 32768 positions.)  A CTA takes kEvSumKeys positions, each by
+// kEvSumParts threads that share its heads, so that a position's loads are under way together.
+constexpr int kEvSumKeys = 64, kEvSumParts = 4;
+__global__ void __launch_bounds__(kEvSumKeys * kEvSumParts)
 evict_sum_kernel(const float* __restrict__ scores, long long sc_sb, long long sc_sh, int group, KvLen len, int Hkv, int S, float* __restrict__ out) {
+  __shared__ double part[kEvSumParts][kEvSumKeys];
   griddep_wait();
   griddep_launch();
-  const int tiles = (S + kEvSumThreads - 1) / kEvSumThreads;
-  const int row = static_cast<int>(blockIdx.x) / tiles, j = static_cast<int>(blockIdx.x) % tiles * kEvSumThreads + static_cast<int>(threadIdx.x);
+  const int tiles = (S + kEvSumKeys - 1) / kEvSumKeys;
+  const int row = static_cast<int>(blockIdx.x) / tiles, k = static_cast<int>(threadIdx.x) % kEvSumKeys, q = static_cast<int>(threadIdx.x) / kEvSumKeys;
+  const int j = static_cast<int>(blockIdx.x) % tiles * kEvSumKeys + k;
   const int b = row / Hkv, h = row % Hkv;
-  if (j >= len(b)) return;
-  const float* src = scores + b * sc_sb + static_cast<long long>(h) * group * sc_sh + j;
+  const bool there = j < len(b);
   double acc = 0.0;
-#pragma unroll 16
-  for (int g = 0; g < group; ++g) acc += static_cast<double>(src[g * sc_sh]);
-  out[static_cast<long long>(row) * S + j] = static_cast<float>(acc);
+  if (there) {
+    const int g0 = group * q / kEvSumParts, g1 = group * (q + 1) / kEvSumParts;
+    const float* src = scores + b * sc_sb + static_cast<long long>(h) * group * sc_sh + j;
+#pragma unroll 10
+    for (int g = g0; g < g1; ++g) acc += static_cast<double>(src[g * sc_sh]);
+  }
+  part[q][k] = acc;
+  __syncthreads();
+  if (q == 0 && there) {
+#pragma unroll
+    for (int i = 1; i < kEvSumParts; ++i) acc += part[i][k];
+    out[static_cast<long long>(row) * S + j] = static_cast<float>(acc);
+  }
 }
 
 __global__ void __launch_bounds__(kEvThreads)
@@ -391,7 +403,7 @@ int launch_cache_evict(const TrnCacheEvictArgs& a, cudaStream_t st, const Device
   // a cluster pays a barrier among its CTAs for each digit: it splits a row only where its scores are many (and SMs idle)
   int cluster = 1;
   const long long row_scores = static_cast<long long>(longest) * (sum_first ? 1 : group);
-  while (cluster < kEvMaxCluster && row_scores > 8192LL * cluster && rows * cluster * 2 <= ds.sm_count) cluster *= 2;
+  while (cluster < kEvMaxCluster && (longest > 4096LL * cluster || row_scores > 32768LL * cluster) && rows * cluster * 2 <= ds.sm_count) cluster *= 2;
   while (cluster < kEvMaxCluster && longest > 32768 * cluster) cluster *= 2;      // 128 KB of keys at most
   EvictParams p{};
   p.scores = a.scores;
@@ -428,9 +440,9 @@ int launch_cache_evict(const TrnCacheEvictArgs& a, cudaStream_t st, const Device
   const int rc = ensure_dyn_smem(reinterpret_cast<const void*>(evict_select_kernel), 32768 * 4, ds.device);
   if (rc != TRN_OK) return rc;
   if (sum_first) {
-    const long long sum_grid = rows * ((a.src.S + kEvSumThreads - 1) / kEvSumThreads);
+    const long long sum_grid = rows * ((a.src.S + kEvSumKeys - 1) / kEvSumKeys);
     if (sum_grid > 0x7fffffffLL) return TRN_E_SHAPE;
-    TRN_CUDA_TRY(launch_pdl(evict_sum_kernel, dim3(static_cast<unsigned>(sum_grid)), dim3(kEvSumThreads), 0, st, a.scores,
+    TRN_CUDA_TRY(launch_pdl(evict_sum_kernel, dim3(static_cast<unsigned>(sum_grid)), dim3(kEvSumKeys * kEvSumParts), 0, st, a.scores,
                             static_cast<long long>(a.score_stride_b), static_cast<long long>(a.score_stride_h), group, p.len, a.Hkv,
                             a.src.S, static_cast<float*>(a.workspace)));
   }

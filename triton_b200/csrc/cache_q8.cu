@@ -78,7 +78,7 @@ cache_append_kernel(const __grid_constant__ AppendParams p) {
   top = block_max(top);
   const bool all_finite = top < kInf;
   // the paths below that few blocks take are rolled loops that read the rows again: unrolled over the pieces in registers,
-  // they were most of the kernel's code, and every CTA waited for it to be fetched (prompts: 32 us against 24)
+  // they were most of the kernel's code, and every CTA waited for it to be fetched (8 x 2048 rows of 8 heads of 128: 32.4 us against 17.5)
   auto again = [&](int i, uint32_t (&w)[4], int& row, int& seg) {
     const int v = i * kAppendThreads + static_cast<int>(threadIdx.x);
     row = v / SEG;

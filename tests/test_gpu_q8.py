@@ -273,6 +273,88 @@ def test_attention_q8(B, M, Hq, Hkv, D, S, lens, block, dt, causal, layout):
         _check(o, lse, None, r, q, dt, D, lens, Hq // Hkv)
 
 
+LONG = [
+    # caches too long for one launch of clusters: shares of all chunks, pieces, the merge
+    (3, 1, 8, 2, 128, 9100, [5000, 0, 9100], 64, BF, True),
+    (2, 2, 6, 2, 64, 20000, [17, 19999], 16, HF, True),
+    (40, 1, 4, 4, 64, 4500, None, 32, BF, True),                        # more units than CTAs, many lengths
+    (1, 16, 2, 1, 128, 6000, [6000], 128, HF, True),                    # 32 rows: two tiles of 16
+    (1, 3, 20, 1, 64, 7000, [6990], 16, BF, False),
+    (1, 300, 2, 1, 64, 9000, [8999], 32, HF, True),                     # tensor-core kernel, keys divided among CTAs
+    (2, 9, 71, 1, 64, 5000, [4990, 5], 16, BF, True),
+]
+
+
+@pytest.mark.parametrize("workspace", [True, False])
+@pytest.mark.parametrize("B,M,Hq,Hkv,D,S,lens,block,dt,causal", LONG)
+def test_attention_q8_long(B, M, Hq, Hkv, D, S, lens, block, dt, causal, workspace):
+    lens = [(i * 997) % (S + 1) for i in range(B)] if lens is None else lens
+    q, kc, vc, ks, vs = _attend_inputs(B, M, Hq, Hkv, D, S, block, dt, 41)
+    _spoil_behind(kc, vc, ks, vs, lens, block)
+    r = O.attend(q, _values(kc, ks, block), _values(vc, vs, block), lens, causal, D ** -0.5)
+    cache, _, _ = _cache(kc, vc, ks, vs, block)
+    o = torch.full((B, M, Hq, D), 9.0, dtype=dt, device="cuda")
+    lse = torch.full((B, Hq, M), 9.0, device="cuda")
+    w = torch.full((B, Hkv, S + 1), 5.0, device="cuda") if workspace and M <= 16 else None
+    plan = ops.AttentionQ8Plan(q.cuda(), cache, o, kv_len=torch.tensor(lens, dtype=torch.int32).cuda(), causal=causal, lse=lse, weight=w)
+    if not workspace:
+        plan.args.workspace, plan.args.workspace_bytes = None, 0         # the key range is not divided
+    plan.run()
+    _done()
+    _check(o, lse, w, r, q, dt, D, lens, Hq // Hkv)
+    first = o.clone()
+    if w is not None:
+        assert all(bool((w[b, :, n:] == 5.0).all()) for b, n in enumerate(lens))
+    plan.run()
+    _done()
+    assert torch.equal(o, first)
+
+
+def test_lengths_outside_the_cache_count_as_the_nearer_end():
+    B, Hq, Hkv, D, S, block, dt = 2, 4, 2, 64, 60, 16, BF
+    q, kc, vc, ks, vs = _attend_inputs(B, 1, Hq, Hkv, D, S, block, dt, 43)
+    cache, _, _ = _cache(kc, vc, ks, vs, block)
+    want = ops.attention_q8(q.cuda(), cache, kv_len=torch.tensor([0, S], dtype=torch.int32).cuda())
+    got = ops.attention_q8(q.cuda(), cache, kv_len=torch.tensor([-3, S + 9], dtype=torch.int32).cuda())
+    before = [t.clone() for t in cache.tensors()[2:]] + [t.view(torch.uint8).clone() for t in cache.tensors()[:2]]
+    k = torch.randn(B, 3, Hkv, D, device="cuda").to(dt)
+    ops.cache_append(cache, k, k, kv_len=torch.full((B,), S + 1, dtype=torch.int32, device="cuda"))      # nothing fits
+    out = torch.zeros(B, S, Hkv, D, dtype=dt, device="cuda")
+    ops.cache_read(cache, out[:, :50], out[:, :50].clone(), kv_len=torch.tensor([-1, S + 1], dtype=torch.int32).cuda())
+    _done()
+    assert torch.equal(want, got)
+    after = [t for t in cache.tensors()[2:]] + [t.view(torch.uint8) for t in cache.tensors()[:2]]
+    assert all(torch.equal(a, c) for a, c in zip(before, after))
+    assert bool((out[0] == 0).all()) and bool((out[1, 50:] == 0).all()) and bool((out[1, :50] != 0).any())
+
+
+@pytest.mark.parametrize("which", ["position", "batch"])
+def test_offsets_beyond_32_bits(which):
+    """Caches spread over gigabytes: strides of positions or of batch items that carry offsets past 2^32 bytes."""
+    B, S, Hkv, D, block = 2, 150, 1, 64, 16
+    g = torch.Generator().manual_seed(47)
+    wide = 9_000_000_000
+    sb, ss = (D, 32_000_000) if which == "position" else (4_400_000_000, D)
+    buf = torch.zeros(wide, dtype=torch.uint8, device="cuda")
+    cache = ops.CacheQ8.empty(B, S, Hkv, D, block=block, layout="bshd")
+    spread = [buf[o:].as_strided((B, S, Hkv, D), (sb, ss, D, 1)).view(torch.float8_e4m3fn) for o in (0, 4 * D * S)]
+    far = ops.CacheQ8(*spread, torch.zeros(B, -(-S // block), Hkv, device="cuda"), torch.zeros(B, -(-S // block), Hkv, device="cuda"),
+                      block=block, layout="bshd")
+    k, v = torch.randn(B, S, Hkv, D, generator=g).to(BF).cuda(), torch.randn(B, S, Hkv, D, generator=g).to(BF).cuda()
+    outs = []
+    for c in (cache, far):
+        ops.cache_append(c, k, v, kv_len=0)
+        ko, vo = torch.zeros_like(k), torch.zeros_like(v)
+        ops.cache_read(c, ko, vo, kv_len=S)
+        small = ops.attention_q8(k[:, :4].contiguous(), c, kv_len=S)
+        large = ops.attention_q8(k[:, :100].contiguous(), c, kv_len=S)
+        to = ops.CacheQ8.empty(B, 40, Hkv, D, block=block, layout="bshd")
+        idx = ops.cache_evict(c, to, torch.rand(B, 1, S, generator=torch.Generator().manual_seed(1)).cuda(), kv_len=S, keep=40)
+        outs.append((ko, vo, small, large, idx, to.k.view(torch.uint8), to.v_scale))
+    _done()
+    assert all(torch.equal(a, c) for a, c in zip(*outs))
+
+
 @pytest.mark.parametrize("M,Hq,Hkv,D,n,block,dt", [(4, 4, 2, 128, 77, 16, BF), (8, 4, 1, 64, 200, 32, HF), (160, 2, 1, 128, 300, 64, BF),
                                                    (40, 8, 2, 64, 170, 16, HF)])
 def test_attention_q8_nan_reaches_exactly_the_rows_that_see_it(M, Hq, Hkv, D, n, block, dt):
@@ -426,6 +508,29 @@ def test_evict(B, Hs, Hkv, D, S, lens, keep, recent, first, block, dt, layout, k
                     assert torch.equal(to[b, h, :m].cpu(), have[b, h][kept[h]]) and bool((to[b, h, m:] == 3.0).all())
 
 
+def test_evict_sums_the_same_with_and_without_scratch():
+    B, Hs, Hkv, n, keep = 2, 21, 3, 9001, 1000
+    g = torch.Generator().manual_seed(51)
+    scores = torch.exp(3 * torch.randn(B, Hs, n, generator=g))
+    k = torch.randn(B, n, Hkv, 64, generator=g).to(BF).cuda()
+    kv_len = torch.tensor([n, 5000], dtype=torch.int32).cuda()
+    outs = []
+    for scratch in (True, False):
+        to, sout = torch.zeros(B, keep, Hkv, 64, dtype=BF, device="cuda"), torch.zeros(B, Hkv, keep, device="cuda")
+        plan = ops.CacheEvictPlan((k, k), (to, to.clone()), scores.cuda(), kv_len=kv_len, keep=keep, recent=7, first=2, scores_out=sout)
+        assert plan.args.workspace_bytes == 4 * B * Hkv * n
+        if not scratch:
+            plan.args.workspace = None
+        plan.run()
+        _done()
+        outs.append((plan.idx, sout, to))
+    assert all(torch.equal(a, c) for a, c in zip(*outs))
+    for b, m in enumerate((n, 5000)):
+        kept, w = O.select(scores[b, :, :m], m, keep, 7, 2, Hs // Hkv)
+        for h in range(Hkv):
+            assert outs[0][0][b, h].tolist() == kept[h] and torch.equal(outs[0][1][b, h].cpu(), w[h][kept[h]])
+
+
 def test_evict_long_rows_with_many_equals():
     """262144 positions, the longest a call takes, three values only."""
     S, keep = 262144, 70001
@@ -496,17 +601,18 @@ def test_a_decode_loop_with_eviction():
             assert bool(((acc[b, :, :n].double().cpu() - want[b, :, :n]).abs() <= 1e-3 * want[b, :, :n]).all())
 
 
-def test_captured_steps_replay_with_growing_lengths():
-    """append + lengths + attention + eviction captured once; replays equal direct calls bit for bit.  Two graphs that share
-    one scratch area, replayed one after the other."""
-    B, Hq, Hkv, D, block, S, dt = 2, 8, 2, 128, 32, 600, HF
+@pytest.mark.parametrize("S", [600, 9000])            # one launch of clusters; shares and the merge
+def test_captured_steps_replay_with_growing_lengths(S):
+    """append + lengths + attention captured once; replays equal direct calls bit for bit.  Two graphs that share one scratch
+    area, replayed one after the other."""
+    B, Hq, Hkv, D, block, dt = 2, 8, 2, 128, 32, HF
     g = torch.Generator().manual_seed(23)
     def fresh():
         gg = torch.Generator().manual_seed(29)
         q, kc, vc, ks, vs = _attend_inputs(B, 1, Hq, Hkv, D, S, block, dt, 29)
         cache, _, _ = _cache(kc, vc, ks, vs, block)
         return dict(cache=cache, q=q.cuda(), k=torch.randn(B, 1, Hkv, D, generator=gg).to(dt).cuda(), o=torch.zeros(B, 1, Hq, D, dtype=dt, device="cuda"),
-                    n=torch.tensor([500, 37], dtype=torch.int32, device="cuda"), w=torch.zeros(B, Hkv, S, device="cuda"))
+                    n=torch.tensor([S - 100, 37], dtype=torch.int32, device="cuda"), w=torch.zeros(B, Hkv, S, device="cuda"))
     ws = torch.empty(ops.attention_q8_workspace_bytes(B, 1, Hq, Hkv, D, S, weight=True), dtype=torch.uint8, device="cuda")
     def step(t):
         t["append"].run()

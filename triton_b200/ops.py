@@ -398,14 +398,15 @@ class _BoundCall:
         self.args = args
         self._ref = C.byref(args)
         self._fn = getattr(L.load(), name)
+        # the raw-handle forms of current_device() and current_stream(): a decode step is a few microseconds of work
+        self._get_device, self._get_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
     def run(self) -> None:
-        # the raw-handle forms of current_device() and current_stream(): a decode step is a few microseconds of work
-        if torch._C._cuda_getDevice() == self._index:
-            rc = self._fn(self._ref, torch._C._cuda_getCurrentRawStream(self._index))
+        if self._get_device() == self._index:
+            rc = self._fn(self._ref, self._get_stream(self._index))
         else:
             with torch.cuda.device(self._index):
-                rc = self._fn(self._ref, torch._C._cuda_getCurrentRawStream(self._index))
+                rc = self._fn(self._ref, self._get_stream(self._index))
         if rc != 0:
             L.check(rc)
 

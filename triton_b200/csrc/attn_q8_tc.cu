@@ -32,11 +32,12 @@ static_assert(kTcConvert == 32 * kTcMmaWarp && kTcThreads == 32 * (kTcMmaWarp + 
 constexpr int kTcTmemCols = 512;              // S0 [0,128) S1 [128,256) O0 [256,256+D) O1 [384,384+D)
 constexpr float kTcRescale = 8.0f;            // log2 units a row's maximum may pass the offset in use
 constexpr float kTcPBias = 6.0f;              // P' <= 2^14 with it
-constexpr int kTcMaxSplits = 16;
+constexpr int kTcMinShare = 2;                // key blocks a CTA takes at least where they are divided
 
 struct TcParams {
   Q8Params c;
-  int pairs, n_splits;
+  int pairs;
+  int ctas;          // CTAs the key blocks of all pairs of tiles are divided among; 0: a CTA per pair
 };
 
 template <int D>
@@ -146,13 +147,58 @@ attn_q8_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
   griddep_wait();                              // q, the codes and the lengths may come from the launch before
   griddep_launch();
-  const bool dead = *reinterpret_cast<volatile int*>(p.status) != 0;
+  bool dead = *reinterpret_cast<volatile int*>(p.status) != 0;
 
-  // ---- which rows and blocks: late (heavy) pairs of tiles first
-  const int per_split = p.B * p.Hkv * tp.pairs;
-  const int split = static_cast<int>(blockIdx.x) / per_split, cta = static_cast<int>(blockIdx.x) % per_split;
-  const int pair = tp.pairs - 1 - cta / (p.B * p.Hkv), bh = cta % (p.B * p.Hkv);
-  const int b = bh / p.Hkv, h = bh % p.Hkv;
+  // ---- which rows and blocks
+  const int cta = static_cast<int>(blockIdx.x);
+  int b, h, pair, split = 0, pieces = 1;
+  if (tp.ctas == 0) {
+    pair = tp.pairs - 1 - cta / (p.B * p.Hkv);                     // late (heavy) pairs of tiles first
+    h = cta % p.Hkv;
+    b = cta / p.Hkv % p.B;
+  } else {
+    // A pair's key blocks are cut into pieces of at most `share`: the least share with which all pairs' pieces find a CTA
+    const int per = p.Hkv * tp.pairs;
+    auto blocks_of = [&](int i) { return max((p.len(i) + kTcKeys - 1) / kTcKeys, 1); };
+    unsigned sum = 0u;
+    for (int i = lane; i < p.B; i += 32) sum += blocks_of(i);
+    const int total = static_cast<int>(__reduce_add_sync(0xffffffffu, sum)) * per;
+    int share = max((total + tp.ctas - 1) / tp.ctas, kTcMinShare);
+    for (;;) {
+      unsigned c = 0u;
+      for (int i = lane; i < p.B; i += 32) c += (blocks_of(i) + share - 1) / share;
+      if (static_cast<int>(__reduce_add_sync(0xffffffffu, c)) * per <= tp.ctas || share >= total) break;
+      share += max(share >> 3, 1);
+    }
+    int at = cta;
+    b = -1;
+    for (int b0 = 0; b0 < p.B; b0 += 32) {
+      const int c = b0 + lane < p.B ? (blocks_of(b0 + lane) + share - 1) / share * per : 0;
+      int incl = c;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      const uint32_t past = __ballot_sync(0xffffffffu, incl > at);
+      if (past != 0u) {
+        const int l = __ffs(past) - 1;
+        b = b0 + l;
+        at -= __shfl_sync(0xffffffffu, incl - c, l);
+        break;
+      }
+      at -= __shfl_sync(0xffffffffu, incl, 31);
+    }
+    const bool idle = b < 0;                   // more CTAs than pieces: no blocks, and nothing written
+    if (idle) b = 0;
+    pieces = (blocks_of(b) + share - 1) / share;
+    split = idle ? 0 : at % pieces;
+    const int u = idle ? 0 : min(at / pieces, per - 1);
+    h = u / tp.pairs;
+    pair = u % tp.pairs;
+    dead = dead || idle;
+  }
+  const int bh = b * p.Hkv + h;
   const int n = p.len(b);
   int n_blocks[2], lim_max[2];
 #pragma unroll
@@ -162,10 +208,10 @@ attn_q8_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     n_blocks[t] = (lim_max[t] + kTcKeys) / kTcKeys;
   }
   int j0 = 0;
-  if (tp.n_splits > 1) {
+  if (pieces > 1) {
     const int full = max(n_blocks[0], n_blocks[1]);
-    j0 = full * split / tp.n_splits;
-    const int j1 = full * (split + 1) / tp.n_splits;
+    j0 = full * split / pieces;
+    const int j1 = full * (split + 1) / pieces;
     n_blocks[0] = max(0, min(j1, n_blocks[0]) - j0);
     n_blocks[1] = max(0, min(j1, n_blocks[1]) - j0);
   }
@@ -532,8 +578,10 @@ attn_q8_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     }
     if (ok && !dead && warp_active) {
       const int tile = 2 * pair + t;
-      const long long slot = static_cast<long long>(bh * p.tiles + tile) * tp.n_splits + split;
-      const bool parts = tp.n_splits > 1, any_nan = *reinterpret_cast<volatile int*>(nan_any) != 0;
+      // a piece begins a new pair, a new CTA or both: pair + CTA numbers the pieces, tile 1's behind all of tile 0's
+      const int all_pairs = p.B * p.Hkv * tp.pairs;
+      const long long slot = static_cast<long long>(t) * (all_pairs + tp.ctas) + bh * tp.pairs + pair + cta;
+      const bool parts = pieces > 1, any_nan = *reinterpret_cast<volatile int*>(nan_any) != 0;
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         if (nb > 0) {
@@ -576,9 +624,9 @@ attn_q8_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         else if (p.lse != nullptr)
           p.lse[(static_cast<long long>(b) * p.Hq + h * p.G + r % p.G) * p.M + r / p.G] = m_run + log2f(l_run);
       }
-      if (parts && split == 0 && lrow == 0) {
-        const int u = bh * p.tiles + tile;                         // its pieces' slots begin at u * n_splits
-        p.pieces[u] = make_int2(u * (tp.n_splits - 1), u * (tp.n_splits - 1) + tp.n_splits - 1);
+      if (p.pieces != nullptr && split == 0 && lrow == 0) {        // where the merge finds them: slot = unit + entry
+        const int u = bh * p.tiles + tile, first = static_cast<int>(slot) - u;
+        p.pieces[u] = make_int2(first, first + pieces - 1);
       }
       tc_fence_before();
     }
@@ -598,22 +646,22 @@ attn_q8_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 }
 
 struct TcPlan {
-  int tiles, pairs, n_splits;
+  int tiles, pairs, ctas;
   size_t ml_off, o_off, piece_off, total;
 };
 
-// key blocks divided among CTAs while that fills SMs, at least two blocks each
+// key blocks divided among one CTA for each SM where that is at least two CTAs a pair and two blocks a CTA
 TcPlan tc_plan(const TrnAttnQ8Args& a) {
   TcPlan w{};
   const int R = a.M * (a.Hq / a.Hkv);
   w.tiles = (R + kTcRows - 1) / kTcRows;
   w.pairs = (w.tiles + 1) / 2;
-  const long long ctas = static_cast<long long>(a.B) * a.Hkv * w.pairs;
+  const long long pairs = static_cast<long long>(a.B) * a.Hkv * w.pairs;
   const int longest = a.kv_len != nullptr ? a.cache.S : min(max(a.kv_len_all, 1), a.cache.S);
-  const long long blocks = (longest - 1) / kTcKeys + 1;
-  w.n_splits = static_cast<int>(max(min(min(kAttnNominalSMs / ctas, blocks / 2), static_cast<long long>(kTcMaxSplits)), 1LL));
-  if (w.n_splits == 1) return w;
-  const size_t rows = static_cast<size_t>(a.B) * a.Hkv * w.tiles * w.n_splits * kTcRows;
+  const int blocks = (longest - 1) / kTcKeys + 1;
+  if (2 * pairs > kAttnNominalSMs || blocks < 2 * kTcMinShare) return w;
+  w.ctas = static_cast<int>(min(static_cast<long long>(kAttnNominalSMs), pairs * ((blocks + kTcMinShare - 1) / kTcMinShare)));
+  const size_t rows = 2 * static_cast<size_t>(pairs + w.ctas) * kTcRows;
   w.ml_off = 0;
   w.o_off = up256(rows * sizeof(float2));
   w.piece_off = w.o_off + up256(rows * a.D * sizeof(float));
@@ -625,21 +673,21 @@ template <typename T, int D, int GRP>
 int launch_grp(const TrnAttnQ8Args& a, cudaStream_t st, const DeviceState& ds) {
   using SM = TcSmem<D>;
   TcPlan w = tc_plan(a);
-  if (a.workspace == nullptr) w.n_splits = 1;
+  if (a.workspace == nullptr) w.ctas = 0;
   TcParams tp{};
   tp.c = q8_params(a, ds);
   tp.pairs = w.pairs;
-  tp.n_splits = w.n_splits;
+  tp.ctas = w.ctas;
   tp.c.tiles = w.tiles;
   tp.c.tile_rows = kTcRows;
-  if (w.n_splits > 1) {
+  if (w.ctas > 0) {
     uint8_t* ws = static_cast<uint8_t*>(a.workspace);
     tp.c.part_ml = reinterpret_cast<float2*>(ws + w.ml_off);
     tp.c.part_o = reinterpret_cast<float*>(ws + w.o_off);
     tp.c.pieces = reinterpret_cast<int2*>(ws + w.piece_off);
   }
-  const long long grid = static_cast<long long>(a.B) * a.Hkv * w.pairs * w.n_splits;
-  if (grid > 0x7fffffffLL || static_cast<long long>(a.B) * a.Hkv * w.tiles * w.n_splits > 0x7fffffffLL) return TRN_E_SHAPE;
+  const long long grid = w.ctas > 0 ? w.ctas : static_cast<long long>(a.B) * a.Hkv * w.pairs;
+  if (grid > 0x7fffffffLL || static_cast<long long>(a.B) * a.Hkv * w.tiles > 0x7fffffffLL) return TRN_E_SHAPE;
   CUtensorMap tm_k, tm_v;
   int rc = make_code_tmap(&tm_k, &tp.c.ki, a.cache.k, a.cache.S, a.Hkv, a.B, D, kTcKeys);
   if (rc == TRN_OK) rc = make_code_tmap(&tm_v, &tp.c.vi, a.cache.v, a.cache.S, a.Hkv, a.B, D, kTcKeys);
@@ -648,7 +696,7 @@ int launch_grp(const TrnAttnQ8Args& a, cudaStream_t st, const DeviceState& ds) {
   rc = ensure_dyn_smem(reinterpret_cast<const void*>(kern), SM::kTotal, ds.device);
   if (rc != TRN_OK) return rc;
   TRN_CUDA_TRY(launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(kTcThreads), SM::kTotal, st, tm_k, tm_v, tp));
-  return w.n_splits > 1 ? launch_q8_join(tp.c, a, true, st) : TRN_OK;
+  return w.ctas > 0 ? launch_q8_join(tp.c, a, true, st) : TRN_OK;
 }
 
 template <typename T, int D>

@@ -671,7 +671,7 @@ attn_q8_cluster_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
 // columns a thread; the rest: four positions a thread of a (b, kv head), rows in ascending order.
 constexpr int kQ8JoinThreads = 256;
 constexpr int kQ8JoinWarps = kQ8JoinThreads / 32;
-constexpr int kQ8JoinKeys = 4 * kQ8JoinThreads;
+constexpr int kQ8JoinKeys = 8 * kQ8JoinThreads;
 // maximum and sum of a row over its pieces by one warp; at: the row in the first piece's slot
 __device__ __forceinline__ float2 join_ml(const Q8Params& p, long long at, int here, int lane) {
   float2 mine = make_float2(-INFINITY, 0.f);   // a lane's pieces lane, lane + 32, ...
@@ -703,7 +703,13 @@ attn_q8_join_kernel(const __grid_constant__ Q8Params p, int merge_ctas, int key_
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (static_cast<int>(blockIdx.x) < merge_ctas) {
     const int groups = p.tile_rows / ROWS;     // tile_rows and ROWS are powers of two; at least one
-    const int unit = static_cast<int>(blockIdx.x) / max(groups, 1), r_first = static_cast<int>(blockIdx.x) % max(groups, 1) * ROWS;
+    int unit = static_cast<int>(blockIdx.x) / max(groups, 1);
+    const int r_first = static_cast<int>(blockIdx.x) % max(groups, 1) * ROWS;
+    if (p.join_pairs > 0) {
+      const int u = p.join_first + unit / 2, t = 2 * (p.join_pairs - 1 - u / (p.B * p.Hkv)) + unit % 2;
+      if (t >= p.tiles) return;
+      unit = u % (p.B * p.Hkv) * p.tiles + t;
+    }
     const int tile = unit % p.tiles, bh = unit / p.tiles, rows = min(p.tile_rows, p.R - tile * p.tile_rows);
     if (r_first >= rows) return;
     const int2 on = p.pieces[unit];
@@ -736,7 +742,7 @@ attn_q8_join_kernel(const __grid_constant__ Q8Params p, int merge_ctas, int key_
   const int id = static_cast<int>(blockIdx.x) - merge_ctas;
   const int bh = id / key_tiles, b = bh / p.Hkv, h = bh % p.Hkv;
   const int n = p.len(b);
-  const int key0 = (id % key_tiles) * kQ8JoinKeys, key = key0 + 4 * tid;
+  const int key0 = (id % key_tiles) * kQ8JoinKeys;
   if (key0 >= n) return;
   for (int r = warp; r < p.R; r += kQ8JoinWarps) {
     const int unit = bh * p.tiles + r / p.tile_rows;
@@ -745,27 +751,28 @@ attn_q8_join_kernel(const __grid_constant__ Q8Params p, int merge_ctas, int key_
     if (lane == 0) q8_join[r] = ml.x - kQ8PBias + log2f(ml.y);
   }
   __syncthreads();
-  if (key >= n) return;
   // causal: position j is seen by the queries i >= j - (n - M).  What a row kept of positions that it does not see is not
   // taken, whatever it is.
-  const int first = p.causal ? max(key - (n - p.M), 0) * p.G : 0;
-  const float* src = p.scores + static_cast<long long>(bh) * p.R * p.pitch + key;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  const bool edge = key + 3 > last_seen(p, n, first);
+  for (int key = key0 + 4 * tid; key < n && key < key0 + kQ8JoinKeys; key += 4 * kQ8JoinThreads) {
+    const int first = p.causal ? max(key - (n - p.M), 0) * p.G : 0;
+    const float* src = p.scores + static_cast<long long>(bh) * p.R * p.pitch + key;
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    const bool edge = key + 3 > last_seen(p, n, first);
 #pragma unroll 4
-  for (int r = first; r < p.R; ++r) {
-    const float4 x = *reinterpret_cast<const float4*>(src + r * p.pitch);
-    const float l = q8_join[r];
-    const int seen = edge ? last_seen(p, n, r) - key : 3;
-    acc[0] += ex2_approx(x.x - l);
-    if (seen >= 1) acc[1] += ex2_approx(x.y - l);
-    if (seen >= 2) acc[2] += ex2_approx(x.z - l);
-    if (seen >= 3) acc[3] += ex2_approx(x.w - l);
-  }
-  float* w = p.weight + b * p.w_sb + h * p.w_sh + key;
+    for (int r = first; r < p.R; ++r) {
+      const float4 x = *reinterpret_cast<const float4*>(src + r * p.pitch);
+      const float l = q8_join[r];
+      const int seen = edge ? last_seen(p, n, r) - key : 3;
+      acc[0] += ex2_approx(x.x - l);
+      if (seen >= 1) acc[1] += ex2_approx(x.y - l);
+      if (seen >= 2) acc[2] += ex2_approx(x.z - l);
+      if (seen >= 3) acc[3] += ex2_approx(x.w - l);
+    }
+    float* w = p.weight + b * p.w_sb + h * p.w_sh + key;
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (key + e < n) w[e] = p.weight_add ? w[e] + acc[e] : acc[e];
+    for (int e = 0; e < 4; ++e)
+      if (key + e < n) w[e] = p.weight_add ? w[e] + acc[e] : acc[e];
+  }
 }
 
 struct Q8Plan {
@@ -874,7 +881,8 @@ int launch_typed(const TrnAttnQ8Args& a, cudaStream_t st, const DeviceState& ds)
 template <typename T, int D>
 int launch_join(const Q8Params& p, const TrnAttnQ8Args& a, bool merge, cudaStream_t st) {
   constexpr int kMergeRows = kQ8JoinThreads / (D / 2);
-  const long long units = static_cast<long long>(a.B) * a.Hkv * p.tiles;
+  const long long bh = static_cast<long long>(a.B) * a.Hkv;
+  const long long units = p.join_pairs > 0 ? 2 * (bh * p.join_pairs - p.join_first) : bh * p.tiles;
   const long long merge_ctas = merge ? units * max(p.tile_rows / kMergeRows, 1) : 0;
   const int longest = a.kv_len != nullptr ? a.cache.S : min(max(a.kv_len_all, 0), a.cache.S);
   const int key_tiles = a.weight != nullptr ? (longest + kQ8JoinKeys - 1) / kQ8JoinKeys : 0;

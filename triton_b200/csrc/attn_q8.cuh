@@ -27,6 +27,8 @@ struct Q8Params {
   float* part_o;                               // [units + ctas][tile_rows][D], units = B * Hkv * tiles
   float2* part_ml;                             // [units + ctas][tile_rows]; without division [units][tile_rows] or NULL
   int2* pieces;                                // [units] CTAs of a unit's first and last piece
+  // join_pairs > 0: the merge visits only the pairs of row tiles from join_first on, in the order late pairs first
+  int join_pairs, join_first;
   float* scores;                               // [B * Hkv][R][pitch], log2 domain, or NULL
   long long pitch;
   float* weight;

@@ -32,12 +32,14 @@ static_assert(kTcConvert == 32 * kTcMmaWarp && kTcThreads == 32 * (kTcMmaWarp + 
 constexpr int kTcTmemCols = 512;              // S0 [0,128) S1 [128,256) O0 [256,256+D) O1 [384,384+D)
 constexpr float kTcRescale = 8.0f;            // log2 units a row's maximum may pass the offset in use
 constexpr float kTcPBias = 6.0f;              // P' <= 2^14 with it
+constexpr int kTcMaxRounds = 8, kTcMaxCut = 8;
 constexpr int kTcMinShare = 2;                // key blocks a CTA takes at least where they are divided
 
 struct TcParams {
   Q8Params c;
   int pairs;
   int ctas;          // CTAs the key blocks of all pairs of tiles are divided among; 0: a CTA per pair
+  int whole, cut;    // ctas == 0: the first `whole` pairs are not divided, the rest into `cut` pieces each
 };
 
 template <int D>
@@ -153,9 +155,15 @@ attn_q8_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   const int cta = static_cast<int>(blockIdx.x);
   int b, h, pair, split = 0, pieces = 1;
   if (tp.ctas == 0) {
-    pair = tp.pairs - 1 - cta / (p.B * p.Hkv);                     // late (heavy) pairs of tiles first
-    h = cta % p.Hkv;
-    b = cta / p.Hkv % p.B;
+    int u = cta;                                                   // late (heavy) pairs of tiles first
+    if (u >= tp.whole) {                                           // those of the last, incomplete round of CTAs: in pieces
+      pieces = tp.cut;
+      split = (cta - tp.whole) % tp.cut;
+      u = tp.whole + (cta - tp.whole) / tp.cut;
+    }
+    pair = tp.pairs - 1 - u / (p.B * p.Hkv);
+    h = u % p.Hkv;
+    b = u / p.Hkv % p.B;
   } else {
     // A pair's key blocks are cut into pieces of at most `share`: the least share with which all pairs' pieces find a CTA
     const int per = p.Hkv * tp.pairs;
@@ -578,9 +586,10 @@ attn_q8_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     }
     if (ok && !dead && warp_active) {
       const int tile = 2 * pair + t;
-      // a piece begins a new pair, a new CTA or both: pair + CTA numbers the pieces, tile 1's behind all of tile 0's
+      // Dealt out: a piece begins a new pair, a new CTA or both, so pair + CTA numbers the pieces.  Tile 1's behind tile 0's.
       const int all_pairs = p.B * p.Hkv * tp.pairs;
-      const long long slot = static_cast<long long>(t) * (all_pairs + tp.ctas) + bh * tp.pairs + pair + cta;
+      const long long slot = tp.ctas > 0 ? static_cast<long long>(t) * (all_pairs + tp.ctas) + bh * tp.pairs + pair + cta
+                                         : static_cast<long long>(t) * (all_pairs - tp.whole) * tp.cut + cta - tp.whole;
       const bool parts = pieces > 1, any_nan = *reinterpret_cast<volatile int*>(nan_any) != 0;
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
@@ -624,7 +633,7 @@ attn_q8_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         else if (p.lse != nullptr)
           p.lse[(static_cast<long long>(b) * p.Hq + h * p.G + r % p.G) * p.M + r / p.G] = m_run + log2f(l_run);
       }
-      if (p.pieces != nullptr && split == 0 && lrow == 0) {        // where the merge finds them: slot = unit + entry
+      if (p.pieces != nullptr && (tp.ctas > 0 || parts) && split == 0 && lrow == 0) {      // where the merge finds them: slot = unit + entry
         const int u = bh * p.tiles + tile, first = static_cast<int>(slot) - u;
         p.pieces[u] = make_int2(first, first + pieces - 1);
       }
@@ -646,7 +655,7 @@ attn_q8_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 }
 
 struct TcPlan {
-  int tiles, pairs, ctas;
+  int tiles, pairs, ctas, whole, cut;
   size_t ml_off, o_off, piece_off, total;
 };
 
@@ -659,9 +668,23 @@ TcPlan tc_plan(const TrnAttnQ8Args& a) {
   const long long pairs = static_cast<long long>(a.B) * a.Hkv * w.pairs;
   const int longest = a.kv_len != nullptr ? a.cache.S : min(max(a.kv_len_all, 1), a.cache.S);
   const int blocks = (longest - 1) / kTcKeys + 1;
-  if (2 * pairs > kAttnNominalSMs || blocks < 2 * kTcMinShare) return w;
-  w.ctas = static_cast<int>(min(static_cast<long long>(kAttnNominalSMs), pairs * ((blocks + kTcMinShare - 1) / kTcMinShare)));
-  const size_t rows = 2 * static_cast<size_t>(pairs + w.ctas) * kTcRows;
+  size_t rows;
+  if (2 * pairs <= kAttnNominalSMs && blocks >= 2 * kTcMinShare) {
+    w.ctas = static_cast<int>(min(static_cast<long long>(kAttnNominalSMs), pairs * ((blocks + kTcMinShare - 1) / kTcMinShare)));
+    rows = 2 * static_cast<size_t>(pairs + w.ctas) * kTcRows;
+  } else {
+    // Whole rounds of CTAs, and a last one that would leave most SMs idle: its pairs are cut into pieces that fill it (512
+    // pairs: 3 rounds and 68 pairs in two pieces each, instead of 4 rounds)
+    w.whole = static_cast<int>(min(pairs, 0x7fffffffLL));
+    w.cut = 1;
+    const long long rest = pairs % kAttnNominalSMs, rounds = pairs / kAttnNominalSMs;
+    if (rest == 0 || rounds == 0 || rounds > kTcMaxRounds) return w;
+    const int cut = static_cast<int>(min(min(kAttnNominalSMs / rest, static_cast<long long>(blocks / kTcMinShare)), static_cast<long long>(kTcMaxCut)));
+    if (cut < 2) return w;
+    w.cut = cut;
+    w.whole = static_cast<int>(pairs - rest);
+    rows = 2 * static_cast<size_t>(rest * cut) * kTcRows;
+  }
   w.ml_off = 0;
   w.o_off = up256(rows * sizeof(float2));
   w.piece_off = w.o_off + up256(rows * a.D * sizeof(float));
@@ -673,21 +696,33 @@ template <typename T, int D, int GRP>
 int launch_grp(const TrnAttnQ8Args& a, cudaStream_t st, const DeviceState& ds) {
   using SM = TcSmem<D>;
   TcPlan w = tc_plan(a);
-  if (a.workspace == nullptr) w.ctas = 0;
+  const long long pairs = static_cast<long long>(a.B) * a.Hkv * w.pairs;
+  if (pairs > 0x7fffffffLL || static_cast<long long>(a.B) * a.Hkv * w.tiles > 0x7fffffffLL) return TRN_E_SHAPE;
+  if (a.workspace == nullptr) {                          // nothing is divided
+    w.ctas = 0;
+    w.cut = 1;
+    w.whole = static_cast<int>(pairs);
+  }
   TcParams tp{};
   tp.c = q8_params(a, ds);
   tp.pairs = w.pairs;
   tp.ctas = w.ctas;
+  tp.whole = w.whole;
+  tp.cut = w.cut;
   tp.c.tiles = w.tiles;
   tp.c.tile_rows = kTcRows;
-  if (w.ctas > 0) {
+  const bool parts = w.ctas > 0 || w.cut > 1;
+  if (parts) {
     uint8_t* ws = static_cast<uint8_t*>(a.workspace);
     tp.c.part_ml = reinterpret_cast<float2*>(ws + w.ml_off);
     tp.c.part_o = reinterpret_cast<float*>(ws + w.o_off);
     tp.c.pieces = reinterpret_cast<int2*>(ws + w.piece_off);
   }
-  const long long grid = w.ctas > 0 ? w.ctas : static_cast<long long>(a.B) * a.Hkv * w.pairs;
-  if (grid > 0x7fffffffLL || static_cast<long long>(a.B) * a.Hkv * w.tiles > 0x7fffffffLL) return TRN_E_SHAPE;
+  const long long grid = w.ctas > 0 ? w.ctas : w.whole + (pairs - w.whole) * w.cut;
+  if (w.ctas == 0 && parts) {                            // the merge visits the pairs in pieces alone
+    tp.c.join_pairs = w.pairs;
+    tp.c.join_first = w.whole;
+  }
   CUtensorMap tm_k, tm_v;
   int rc = make_code_tmap(&tm_k, &tp.c.ki, a.cache.k, a.cache.S, a.Hkv, a.B, D, kTcKeys);
   if (rc == TRN_OK) rc = make_code_tmap(&tm_v, &tp.c.vi, a.cache.v, a.cache.S, a.Hkv, a.B, D, kTcKeys);
@@ -696,7 +731,7 @@ int launch_grp(const TrnAttnQ8Args& a, cudaStream_t st, const DeviceState& ds) {
   rc = ensure_dyn_smem(reinterpret_cast<const void*>(kern), SM::kTotal, ds.device);
   if (rc != TRN_OK) return rc;
   TRN_CUDA_TRY(launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(kTcThreads), SM::kTotal, st, tm_k, tm_v, tp));
-  return w.ctas > 0 ? launch_q8_join(tp.c, a, true, st) : TRN_OK;
+  return parts ? launch_q8_join(tp.c, a, true, st) : TRN_OK;
 }
 
 template <typename T, int D>

@@ -21,6 +21,7 @@ constexpr int kEvMaxN = 262144;
 constexpr int kEvThreads = 1024;
 constexpr int kEvAhead = 4;             // positions a thread sums side by side
 constexpr int kEvWarps = kEvThreads / 32;
+static_assert(kEvWarps == 32, "one lane for each warp's counts");
 constexpr int kEvMoveThreads = 256;
 constexpr int kEvGroup16 = 64;          // destination positions per CTA of a 16-bit move
 
@@ -212,14 +213,17 @@ evict_select_kernel(const __grid_constant__ EvictParams p, int cluster) {
   }
   if (lane == 0) { warp_gt[warp] = ngt; warp_eq[warp] = neq; }
   __syncthreads();
-  if (tid == 0) {
-    uint32_t a = 0u, e = 0u;
-    for (int i = 0; i < kEvWarps; ++i) {
-      const uint32_t x = warp_gt[i], y = warp_eq[i];
-      warp_gt[i] = a; warp_eq[i] = e;
-      a += x; e += y;
+  if (warp == 0) {                                             // kEvWarps == 32: one warp's counts a lane
+    const uint32_t x = warp_gt[lane], y = warp_eq[lane];
+    uint32_t a = x, e = y;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t u = __shfl_up_sync(0xffffffffu, a, o), v = __shfl_up_sync(0xffffffffu, e, o);
+      if (lane >= o) { a += u; e += v; }
     }
-    cta_cnt[0] = a; cta_cnt[1] = e;
+    warp_gt[lane] = a - x;
+    warp_eq[lane] = e - y;
+    if (lane == 31) { cta_cnt[0] = a; cta_cnt[1] = e; }
   }
   if (cluster > 1) cluster_sync_all(); else __syncthreads();
   uint32_t gt0 = warp_gt[warp], eq0 = warp_eq[warp];
@@ -273,48 +277,54 @@ evict_move_kernel(const __grid_constant__ MoveParams p) {
   const int g0 = grp * size, g1 = min(g0 + size, m);
   if (g0 >= g1) return;
   const int tid = static_cast<int>(threadIdx.x);
-  float top = 0.f;
+  float mine = 0.f;
   if (tid < g1 - g0) {
     const int j = p.idx[static_cast<long long>(row) * p.keep + g0 + tid];
     from[tid] = j;
-    if constexpr (Q8) {
-      top = *p.s_src[kv].at(b, j >> p.shift, h);
-      had[tid] = top;
-    }
+    if constexpr (Q8) mine = *p.s_src[kv].at(b, j >> p.shift, h);
   }
+  __syncthreads();
+  // the rows are asked for before the scales are looked at: one memory latency for both
+  constexpr int ITER = ((Q8 ? 128 : kEvGroup16) + ROWS - 1) / ROWS;
+  const TrnHeadTensor src = p.src[kv], dst = p.dst[kv];
+  const int seg = tid % SEG, r0 = tid / SEG;
+  const uint8_t* s0 = static_cast<const uint8_t*>(src.ptr) + (b * src.stride_b + h * src.stride_h) * ELEM + seg * 16;
+  uint8_t* d0 = static_cast<uint8_t*>(dst.ptr) + (b * dst.stride_b + h * dst.stride_h) * ELEM + seg * 16;
+  uint4 c[ITER];
+#pragma unroll
+  for (int i = 0; i < ITER; ++i)
+    if (r0 + i * ROWS < g1 - g0) c[i] = *reinterpret_cast<const uint4*>(s0 + from[r0 + i * ROWS] * (src.stride_s * ELEM));
+  float top = 0.f;
   if constexpr (Q8) {
+    if (tid < g1 - g0) had[tid] = mine;
+    top = mine;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if ((tid & 31) == 0) part[tid >> 5] = top;
-  }
-  __syncthreads();
-  if constexpr (Q8) {
+    __syncthreads();
     top = part[0];
 #pragma unroll
     for (int i = 1; i < kEvMoveThreads / 32; ++i) top = fmaxf(top, part[i]);
     if (tid == 0) *p.s_dst[kv].at(b, grp, h) = top;
   }
-  const TrnHeadTensor src = p.src[kv], dst = p.dst[kv];
-  const int seg = tid % SEG;
-  const uint8_t* s0 = static_cast<const uint8_t*>(src.ptr) + (b * src.stride_b + h * src.stride_h) * ELEM + seg * 16;
-  uint8_t* d0 = static_cast<uint8_t*>(dst.ptr) + (b * dst.stride_b + h * dst.stride_h) * ELEM + seg * 16;
-#pragma unroll 4
-  for (int r = tid / SEG; r < g1 - g0; r += ROWS) {
-    uint4 c = *reinterpret_cast<const uint4*>(s0 + from[r] * (src.stride_s * ELEM));
+#pragma unroll
+  for (int i = 0; i < ITER; ++i) {
+    const int r = r0 + i * ROWS;
+    if (r >= g1 - g0) continue;
     if constexpr (Q8) {
       const float s = had[r];
       if (s != top) {                                          // s < top (or NaN): the codes move to the larger scale
         const float ratio = s / top;
-        uint32_t w[4] = {c.x, c.y, c.z, c.w};
+        uint32_t w[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float2 a = e4m3x2_to_f32(w[e] & 0xffffu), g = e4m3x2_to_f32(w[e] >> 16);
           w[e] = f32_to_e4m3x2(a.x * ratio, a.y * ratio) | (f32_to_e4m3x2(g.x * ratio, g.y * ratio) << 16);
         }
-        c = make_uint4(w[0], w[1], w[2], w[3]);
+        c[i] = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
-    *reinterpret_cast<uint4*>(d0 + (g0 + r) * (dst.stride_s * ELEM)) = c;
+    *reinterpret_cast<uint4*>(d0 + (g0 + r) * (dst.stride_s * ELEM)) = c[i];
   }
 }
 

@@ -407,38 +407,48 @@ attn_q8_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     if (nb > 0) {
       constexpr int LPR = D / 8, RPI = 32 / LPR;                   // lanes per row, rows per iteration
       const int sub = lane / LPR, u = lane % LPR;
-#pragma unroll 4
-      for (int it = 0; it < 32 / RPI; ++it) {
-        const int lr = quad * 32 + it * RPI + sub, rr = (2 * pair + t) * kTcRows + lr;
-        uint4 x = make_uint4(0u, 0u, 0u, 0u);
-        if (rr < p.R)
-          x = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q.ptr) + b * p.q.stride_b + static_cast<long long>(rr / p.G) * p.q.stride_s +
-                                              static_cast<long long>(h * p.G + rr % p.G) * p.q.stride_h + u * 8);
-        // largest magnitude by its bits: 0x7f80 (bf16) / 0x7c00 (fp16) and up is not finite
-        uint32_t top = __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
-        top = max(top & 0xffffu, top >> 16);
+      constexpr int IT = 32 / RPI, AHEAD = 8;                      // rows of 8 iterations are under way together
+#pragma unroll 1
+      for (int it0 = 0; it0 < IT; it0 += AHEAD) {
+        uint4 rows[AHEAD];
 #pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        float up = 1.f, down = 1.f;
-        if constexpr (Io<T>::kFmt == 1) {
-          const int e = min(max(static_cast<int>(top >> 7) - 127, -100), 127);
-          up = exp2_int(14 - e);
-          down = exp2_int(e - 14);
+        for (int i = 0; i < AHEAD; ++i) {
+          const int rr = (2 * pair + t) * kTcRows + quad * 32 + (it0 + i) * RPI + sub;
+          rows[i] = make_uint4(0u, 0u, 0u, 0u);
+          if (rr < p.R)
+            rows[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q.ptr) + b * p.q.stride_b + static_cast<long long>(rr / p.G) * p.q.stride_s +
+                                                      static_cast<long long>(h * p.G + rr % p.G) * p.q.stride_h + u * 8);
         }
-        // a row with an infinite or NaN element: every score is infinite or NaN, and so is its softmax NaN
-        const float c = top >= (Io<T>::kFmt == 1 ? 0x7f80u : 0x7c00u) ? __uint_as_float(0x7fffffffu) : p.scale_log2 * down;
-        const float mine = __shfl_sync(0xffffffffu, c, (lane % RPI) * LPR);
-        if (lane / RPI == it) c_row = mine;
-        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-        uint32_t f[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 g = Io<T>::unpack2(w[e]);
-          f[e] = Io<__half>::pack2(g.x * up, g.y * up);
+        for (int i = 0; i < AHEAD; ++i) {
+          const int it = it0 + i, lr = quad * 32 + it * RPI + sub;
+          const uint4 x = rows[i];
+          // largest magnitude by its bits: 0x7f80 (bf16) / 0x7c00 (fp16) and up is not finite
+          uint32_t top = __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
+          top = max(top & 0xffffu, top >> 16);
+#pragma unroll
+          for (int o = LPR / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+          float up = 1.f, down = 1.f;
+          if constexpr (Io<T>::kFmt == 1) {
+            const int e = min(max(static_cast<int>(top >> 7) - 127, -100), 127);
+            up = exp2_int(14 - e);
+            down = exp2_int(e - 14);
+          }
+          // a row with an infinite or NaN element: every score is infinite or NaN, and so is its softmax NaN
+          const float c = top >= (Io<T>::kFmt == 1 ? 0x7f80u : 0x7c00u) ? __uint_as_float(0x7fffffffu) : p.scale_log2 * down;
+          const float mine = __shfl_sync(0xffffffffu, c, (lane % RPI) * LPR);
+          if (lane / RPI == it) c_row = mine;
+          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+          uint32_t f[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 g = Io<T>::unpack2(w[e]);
+            f[e] = Io<__half>::pack2(g.x * up, g.y * up);
+          }
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};"
+                       ::"r"(q_s(t) + (u >> 3) * SM::kChunkBytes + swz128(lr, u & 7)), "r"(f[0]), "r"(f[1]), "r"(f[2]), "r"(f[3])
+                       : "memory");
         }
-        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};"
-                     ::"r"(q_s(t) + (u >> 3) * SM::kChunkBytes + swz128(lr, u & 7)), "r"(f[0]), "r"(f[1]), "r"(f[2]), "r"(f[3])
-                     : "memory");
       }
       fence_proxy_async_smem();
       mbar_arrive(q_full(t));
@@ -605,27 +615,38 @@ attn_q8_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           for (int i = 0; i < 32; ++i)
             if (nan_from[c * 32 + i] <= limit) x[i] = 0x7fffffffu;
         }
-        if (!there) continue;
         if (parts) {
+          if (!there) continue;
           float* dst = p.part_o + (slot * kTcRows + lrow) * D + c * 32;
 #pragma unroll
           for (int i = 0; i < 32; i += 4)
             *reinterpret_cast<float4*>(dst + i) = make_float4(__uint_as_float(x[i]), __uint_as_float(x[i + 1]),
                                                               __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
         } else {
-          const int hq = h * p.G + r % p.G;
+          // rows meet in the q tile's place (its products are done), so that the warp can write whole lines
           const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;
-          T* dst = static_cast<T*>(p.o.ptr) + b * p.o.stride_b + static_cast<long long>(r / p.G) * p.o.stride_s +
-                   static_cast<long long>(hq) * p.o.stride_h + c * 32;
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            uint4 v;
-            v.x = Io<T>::pack2(__uint_as_float(x[i]) * inv, __uint_as_float(x[i + 1]) * inv);
-            v.y = Io<T>::pack2(__uint_as_float(x[i + 2]) * inv, __uint_as_float(x[i + 3]) * inv);
-            v.z = Io<T>::pack2(__uint_as_float(x[i + 4]) * inv, __uint_as_float(x[i + 5]) * inv);
-            v.w = Io<T>::pack2(__uint_as_float(x[i + 6]) * inv, __uint_as_float(x[i + 7]) * inv);
-            *reinterpret_cast<uint4*>(dst + i) = v;
-          }
+          for (int i = 0; i < 32; i += 8)
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};"
+                         ::"r"(q_s(t) + (c >> 1) * SM::kChunkBytes + swz128(lrow, (c & 1) * 4 + (i >> 3))),
+                           "r"(Io<T>::pack2(__uint_as_float(x[i]) * inv, __uint_as_float(x[i + 1]) * inv)),
+                           "r"(Io<T>::pack2(__uint_as_float(x[i + 2]) * inv, __uint_as_float(x[i + 3]) * inv)),
+                           "r"(Io<T>::pack2(__uint_as_float(x[i + 4]) * inv, __uint_as_float(x[i + 5]) * inv)),
+                           "r"(Io<T>::pack2(__uint_as_float(x[i + 6]) * inv, __uint_as_float(x[i + 7]) * inv))
+                         : "memory");
+        }
+      }
+      if (!parts) {
+        __syncwarp();
+        constexpr int LPR = D / 8, RPI = 32 / LPR;
+        const int sub = lane / LPR, u = lane % LPR;
+#pragma unroll 4
+        for (int it = 0; it < 32 / RPI; ++it) {
+          const int lr = quad * 32 + it * RPI + sub, rr = (2 * pair + t) * kTcRows + lr;
+          const uint4 v = lds128(q_s(t) + (u >> 3) * SM::kChunkBytes + swz128(lr, u & 7));
+          if (rr < p.R)
+            *reinterpret_cast<uint4*>(static_cast<T*>(p.o.ptr) + b * p.o.stride_b + static_cast<long long>(rr / p.G) * p.o.stride_s +
+                                      static_cast<long long>(h * p.G + rr % p.G) * p.o.stride_h + u * 8) = v;
         }
       }
       if (there) {

@@ -283,8 +283,8 @@ LONG = [
     (1, 300, 2, 1, 64, 9000, [8999], 32, HF, True),                     # tensor-core kernel, keys divided among CTAs
     (2, 9, 71, 1, 64, 5000, [4990, 5], 16, BF, True),
     # more pairs of row tiles than SMs: 192 and 320, whole rounds and a rest in pieces
-    (4, 257, 40, 8, 64, 1100, [1100, 300, 257, 1000], 64, BF, True),
-    (5, 130, 64, 32, 64, 700, [700, 699, 5, 0, 130], 16, HF, True),
+    (4, 257, 40, 8, 64, 5200, [5200, 300, 257, 5000], 64, BF, True),
+    (5, 130, 64, 32, 64, 700, [700, 699, 5, 0, 130], 16, HF, True),     # ... too short for pieces
 ]
 
 

@@ -33,6 +33,8 @@ constexpr int kTcTmemCols = 512;              // S0 [0,128) S1 [128,256) O0 [256
 constexpr float kTcRescale = 8.0f;            // log2 units a row's maximum may pass the offset in use
 constexpr float kTcPBias = 6.0f;              // P' <= 2^14 with it
 constexpr int kTcMaxRounds = 8, kTcMaxCut = 8;
+// 512 pairs without a mask: 16 key blocks 200 us whole, 213 with the last round in pieces; 32: 359, 357; 64: 677, 647
+constexpr int kTcMinCutBlocks = 40;
 constexpr int kTcMinShare = 2;                // key blocks a CTA takes at least where they are divided
 
 struct TcParams {
@@ -137,6 +139,10 @@ attn_q8_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     *abort_flag = 0;
     *nan_any = 0;
     fence_mbar_init();
+  }
+  if (threadIdx.x == 32) {
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
   }
   for (int i = threadIdx.x; i < D; i += kTcThreads) nan_from[i] = 0x7fffffff;
   if (warp == kTcMmaWarp) {
@@ -404,7 +410,7 @@ attn_q8_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     float c_row = 0.f;
     // ---- q rows -> fp16 times 2^(14 - exponent of a row's largest element), swizzled.  D / 8 lanes take a row, so that a
     // warp reads whole lines (a row per thread: 8 us more for each CTA); lane L ends up with row L's factor.
-    if (nb > 0) {
+    {                                          // whether or not a block follows: that takes the sequence's length to know
       constexpr int LPR = D / 8, RPI = 32 / LPR;                   // lanes per row, rows per iteration
       const int sub = lane / LPR, u = lane % LPR;
       constexpr int IT = 32 / RPI, AHEAD = 8;                      // rows of 8 iterations are under way together
@@ -699,7 +705,7 @@ TcPlan tc_plan(const TrnAttnQ8Args& a) {
     w.whole = static_cast<int>(min(pairs, 0x7fffffffLL));
     w.cut = 1;
     const long long rest = pairs % kAttnNominalSMs, rounds = pairs / kAttnNominalSMs;
-    if (rest == 0 || rounds == 0 || rounds > kTcMaxRounds) return w;
+    if (rest == 0 || rounds == 0 || rounds > kTcMaxRounds || blocks < kTcMinCutBlocks) return w;
     const int cut = static_cast<int>(min(min(kAttnNominalSMs / rest, static_cast<long long>(blocks / kTcMinShare)), static_cast<long long>(kTcMaxCut)));
     if (cut < 2) return w;
     w.cut = cut;

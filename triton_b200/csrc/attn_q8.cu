@@ -667,8 +667,8 @@ attn_q8_cluster_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
   if (cluster > 1) cluster_sync_all();                             // no CTA leaves while its results may be read
 }
 
-// Merge of the pieces, and weights of the positions.  CTAs [0, merge_ctas): kQ8JoinThreads / (D / 2) rows of a unit each, two
-// columns a thread; the rest: four positions a thread of a (b, kv head), rows in ascending order.
+// Merge of the pieces, and weights of the positions.  CTAs [0, merge_ctas): join_rows rows of a unit each; the rest: positions
+// of a (b, kv head), four at a time a thread, rows in ascending order.
 constexpr int kQ8JoinThreads = 256;
 constexpr int kQ8JoinWarps = kQ8JoinThreads / 32;
 constexpr int kQ8JoinKeys = 8 * kQ8JoinThreads;
@@ -695,16 +695,16 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kQ8JoinThreads)
 attn_q8_join_kernel(const __grid_constant__ Q8Params p, int merge_ctas, int key_tiles) {
   extern __shared__ float q8_join[];           // weight CTAs: [R] log-sum-exps
-  constexpr int ROWS = kQ8JoinThreads / (D / 2);
-  __shared__ float2 all[ROWS];
+  constexpr int GROUPS = kQ8JoinThreads / (D / 2);
+  __shared__ float2 all[GROUPS], part[GROUPS][D / 2];
   griddep_wait();
   griddep_launch();
   if (*reinterpret_cast<volatile int*>(p.status) != 0) return;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (static_cast<int>(blockIdx.x) < merge_ctas) {
-    const int groups = p.tile_rows / ROWS;     // tile_rows and ROWS are powers of two; at least one
-    int unit = static_cast<int>(blockIdx.x) / max(groups, 1);
-    const int r_first = static_cast<int>(blockIdx.x) % max(groups, 1) * ROWS;
+    const int per_unit = p.tile_rows / p.join_rows;
+    int unit = static_cast<int>(blockIdx.x) / per_unit;
+    const int r_first = static_cast<int>(blockIdx.x) % per_unit * p.join_rows;
     if (p.join_pairs > 0) {
       const int u = p.join_first + unit / 2, t = 2 * (p.join_pairs - 1 - u / (p.B * p.Hkv)) + unit % 2;
       if (t >= p.tiles) return;
@@ -716,27 +716,41 @@ attn_q8_join_kernel(const __grid_constant__ Q8Params p, int merge_ctas, int key_
     const int here = on.y - on.x + 1;
     if (here == 1) return;                     // written by the one piece itself
     const long long at = static_cast<long long>(unit + on.x) * p.tile_rows + r_first;
-    if (warp < ROWS && r_first + warp < rows) {
+    if (warp < p.join_rows && r_first + warp < rows) {
       const float2 ml = join_ml(p, at + warp, here, lane);
       if (lane == 0) all[warp] = ml;
     }
     __syncthreads();
-    const int r = tid / (D / 2), d = (tid % (D / 2)) * 2;
-    if (r_first + r >= rows) return;
+    // a group of D / 2 threads, two columns each, has a row of its own, or all groups share one row's pieces
+    const bool share = p.join_rows == 1;
+    const int g = tid / (D / 2), d = (tid % (D / 2)) * 2, r = share ? 0 : g, step = share ? GROUPS : 1;
+    const bool there = r_first + r < rows;
     const float2 ml = all[r];
     float acc[2] = {0.f, 0.f};
-#pragma unroll 4
-    for (int s = 0; s < here; ++s) {
-      const long long row = at + r + static_cast<long long>(s) * p.tile_rows;
-      const float2 x = p.part_ml[row];
-      const float2 v = *reinterpret_cast<const float2*>(p.part_o + row * D + d);
-      const float w = x.y == 0.f ? 0.f : ex2_approx(x.x - ml.x);
-      if (x.y != 0.f) {                        // a piece that saw nothing has written zeros or, where v has NaN, nothing to weigh
-        acc[0] = fmaf(w, v.x, acc[0]);
-        acc[1] = fmaf(w, v.y, acc[1]);
+    if (there) {
+#pragma unroll 8
+      for (int s = share ? g : 0; s < here; s += step) {
+        const long long row = at + r + static_cast<long long>(s) * p.tile_rows;
+        const float2 x = p.part_ml[row];
+        const float2 v = *reinterpret_cast<const float2*>(p.part_o + row * D + d);
+        const float w = x.y == 0.f ? 0.f : ex2_approx(x.x - ml.x);
+        if (x.y != 0.f) {                      // a piece that saw nothing has nothing to weigh
+          acc[0] = fmaf(w, v.x, acc[0]);
+          acc[1] = fmaf(w, v.y, acc[1]);
+        }
       }
     }
-    q8_store_row<T, 2>(p, bh / p.Hkv, bh % p.Hkv, tile * p.tile_rows + r_first + r, d, acc, ml.x, ml.y);
+    if (share) {
+      part[g][tid % (D / 2)] = make_float2(acc[0], acc[1]);
+      __syncthreads();
+      if (g != 0) return;
+#pragma unroll
+      for (int i = 1; i < GROUPS; ++i) {
+        acc[0] += part[i][tid].x;
+        acc[1] += part[i][tid].y;
+      }
+    }
+    if (there) q8_store_row<T, 2>(p, bh / p.Hkv, bh % p.Hkv, tile * p.tile_rows + r_first + r, d, acc, ml.x, ml.y);
     return;
   }
   const int id = static_cast<int>(blockIdx.x) - merge_ctas;
@@ -880,17 +894,19 @@ int launch_typed(const TrnAttnQ8Args& a, cudaStream_t st, const DeviceState& ds)
 
 template <typename T, int D>
 int launch_join(const Q8Params& p, const TrnAttnQ8Args& a, bool merge, cudaStream_t st) {
-  constexpr int kMergeRows = kQ8JoinThreads / (D / 2);
   const long long bh = static_cast<long long>(a.B) * a.Hkv;
   const long long units = p.join_pairs > 0 ? 2 * (bh * p.join_pairs - p.join_first) : bh * p.tiles;
-  const long long merge_ctas = merge ? units * max(p.tile_rows / kMergeRows, 1) : 0;
+  // Few units lie on many CTAs each: then a CTA merges one row, its threads sharing the pieces
+  Q8Params jp = p;
+  jp.join_rows = p.ctas >= 4 * bh * p.tiles ? 1 : kQ8JoinThreads / (D / 2);
+  const long long merge_ctas = merge ? units * (p.tile_rows / jp.join_rows) : 0;
   const int longest = a.kv_len != nullptr ? a.cache.S : min(max(a.kv_len_all, 0), a.cache.S);
   const int key_tiles = a.weight != nullptr ? (longest + kQ8JoinKeys - 1) / kQ8JoinKeys : 0;
   const long long grid = merge_ctas + static_cast<long long>(a.B) * a.Hkv * key_tiles;
   if (grid > 0x7fffffffLL) return TRN_E_SHAPE;
   if (grid > 0)
     TRN_CUDA_TRY(launch_pdl(attn_q8_join_kernel<T, D>, dim3(static_cast<unsigned>(grid)), dim3(kQ8JoinThreads),
-                            a.weight != nullptr ? p.R * sizeof(float) : 0, st, p, static_cast<int>(merge_ctas), max(key_tiles, 1)));
+                            a.weight != nullptr ? p.R * sizeof(float) : 0, st, jp, static_cast<int>(merge_ctas), max(key_tiles, 1)));
   return TRN_OK;
 }
 

@@ -29,6 +29,7 @@ struct Q8Params {
   int2* pieces;                                // [units] CTAs of a unit's first and last piece
   // join_pairs > 0: the merge visits only the pairs of row tiles from join_first on, in the order late pairs first
   int join_pairs, join_first;
+  int join_rows;                               // rows a CTA of the merge takes: 1, or as many as its threads are for
   float* scores;                               // [B * Hkv][R][pitch], log2 domain, or NULL
   long long pitch;
   float* weight;

@@ -37,20 +37,27 @@ namespace {
 constexpr int kQ8Warps = 4;
 constexpr int kQ8Threads = 32 * kQ8Warps;
 constexpr int kQ8Keys = 32;                    // positions per chunk
-constexpr int kQ8Stages = 2;
 constexpr float kQ8Slack = 3.f;                // log2 of how far a score may pass the running maximum (2^15 fits fp16)
 constexpr int kQ8MaxCluster = 8;
 constexpr int kQ8Keep = 4;                     // chunks a warp of a cluster takes at most
-constexpr int kQ8TargetCtas = 3;               // resident CTAs per SM (shared memory)
+// Stages of a warp's ring, and how many CTAs an SM then has room for.  Three CTAs of two stages where units are many (a CTA
+// ends one and begins others, while the rest of the SM keeps loading); two CTAs of three stages where a unit lies on
+// two CTAs and more.  Measured at head_dim 128 (us, bf16): 256 units of 1000..8192 positions 66.0 against 71.2; 16 units of
+// 100001..131071 92.1 against 85.1; 128 units of 16384 100.2 against 94.1.  Head_dim 64 keeps the first (26.9 against 31.9).
+// Two CTAs also where a lane's 200 and more registers leave no room for a third: 16 rows of head_dim 128, 32 of 64.
+int q8_stages(int D, int tile_rows, long long units, int sm_count) {
+  return D == 128 && (tile_rows == 16 || units <= sm_count) ? 3 : 2;
+}
+int q8_ctas(int D, int tile_rows, int stages) { return stages == 3 || (D == 64 && tile_rows == 32) ? 2 : 3; }
 
 // rows a CTA takes: 8, 16 or (head_dim 64, where the output leaves registers for it) 32
 __host__ __device__ constexpr int q8_max_tiles(int D) { return D == 64 ? 4 : 2; }
 
-template <int D, int NT>
+template <int D, int NT, int ST>
 struct Q8Smem {
   static constexpr int kRows = 8 * NT;
   static constexpr int kTile = kQ8Keys * D;                        // bytes of k or v of a chunk
-  static constexpr int kWarpRing = kQ8Stages * 2 * kTile;
+  static constexpr int kWarpRing = ST * 2 * kTile;
   static constexpr int kRing = kQ8Warps * kWarpRing;
   static constexpr int kRow = D + 4;                               // o | max, sum  of a warp's partial result
   static constexpr int kPart = kQ8Warps * kRows * kRow * 4;        // overlays the ring after the key loop
@@ -146,18 +153,18 @@ __device__ __forceinline__ Q8Piece piece_of(const Q8Params& p, int b, int h, int
 // with its row's running maximum, sum and CW columns of the unnormalised output.  HILO: P' enters the product as two
 // fp16 parts.  All threads of the CTA; the rings are empty and shared memory is free for the next piece's tiles after a
 // proxy fence and a barrier.
-template <typename T, int D, int NT, bool HILO>
+template <typename T, int D, int NT, bool HILO, int ST>
 __device__ __forceinline__ void q8_piece(const Q8Params& p, const CUtensorMap& tm_k, const CUtensorMap& tm_v, const Q8Piece& w,
                                          uint8_t* gen, uint32_t base, int* nan_from, const Ctl& ctl,
-                                         float (&acc)[Q8Smem<D, NT>::kCW], float& mx, float& tot) {
-  using SM = Q8Smem<D, NT>;
+                                         float (&acc)[Q8Smem<D, NT, ST>::kCW], float& mx, float& tot) {
+  using SM = Q8Smem<D, NT, ST>;
   constexpr int ROWS = SM::kRows, CW = SM::kCW;
   constexpr int KS = D / 16;                   // k steps of k q^T
   constexpr int DT = D / 16;                   // 16-row blocks of o^T
   constexpr int KU = D / 64;                   // 16-byte units a lane reads per key row
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  const uint32_t bars = base + SM::kBars + warp * kQ8Stages * 8;
+  const uint32_t bars = base + SM::kBars + warp * ST * 8;
   int lim[NT][2];                              // last position seen of this lane's columns: rows 8 nt + 2t, + 1
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
@@ -166,13 +173,13 @@ __device__ __forceinline__ void q8_piece(const Q8Params& p, const CUtensorMap& t
   const uint32_t ring = base + warp * SM::kWarpRing;
   auto k_tile = [&](int s) { return ring + s * 2 * SM::kTile; };
   auto load = [&](int c) {                                         // lane 0
-    const int s = (w.loaded + c) % kQ8Stages, key0 = (w.chunk0 + c) * kQ8Keys;
+    const int s = (w.loaded + c) % ST, key0 = (w.chunk0 + c) * kQ8Keys;
     mbar_expect_tx(bars + 8 * s, 2 * SM::kTile);
     tma_load_head_tile(k_tile(s), &tm_k, bars + 8 * s, p.ki, 0, key0, w.h, w.b);
     tma_load_head_tile(k_tile(s) + SM::kTile, &tm_v, bars + 8 * s, p.vi, 0, key0, w.h, w.b);
   };
   if (lane == 0)
-    for (int c = 0; c < min(kQ8Stages, w.n_chunks); ++c) load(c);
+    for (int c = 0; c < min(ST, w.n_chunks); ++c) load(c);
   // scales of a chunk: two halves of 16 positions (the same block unless block is 16)
   auto scales_of = [&](int c, float (&ks)[2], float (&vs)[2]) {
 #pragma unroll
@@ -253,14 +260,14 @@ __device__ __forceinline__ void q8_piece(const Q8Params& p, const CUtensorMap& t
   bool ok = true;
 
   for (int c = 0; c < w.n_chunks; ++c) {
-    const int s = (w.loaded + c) % kQ8Stages, key0 = (w.chunk0 + c) * kQ8Keys;
+    const int s = (w.loaded + c) % ST, key0 = (w.chunk0 + c) * kQ8Keys;
     float lv[2], inv[2];
     const float ks[2] = {ks_next[0], ks_next[1]};
 #pragma unroll
     for (int i = 0; i < 2; ++i) scale_log_inv(vs_next[i] < kMinVScale ? kMinVScale : vs_next[i], lv[i], inv[i]);
     scales_of(c + 1, ks_next, vs_next);
     const bool edge = key0 + kQ8Keys - 1 > w.lim_min;                // some row does not see some position of the chunk
-    ok = mbar_wait(bars + 8 * s, ((w.loaded + c) / kQ8Stages) & 1, ctl, KST_TIMEOUT_CONSUMER);
+    ok = mbar_wait(bars + 8 * s, ((w.loaded + c) / ST) & 1, ctl, KST_TIMEOUT_CONSUMER);
     ok = __all_sync(0xffffffffu, ok);
     if (!ok) break;
     // ---- s^T of two blocks of 16 positions; rows g, g + 8 of a block are its positions q8_key(g), 8 + q8_key(g)
@@ -404,7 +411,7 @@ __device__ __forceinline__ void q8_piece(const Q8Params& p, const CUtensorMap& t
       }
     }
     __syncwarp();                              // every lane has read stage s
-    if (lane == 0 && c + kQ8Stages < w.n_chunks) load(c + kQ8Stages);
+    if (lane == 0 && c + ST < w.n_chunks) load(c + ST);
   }
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
@@ -455,11 +462,11 @@ __device__ __forceinline__ void q8_piece(const Q8Params& p, const CUtensorMap& t
 }
 
 // barriers and the table of NaN columns; then the wait for the launch before this one.  Returns whether an earlier kernel gave up.
-template <int D, int NT>
+template <int D, int NT, int ST>
 __device__ __forceinline__ bool q8_begin(const Q8Params& p, const CUtensorMap& tm_k, const CUtensorMap& tm_v, uint32_t base,
                                          int* nan_from, int* s_abort) {
   if ((threadIdx.x & 31) == 0) {
-    for (int s = 0; s < kQ8Stages; ++s) mbar_init(base + Q8Smem<D, NT>::kBars + ((threadIdx.x >> 5) * kQ8Stages + s) * 8, 1);
+    for (int s = 0; s < ST; ++s) mbar_init(base + Q8Smem<D, NT, ST>::kBars + ((threadIdx.x >> 5) * ST + s) * 8, 1);
     fence_mbar_init();
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
@@ -473,11 +480,11 @@ __device__ __forceinline__ bool q8_begin(const Q8Params& p, const CUtensorMap& t
 }
 
 // Long caches: each CTA takes its share of all chunks, a piece of a unit after the other.
-template <typename T, int D, int NT, bool HILO>
+template <typename T, int D, int NT, bool HILO, int ST>
 __global__ void __launch_bounds__(kQ8Threads)
 attn_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                const __grid_constant__ Q8Params p) {
-  using SM = Q8Smem<D, NT>;
+  using SM = Q8Smem<D, NT, ST>;
   constexpr int ROWS = SM::kRows, CW = SM::kCW;
   extern __shared__ uint8_t q8_smem_raw[];
   __shared__ int nan_from[D];                  // first position whose v code of this column is NaN, in edge chunks
@@ -486,7 +493,7 @@ attn_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
   uint8_t* gen = q8_smem_raw + (base - smem_u32(q8_smem_raw));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Ctl ctl{p.status, &s_abort};
-  if (q8_begin<D, NT>(p, tm_k, tm_v, base, nan_from, &s_abort)) return;
+  if (q8_begin<D, NT, ST>(p, tm_k, tm_v, base, nan_from, &s_abort)) return;
 
   // ---- this CTA's share: chunks [at, end) of all, beginning `skip` chunks into unit (b, h, tile)
   const int cta = static_cast<int>(blockIdx.x);
@@ -539,7 +546,7 @@ attn_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
       w.kept_pitch = p.pitch;
     }
     float acc[CW], mx, tot;
-    q8_piece<T, D, NT, HILO>(p, tm_k, tm_v, w, gen, base, nan_from, ctl, acc, mx, tot);
+    q8_piece<T, D, NT, HILO, ST>(p, tm_k, tm_v, w, gen, base, nan_from, ctl, acc, mx, tot);
     if (s_abort) return;
     const int row = threadIdx.x / SM::kTPR, c0 = (threadIdx.x % SM::kTPR) * CW;
     if (row < w.rows) {
@@ -578,11 +585,11 @@ attn_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
 
 // Short caches (at most kQ8Keep chunks a warp): a cluster of CTAs per unit, which meet in shared memory, so that one launch
 // does everything, the weights too: each warp keeps its scores on chip until the rows' log-sum-exps are known.
-template <typename T, int D, int NT, bool HILO>
+template <typename T, int D, int NT, bool HILO, int ST>
 __global__ void __launch_bounds__(kQ8Threads)
 attn_q8_cluster_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                        const __grid_constant__ Q8Params p, int cluster) {
-  using SM = Q8Smem<D, NT>;
+  using SM = Q8Smem<D, NT, ST>;
   constexpr int ROWS = SM::kRows, CW = SM::kCW;
   extern __shared__ uint8_t q8_smem_raw[];
   __shared__ int nan_from[D];
@@ -593,7 +600,7 @@ attn_q8_cluster_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Ctl ctl{p.status, &s_abort};
   // no CTA leaves before the cluster's last barrier; one that must not work writes nothing
-  const bool dead = q8_begin<D, NT>(p, tm_k, tm_v, base, nan_from, &s_abort);
+  const bool dead = q8_begin<D, NT, ST>(p, tm_k, tm_v, base, nan_from, &s_abort);
   const int rank = static_cast<int>(cluster_ctarank()), unit = static_cast<int>(blockIdx.x) / cluster;
   const int tile = unit % p.tiles, h = unit / p.tiles % p.Hkv, b = unit / p.tiles / p.Hkv;
   const int total = chunks_of(p.len(b)), skip = total * rank / cluster;
@@ -605,7 +612,7 @@ attn_q8_cluster_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
     w.kept_from = w.chunk0 * kQ8Keys;
   }
   float acc[CW], mx, tot;
-  q8_piece<T, D, NT, HILO>(p, tm_k, tm_v, w, gen, base, nan_from, ctl, acc, mx, tot);
+  q8_piece<T, D, NT, HILO, ST>(p, tm_k, tm_v, w, gen, base, nan_from, ctl, acc, mx, tot);
   const bool write = !dead && s_abort == 0;
   float* mine = reinterpret_cast<float*>(gen + SM::kMine);         // [ROWS][kRow], behind the warps' results
   {
@@ -790,7 +797,7 @@ attn_q8_join_kernel(const __grid_constant__ Q8Params p, int merge_ctas, int key_
 }
 
 struct Q8Plan {
-  int tiles, tile_rows, ctas, cluster;         // cluster > 0: one launch of clusters, no scratch
+  int tiles, tile_rows, stages, ctas, cluster;         // cluster > 0: one launch of clusters, no scratch
   long long units;
   size_t ml_off, o_off, piece_off, score_off, total;
   long long pitch;
@@ -808,9 +815,10 @@ Q8Plan plan_of(const TrnAttnQ8Args& a, int sm_count, bool divide) {
   w.units = static_cast<long long>(a.B) * a.Hkv * w.tiles;
   const int longest = a.kv_len != nullptr ? a.cache.S : min(max(a.kv_len_all, 1), a.cache.S);
   const int unit_chunks = (longest - 1) / kQ8Keys + 1;
-  const long long round = static_cast<long long>(sm_count) * kQ8TargetCtas;
+  w.stages = q8_stages(a.D, w.tile_rows, w.units, sm_count);
+  const long long round = static_cast<long long>(sm_count) * q8_ctas(a.D, w.tile_rows, w.stages);
   int cluster = 1;
-  while (cluster < kQ8MaxCluster && 2 * cluster * w.units <= round && 2 * cluster * kQ8Warps <= unit_chunks + kQ8Warps - 1) cluster *= 2;
+  while (cluster < kQ8MaxCluster && 2 * cluster * w.units <= 3LL * sm_count && 2 * cluster * kQ8Warps <= unit_chunks + kQ8Warps - 1) cluster *= 2;
   if (unit_chunks <= kQ8Keep * kQ8Warps * cluster && (a.weight == nullptr || w.tiles == 1)) {
     w.cluster = cluster;
     return w;
@@ -834,8 +842,33 @@ Q8Plan plan_of(const TrnAttnQ8Args& a, int sm_count, bool divide) {
 }
 
 template <typename T, int D, int NT>
+int launch_cluster(const TrnAttnQ8Args& a, const Q8Plan& w, const CUtensorMap& tm_k, const CUtensorMap& tm_v, const Q8Params& p,
+                   cudaStream_t st, const DeviceState& ds) {
+  using SM = Q8Smem<D, NT, 2>;
+  auto kern = attn_q8_cluster_kernel<T, D, NT, Io<T>::kFmt == 0, 2>;
+  const int rc = ensure_dyn_smem(reinterpret_cast<const void*>(kern), SM::kTotalKept, ds.device);
+  if (rc != TRN_OK) return rc;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(w.units * w.cluster), 1, 1);
+  cfg.blockDim = dim3(kQ8Threads, 1, 1);
+  cfg.dynamicSmemBytes = a.weight != nullptr ? SM::kTotalKept : SM::kTotal;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(w.cluster);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  TRN_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tm_k, tm_v, p, w.cluster));
+  return TRN_OK;
+}
+
+template <typename T, int D, int NT, int ST>
 int launch_tiles(const TrnAttnQ8Args& a, const Q8Plan& w, cudaStream_t st, const DeviceState& ds) {
-  using SM = Q8Smem<D, NT>;
+  using SM = Q8Smem<D, NT, ST>;
   constexpr bool HILO = Io<T>::kFmt == 0;
   Q8Params p = q8_params(a, ds);
   CUtensorMap tm_k, tm_v;
@@ -852,28 +885,8 @@ int launch_tiles(const TrnAttnQ8Args& a, const Q8Plan& w, cudaStream_t st, const
   }
   p.pitch = w.pitch;
   if (w.units * max(w.cluster, 1) + w.ctas > 0x7fffffffLL) return TRN_E_SHAPE;
-  if (w.cluster > 0) {
-    auto kern = attn_q8_cluster_kernel<T, D, NT, HILO>;
-    rc = ensure_dyn_smem(reinterpret_cast<const void*>(kern), SM::kTotalKept, ds.device);
-    if (rc != TRN_OK) return rc;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(w.units * w.cluster), 1, 1);
-    cfg.blockDim = dim3(kQ8Threads, 1, 1);
-    cfg.dynamicSmemBytes = a.weight != nullptr ? SM::kTotalKept : SM::kTotal;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = static_cast<unsigned>(w.cluster);
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = pdl_enabled() ? 2 : 1;
-    TRN_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tm_k, tm_v, p, w.cluster));
-    return TRN_OK;
-  }
-  auto kern = attn_q8_kernel<T, D, NT, HILO>;
+  if (w.cluster > 0) return launch_cluster<T, D, NT>(a, w, tm_k, tm_v, p, st, ds);
+  auto kern = attn_q8_kernel<T, D, NT, HILO, ST>;
   rc = ensure_dyn_smem(reinterpret_cast<const void*>(kern), SM::kTotal, ds.device);
   if (rc != TRN_OK) return rc;
   const unsigned grid = static_cast<unsigned>(w.ctas > 0 ? w.ctas : w.units);
@@ -885,11 +898,14 @@ int launch_tiles(const TrnAttnQ8Args& a, const Q8Plan& w, cudaStream_t st, const
 template <typename T, int D>
 int launch_typed(const TrnAttnQ8Args& a, cudaStream_t st, const DeviceState& ds) {
   const Q8Plan w = plan_of(a, kAttnNominalSMs, a.workspace != nullptr);
-  if (w.tile_rows == 8) return launch_tiles<T, D, 1>(a, w, st, ds);
-  if constexpr (q8_max_tiles(D) >= 4) {
-    if (w.tile_rows == 32) return launch_tiles<T, D, 4>(a, w, st, ds);
+  if constexpr (D == 128) {
+    if (w.tile_rows == 16) return launch_tiles<T, D, 2, 3>(a, w, st, ds);
+    return w.stages == 3 ? launch_tiles<T, D, 1, 3>(a, w, st, ds) : launch_tiles<T, D, 1, 2>(a, w, st, ds);
+  } else {
+    if (w.tile_rows == 8) return launch_tiles<T, D, 1, 2>(a, w, st, ds);
+    if (w.tile_rows == 16) return launch_tiles<T, D, 2, 2>(a, w, st, ds);
+    return launch_tiles<T, D, 4, 2>(a, w, st, ds);
   }
-  return launch_tiles<T, D, 2>(a, w, st, ds);
 }
 
 template <typename T, int D>

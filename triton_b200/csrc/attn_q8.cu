@@ -678,7 +678,9 @@ attn_q8_cluster_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
 // of a (b, kv head), four at a time a thread, rows in ascending order.
 constexpr int kQ8JoinThreads = 256;
 constexpr int kQ8JoinWarps = kQ8JoinThreads / 32;
-constexpr int kQ8JoinKeys = 8 * kQ8JoinThreads;
+// Positions of a weight CTA: with few rows per kv head its threads are for positions, with many they share the rows (a
+// thread for all 568 rows of 71 heads and 8 queries: 223 us for a call that takes 53 this way)
+constexpr int kQ8FewRows = 16, kQ8JoinKeys = 8 * kQ8JoinThreads, kQ8JoinKeysRows = 128;
 // maximum and sum of a row over its pieces by one warp; at: the row in the first piece's slot
 __device__ __forceinline__ float2 join_ml(const Q8Params& p, long long at, int here, int lane) {
   float2 mine = make_float2(-INFINITY, 0.f);   // a lane's pieces lane, lane + 32, ...
@@ -763,24 +765,47 @@ attn_q8_join_kernel(const __grid_constant__ Q8Params p, int merge_ctas, int key_
   const int id = static_cast<int>(blockIdx.x) - merge_ctas;
   const int bh = id / key_tiles, b = bh / p.Hkv, h = bh % p.Hkv;
   const int n = p.len(b);
-  const int key0 = (id % key_tiles) * kQ8JoinKeys;
+  const int keys = p.R <= kQ8FewRows ? kQ8JoinKeys : kQ8JoinKeysRows, key0 = (id % key_tiles) * keys;
   if (key0 >= n) return;
-  for (int r = warp; r < p.R; r += kQ8JoinWarps) {
+  auto ml_at = [&](int r, int& here) {
     const int unit = bh * p.tiles + r / p.tile_rows;
     const int2 on = p.pieces[unit];
-    const float2 ml = join_ml(p, static_cast<long long>(unit + on.x) * p.tile_rows + r % p.tile_rows, on.y - on.x + 1, lane);
-    if (lane == 0) q8_join[r] = ml.x - kQ8PBias + log2f(ml.y);
+    here = on.y - on.x + 1;
+    return static_cast<long long>(unit + on.x) * p.tile_rows + r % p.tile_rows;
+  };
+  if (p.R <= kQ8FewRows) {                     // a warp for each row: its pieces side by side
+    for (int r = warp; r < p.R; r += kQ8JoinWarps) {
+      int here;
+      const long long at = ml_at(r, here);
+      const float2 ml = join_ml(p, at, here, lane);
+      if (lane == 0) q8_join[r] = ml.x - kQ8PBias + log2f(ml.y);
+    }
+  } else {                                     // a thread for each row: rows side by side
+    for (int r = tid; r < p.R; r += kQ8JoinThreads) {
+      int here;
+      const long long at = ml_at(r, here);
+      float m = -INFINITY, l = 0.f;
+#pragma unroll 4
+      for (int s = 0; s < here; ++s) {
+        const float2 ml = p.part_ml[at + static_cast<long long>(s) * p.tile_rows];
+        const float mn = fmaxf(m, ml.x);
+        if (ml.y != 0.f) {
+          l = (l == 0.f ? 0.f : l * ex2_approx(m - mn)) + ml.y * ex2_approx(ml.x - mn);
+          m = mn;
+        }
+      }
+      q8_join[r] = m - kQ8PBias + log2f(l);
+    }
   }
   __syncthreads();
   // causal: position j is seen by the queries i >= j - (n - M).  What a row kept of positions that it does not see is not
   // taken, whatever it is.
-  for (int key = key0 + 4 * tid; key < n && key < key0 + kQ8JoinKeys; key += 4 * kQ8JoinThreads) {
+  auto sum_rows = [&](int key, int r0, int step, float (&acc)[4]) {
     const int first = p.causal ? max(key - (n - p.M), 0) * p.G : 0;
     const float* src = p.scores + static_cast<long long>(bh) * p.R * p.pitch + key;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
     const bool edge = key + 3 > last_seen(p, n, first);
-#pragma unroll 4
-    for (int r = first; r < p.R; ++r) {
+#pragma unroll 8
+    for (int r = first + r0; r < p.R; r += step) {
       const float4 x = *reinterpret_cast<const float4*>(src + r * p.pitch);
       const float l = q8_join[r];
       const int seen = edge ? last_seen(p, n, r) - key : 3;
@@ -789,11 +814,35 @@ attn_q8_join_kernel(const __grid_constant__ Q8Params p, int merge_ctas, int key_
       if (seen >= 2) acc[2] += ex2_approx(x.z - l);
       if (seen >= 3) acc[3] += ex2_approx(x.w - l);
     }
+  };
+  auto put = [&](int key, const float (&acc)[4]) {
     float* w = p.weight + b * p.w_sb + h * p.w_sh + key;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (key + e < n) w[e] = p.weight_add ? w[e] + acc[e] : acc[e];
+  };
+  if (p.R <= kQ8FewRows) {
+    for (int key = key0 + 4 * tid; key < n && key < key0 + keys; key += 4 * kQ8JoinThreads) {
+      float acc[4] = {0.f, 0.f, 0.f, 0.f};
+      sum_rows(key, 0, 1, acc);
+      put(key, acc);
+    }
+    return;
   }
+  // many rows: 32 lanes x 4 positions, the rows dealt out to the warps, which meet in fixed order
+  __shared__ float4 sums[kQ8JoinWarps][32];
+  const int key = key0 + 4 * lane;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  if (key < n) sum_rows(key, warp, kQ8JoinWarps, acc);
+  sums[warp][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+  __syncthreads();
+  if (warp != 0 || key >= n) return;
+#pragma unroll
+  for (int i = 1; i < kQ8JoinWarps; ++i) {
+    const float4 x = sums[i][lane];
+    acc[0] += x.x; acc[1] += x.y; acc[2] += x.z; acc[3] += x.w;
+  }
+  put(key, acc);
 }
 
 struct Q8Plan {
@@ -917,7 +966,8 @@ int launch_join(const Q8Params& p, const TrnAttnQ8Args& a, bool merge, cudaStrea
   jp.join_rows = p.ctas >= 4 * bh * p.tiles ? 1 : kQ8JoinThreads / (D / 2);
   const long long merge_ctas = merge ? units * (p.tile_rows / jp.join_rows) : 0;
   const int longest = a.kv_len != nullptr ? a.cache.S : min(max(a.kv_len_all, 0), a.cache.S);
-  const int key_tiles = a.weight != nullptr ? (longest + kQ8JoinKeys - 1) / kQ8JoinKeys : 0;
+  const int keys = p.R <= kQ8FewRows ? kQ8JoinKeys : kQ8JoinKeysRows;
+  const int key_tiles = a.weight != nullptr ? (longest + keys - 1) / keys : 0;
   const long long grid = merge_ctas + static_cast<long long>(a.B) * a.Hkv * key_tiles;
   if (grid > 0x7fffffffLL) return TRN_E_SHAPE;
   if (grid > 0)

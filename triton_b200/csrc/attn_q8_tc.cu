@@ -17,6 +17,11 @@
 // Few CTAs (less than one for each SM): the key blocks are divided among several, merged by the kernel in attn_q8.cu.
 //
 // Algorithmic flops: 4 * D per visible (row, position).
+//
+// Measured: 2 x 2048 queries on 8192 positions, 32 / 8 heads of 128, causal, bf16: 593 to 605 us = 800 TFLOP/s, 48 % of the
+// measured product rate.  Bound by the softmax warps' chain (tensor memory -> maximum -> exponential -> tensor memory; ncu: tensor
+// pipe 39 %, XU 36 %, ALU 34 %): without conversion 4 % less, without exponentials 12 % less; per CTA 9 us of set-up, q
+// and output.  The 16-bit attention core of this library takes 466 us (p in one part) and 605 us (two parts) for the shape.
 #include <type_traits>
 
 #include "attn_q8.cuh"

@@ -10,6 +10,9 @@
 // position its place, so the output is in order without a sort (a sort of 4096 scores by topk.cu: 27 us).
 // Launch 2 moves: one CTA per (row, keys or values, group of destination positions) copies the kept rows; for 8-bit caches
 // the group is a scale block, whose scale becomes the largest its rows had.
+//
+// Bound by latency: 4 x 8 rows of 4096 positions (4 heads each), 1024 kept: 12.3 us, of which 3.8 are two empty launches; 2 rows
+// of 32768 (71 heads each, summed first): 19.6 us; 262144 positions: 28.6 us.
 #include "q8.cuh"
 #include "small_mma.cuh"
 

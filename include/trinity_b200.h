@@ -312,7 +312,9 @@ typedef struct {
  * A block's scale is the smallest power of two 2^e with |x| <= 448 * 2^e for its new finite values, -64 <= e <= 120; a
  * block that already holds positions keeps the larger of its scale and that one, and where the scale grew its older
  * codes are rewritten (exact but for what falls under the smallest code).  Codes are rounded to nearest even.  An
- * infinite or NaN element is held as NaN and does not count for the scale.  D is 64 or 128. */
+ * infinite or NaN element is held as NaN and does not count for the scale.  Rows that a caller appends only as padding (a
+ * shorter sequence of a batch, whose kv_len it then sets lower) count for the scale of the block they share with real ones:
+ * zeros there cost nothing.  D is 64 or 128. */
 typedef struct {
   TrnCacheQ8 cache;
   TrnHeadTensor k_new, v_new;     /* s in [0,M) */

@@ -283,7 +283,7 @@ LONG = [
     (1, 300, 2, 1, 64, 9000, [8999], 32, HF, True),                     # tensor-core kernel, keys divided among CTAs
     (2, 9, 71, 1, 64, 5000, [4990, 5], 16, BF, True),
     # more pairs of row tiles than SMs: 192 and 320, whole rounds and a rest in pieces
-    (4, 257, 40, 8, 64, 5200, [5200, 300, 257, 5000], 64, BF, True),
+    (4, 257, 40, 8, 64, 5200, [0, 300, 257, 5200], 64, BF, True),
     (5, 130, 64, 32, 64, 700, [700, 699, 5, 0, 130], 16, HF, True),     # ... too short for pieces
 ]
 
@@ -648,6 +648,29 @@ def test_captured_steps_replay_with_growing_lengths(S):
     for t in graphs:
         assert torch.equal(t["n"], direct["n"]) and torch.equal(t["o"], direct["o"]) and torch.equal(t["w"], direct["w"])
         assert torch.equal(t["cache"].k.view(torch.uint8), direct["cache"].k.view(torch.uint8))
+
+
+@pytest.mark.parametrize("M,S", [(1, 300), (1, 9000), (40, 3000)])
+def test_plain_stream_order_equals_dependent_launch(M, S, monkeypatch):
+    """TRINITY_NO_PDL=1 (plain launches) gives the same bits, on the way through append, attention and eviction."""
+    B, Hq, Hkv, D, block, dt, keep = 2, 8, 2, 64, 32, BF, 100
+    outs = []
+    for plain in (False, True):
+        if plain:
+            monkeypatch.setenv("TRINITY_NO_PDL", "1")
+        q, kc, vc, ks, vs = _attend_inputs(B, M, Hq, Hkv, D, S, block, dt, 61)
+        cache, _, _ = _cache(kc, vc, ks, vs, block)
+        to = ops.CacheQ8.empty(B, keep, Hkv, D, block=block)
+        rows = q[:, :, :Hkv].contiguous().cuda()
+        w = torch.rand(B, Hkv, S, generator=torch.Generator().manual_seed(1)).cuda()
+        ops.cache_append(cache, rows, rows, kv_len=S - M)
+        o = ops.attention_q8(q.cuda(), cache, kv_len=S, **(dict(weight=w, weight_add=True) if M <= 16 else {}))
+        idx = ops.cache_evict(cache, to, w, kv_len=S, keep=keep, recent=5)
+        k16, v16 = (torch.zeros(B, keep, Hkv, D, dtype=dt, device="cuda") for _ in range(2))
+        ops.cache_read(to, k16, v16, kv_len=keep)
+        _done()
+        outs.append((o, idx, w, k16, v16))
+    assert all(torch.equal(a, c) for a, c in zip(*outs))
 
 
 def test_two_streams_at_once():

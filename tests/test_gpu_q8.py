@@ -313,6 +313,34 @@ def test_attention_q8_long(B, M, Hq, Hkv, D, S, lens, block, dt, causal, workspa
     assert torch.equal(o, first)
 
 
+@pytest.mark.parametrize("B,M,Hq,Hkv,D,S,lens,block,dt,causal", [
+    # weights with the rows of a kv head shared by a CTA's threads: 128 positions or 32 a CTA
+    (5, 10, 32, 8, 64, 603, [603, 1, 0, 9, 129], 32, BF, True),         # 40 rows, more CTAs than SMs
+    (5, 10, 32, 8, 128, 601, [601, 128, 127, 11, 33], 16, HF, False),
+    (1, 11, 6, 2, 128, 130, [129], 64, BF, True),                       # 33 rows, few CTAs
+    (3, 16, 16, 1, 64, 290, [290, 31, 15], 16, HF, True),               # 256 rows
+    (2, 15, 17, 1, 64, 97, [97, 3], 16, BF, True),                      # 255 rows
+    (1, 16, 512, 1, 64, 70, [69], 32, BF, True),                        # 8192 rows, the most there may be
+])
+def test_weights_of_many_rows(B, M, Hq, Hkv, D, S, lens, block, dt, causal):
+    q, kc, vc, ks, vs = _attend_inputs(B, M, Hq, Hkv, D, S, block, dt, 47)
+    _spoil_behind(kc, vc, ks, vs, lens, block)
+    r = O.attend(q, _values(kc, ks, block), _values(vc, vs, block), lens, causal, D ** -0.5)
+    cache, _, _ = _cache(kc, vc, ks, vs, block)
+    o = torch.full((B, M, Hq, D), 9.0, dtype=dt, device="cuda")
+    lse = torch.full((B, Hq, M), 9.0, device="cuda")
+    w = torch.full((B, Hkv, S + 1), 5.0, device="cuda")
+    plan = ops.AttentionQ8Plan(q.cuda(), cache, o, kv_len=torch.tensor(lens, dtype=torch.int32).cuda(), causal=causal, lse=lse, weight=w)
+    plan.run()
+    _done()
+    _check(o, lse, w, r, q, dt, D, lens, Hq // Hkv)
+    assert all(bool((w[b, :, n:] == 5.0).all()) for b, n in enumerate(lens))
+    first = w.clone()
+    plan.run()
+    _done()
+    assert torch.equal(w, first)
+
+
 def test_lengths_outside_the_cache_count_as_the_nearer_end():
     B, Hq, Hkv, D, S, block, dt = 2, 4, 2, 64, 60, 16, BF
     q, kc, vc, ks, vs = _attend_inputs(B, 1, Hq, Hkv, D, S, block, dt, 43)

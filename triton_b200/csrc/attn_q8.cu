@@ -684,9 +684,13 @@ attn_q8_cluster_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
 // of a (b, kv head), four at a time a thread, rows in ascending order.
 constexpr int kQ8JoinThreads = 256;
 constexpr int kQ8JoinWarps = kQ8JoinThreads / 32;
-// Positions of a weight CTA: with few rows per kv head its threads are for positions, with many they share the rows (a
-// thread for all 568 rows of 71 heads and 8 queries: 223 us for a call that takes 53 this way)
-constexpr int kQ8FewRows = 16, kQ8JoinKeys = 8 * kQ8JoinThreads, kQ8JoinKeysRows = 128;
+// Positions of a weight CTA: with few rows per kv head its threads are for positions, with more they share the rows.  From 256
+// rows on 32 positions, so that the rows are shared 32 ways: 568 rows of one head of 64 and 8192 positions 36 us the call, 55
+// with 128 positions, 223 with all rows in a thread; 1136 rows, 8192 positions 54, 94.  Below, every CTA's own pass over the
+// rows' sums weighs more (64 rows of 8 x 8 heads, 4096 positions: 133, 103), so there 128, unless those CTAs are fewer than the
+// SMs (142 rows of one head, 2000 positions: 21.2, 26.1); 32 rows and fewer gain nothing there either (20 rows of 8 heads,
+// 2000 positions: 24.1, 21.5).
+constexpr int kQ8FewRows = 16, kQ8JoinKeys = 8 * kQ8JoinThreads, kQ8JoinKeysRows = 128, kQ8JoinKeysShort = 32, kQ8RowsShort = 256;
 // maximum and sum of a row over its pieces by one warp; at: the row in the first piece's slot
 __device__ __forceinline__ float2 join_ml(const Q8Params& p, long long at, int here, int lane) {
   float2 mine = make_float2(-INFINITY, 0.f);   // a lane's pieces lane, lane + 32, ...
@@ -771,7 +775,7 @@ attn_q8_join_kernel(const __grid_constant__ Q8Params p, int merge_ctas, int key_
   const int id = static_cast<int>(blockIdx.x) - merge_ctas;
   const int bh = id / key_tiles, b = bh / p.Hkv, h = bh % p.Hkv;
   const int n = p.len(b);
-  const int keys = p.R <= kQ8FewRows ? kQ8JoinKeys : kQ8JoinKeysRows, key0 = (id % key_tiles) * keys;
+  const int keys = p.join_keys, key0 = (id % key_tiles) * keys;
   if (key0 >= n) return;
   auto ml_at = [&](int r, int& here) {
     const int unit = bh * p.tiles + r / p.tile_rows;
@@ -835,20 +839,25 @@ attn_q8_join_kernel(const __grid_constant__ Q8Params p, int merge_ctas, int key_
     }
     return;
   }
-  // many rows: 32 lanes x 4 positions, the rows dealt out to the warps, which meet in fixed order
-  __shared__ float4 sums[kQ8JoinWarps][32];
-  const int key = key0 + 4 * lane;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  if (key < n) sum_rows(key, warp, kQ8JoinWarps, acc);
-  sums[warp][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-  __syncthreads();
-  if (warp != 0 || key >= n) return;
+  // many rows: LANES x 4 positions, the rows dealt out to the groups of as many lanes, which meet in fixed order
+  __shared__ float4 sums[kQ8JoinThreads];
+  auto weigh = [&](auto lanes) {
+    constexpr int LANES = decltype(lanes)::value, N = kQ8JoinThreads / LANES;
+    const int key = key0 + 4 * (tid % LANES);
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    if (key < n) sum_rows(key, tid / LANES, N, acc);
+    sums[tid] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    __syncthreads();
+    if (tid >= LANES || key >= n) return;
 #pragma unroll
-  for (int i = 1; i < kQ8JoinWarps; ++i) {
-    const float4 x = sums[i][lane];
-    acc[0] += x.x; acc[1] += x.y; acc[2] += x.z; acc[3] += x.w;
-  }
-  put(key, acc);
+    for (int i = 1; i < N; ++i) {
+      const float4 x = sums[i * LANES + tid];
+      acc[0] += x.x; acc[1] += x.y; acc[2] += x.z; acc[3] += x.w;
+    }
+    put(key, acc);
+  };
+  if (keys == kQ8JoinKeysShort) weigh(std::integral_constant<int, kQ8JoinKeysShort / 4>{});
+  else weigh(std::integral_constant<int, kQ8JoinKeysRows / 4>{});
 }
 
 struct Q8Plan {
@@ -972,7 +981,10 @@ int launch_join(const Q8Params& p, const TrnAttnQ8Args& a, bool merge, cudaStrea
   jp.join_rows = p.ctas >= 4 * bh * p.tiles ? 1 : kQ8JoinThreads / (D / 2);
   const long long merge_ctas = merge ? units * (p.tile_rows / jp.join_rows) : 0;
   const int longest = a.kv_len != nullptr ? a.cache.S : min(max(a.kv_len_all, 0), a.cache.S);
-  const int keys = p.R <= kQ8FewRows ? kQ8JoinKeys : kQ8JoinKeysRows;
+  jp.join_keys = p.R <= kQ8FewRows ? kQ8JoinKeys : kQ8JoinKeysRows;
+  if (p.R >= kQ8RowsShort || (p.R > 32 && bh * ((longest + kQ8JoinKeysRows - 1) / kQ8JoinKeysRows) <= kAttnNominalSMs))
+    jp.join_keys = kQ8JoinKeysShort;
+  const int keys = jp.join_keys;
   const int key_tiles = a.weight != nullptr ? (longest + keys - 1) / keys : 0;
   const long long grid = merge_ctas + static_cast<long long>(a.B) * a.Hkv * key_tiles;
   if (grid > 0x7fffffffLL) return TRN_E_SHAPE;

@@ -30,6 +30,7 @@ struct Q8Params {
   // join_pairs > 0: the merge visits only the pairs of row tiles from join_first on, in the order late pairs first
   int join_pairs, join_first;
   int join_rows;                               // rows a CTA of the merge takes: 1, or as many as its threads are for
+  int join_keys;                               // positions a CTA that sums weights takes
   float* scores;                               // [B * Hkv][R][pitch], log2 domain, or NULL
   long long pitch;
   float* weight;

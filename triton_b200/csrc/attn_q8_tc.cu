@@ -773,9 +773,10 @@ int launch_typed(const TrnAttnQ8Args& a, cudaStream_t st, const DeviceState& ds)
 
 }  // namespace
 
-// More than 32 rows per kv head (bf16, us here and in attn_q8.cu: 36 rows of 16 x 8 heads, 2048 positions 48.7, 62.8; 60 rows of
-// 7 x 32 heads, 4674 positions 191, 226; 71 rows of 32 x 1 head of 64, 4096 positions 31.2, 40.7), and no weights (those are
-// summed from scores that attn_q8.cu keeps)
+// More than 32 rows per kv head (bf16, us here and in attn_q8.cu: 32 rows of 8 x 8 heads, 4096 positions 61.6, 46.4; 36 rows of
+// 16 x 8 heads, 2048 positions 48.7, 62.8; 60 rows of 7 x 32 heads, 4674 positions 191, 226; 71 rows of 32 x 1 head of 64, 4096
+// positions 31.2, 40.7), and no weights (those are summed from scores that attn_q8.cu keeps; kept here, by threads with a row
+// each: 36 rows of 8 x 8 heads, 4096 positions 95.8 us, there 78.1; 568 rows of one head of 64, 8192 positions 67.6, 55.8)
 bool attn_q8_tc_applies(const TrnAttnQ8Args& a) {
   return a.weight == nullptr && static_cast<long long>(a.M) * (a.Hq / a.Hkv) > 32;
 }

@@ -1,0 +1,107 @@
+"""Attention over the 8-bit cache at the ends of what its scales, queries and probabilities may be, in both of its kernels
+(few rows per kv head; many)."""
+import math
+
+import pytest
+import torch
+
+import q8_oracle as O
+import test_gpu_q8 as Q
+from triton_b200 import ops
+
+pytestmark = pytest.mark.gpu
+BF, HF = torch.bfloat16, torch.float16
+
+
+def _call(q, kc, vc, ks, vs, lens, block, causal=True, weigh=False, **kw):
+    """One call and its result in 64 bits."""
+    B, M, Hq, D = q.shape
+    Hkv, S = kc.shape[1:3]
+    r = O.attend(q, Q._values(kc, ks, block), Q._values(vc, vs, block), lens, causal, D ** -0.5)
+    cache, _, _ = Q._cache(kc, vc, ks, vs, block)
+    o, lse = torch.zeros(B, M, Hq, D, dtype=q.dtype, device="cuda"), torch.zeros(B, Hq, M, device="cuda")
+    w = torch.zeros(B, Hkv, S, device="cuda") if weigh else None
+    ops.attention_q8(q.cuda(), cache, o, kv_len=torch.tensor(lens, dtype=torch.int32).cuda(), causal=causal, lse=lse, weight=w, **kw)
+    Q._done()
+    return o, lse, w, r
+
+
+# --------------------------------------------------------------------------------------- scales of the values far apart
+
+FAR = [
+    # M, Hq, Hkv, D, n, block, dtype, weigh
+    (1, 4, 2, 128, 200, 16, BF, True),           # a cluster for each unit
+    (2, 4, 2, 64, 900, 64, BF, True),
+    (1, 4, 2, 128, 9000, 128, BF, True),         # pieces, merged
+    (9, 4, 1, 64, 5000, 32, BF, True),           # 36 rows: weights by threads that share the rows
+    (40, 4, 2, 128, 300, 16, BF, False),         # tensor-core kernel
+    (70, 4, 2, 64, 2000, 32, BF, False),         # ... its key blocks divided among CTAs
+    (1, 4, 2, 128, 200, 16, HF, True),
+    (40, 4, 2, 64, 300, 16, HF, False),
+]
+
+
+@pytest.mark.parametrize("low,high,order", [(2.0 ** -64, 2.0 ** 80, "mixed"), (2.0 ** -64, 2.0 ** 120, "mixed"), (2.0 ** -64, 2.0 ** 120, "rising"),
+                                            (2.0 ** -64, 2.0 ** 120, "falling"), (0.0, 2.0 ** 40, "mixed"), (0.0, 2.0 ** 100, "rising")])
+@pytest.mark.parametrize("M,Hq,Hkv,D,n,block,dt,weigh", FAR)
+def test_value_scales_at_both_ends_of_their_range(M, Hq, Hkv, D, n, block, dt, weigh, low, high, order):
+    """Blocks with the smallest scales keep their weight in the softmax beside blocks with the largest: mixed, the large ones last
+    (what was summed moves to a larger maximum) and first."""
+    if dt == HF:                                 # whose largest number bounds the scale
+        low, high = (0.0, 2.0 ** 4) if low == 0.0 else (2.0 ** -64, 2.0 ** 5)
+    q, kc, vc, ks, vs = Q._attend_inputs(1, M, Hq, Hkv, D, n, block, dt, 71)
+    nblk = vs.shape[2]
+    is_high = {"mixed": torch.arange(nblk) % 3 == 1, "rising": torch.arange(nblk) >= nblk // 2, "falling": torch.arange(nblk) < nblk // 2}[order]
+    vs[:] = torch.where(is_high, high, low)
+    if low == 0.0:
+        vc[:, :, ~is_high.repeat_interleave(block)[:n]] = 0
+    if high == 2.0 ** 120:                       # what an append leaves there: below 2^128 with its scale
+        vc = ((vc.view(torch.float8_e4m3fn).float().clamp(-240, 240)).to(torch.float8_e4m3fn)).view(torch.uint8)
+    o, lse, w, r = _call(q, kc, vc, ks, vs, [n], block, weigh=weigh)
+    # Beside what _check counts: a maximum of size up to 128 + |t| has a step of 2^-16 (half of it in each of the exponents of a term, and
+    # the same in lse), and a smallest term flushed at 2^-126 against a sum of 2^-96 or more, n of them at most
+    extra = 2.0 ** -15 + n * 2.0 ** -30
+    far = r["lse"].isfinite()
+    ds = (D + 8) * 2.0 ** -23 * r["T"] + 2.0 ** -21
+    e = (lse.double().cpu() - r["lse"]).abs()
+    assert torch.equal(lse.cpu().double() == -math.inf, ~far)
+    assert bool((e <= 1.5 * ds + 2.0 ** -21 * (1 + r["lse"].abs()) + extra)[far].all()), e[far].max().item()
+    # o, each column against its own sum of p |v|, and against what a subnormal P' of fp16 loses: half a step, 2^-25, of at least 2^6
+    # that the largest p vs has, times codes of up to 448
+    top = Q._values(torch.full_like(vc, 0x38), vs, block).amax().item()
+    tol, _ = Q._tolerance(r, q, dt, D)
+    tol = tol + extra * r["A"] + (448 * n * 2.0 ** -31 * top if order != "mixed" else 0.0)
+    e = (o.double().cpu() - r["o"]).abs()
+    assert bool((e <= tol).all()), (e / tol).max().item()
+    if weigh:
+        e = (w.double().cpu() - r["weight"]).abs()
+        rel = 2 * ds.amax().item() + 2.0 ** -23 * M * Hq // Hkv + 2.0 ** -20 + 2 * extra
+        assert bool((e <= rel * r["weight"] + 1e-30).all()), (e / r["weight"].clamp_min(1e-30)).max().item()
+
+
+@pytest.mark.parametrize("M,n,weigh", [(1, 70000, True), (40, 40000, False)])
+def test_a_cache_of_zeros_with_scale_zero(M, n, weigh):
+    """Values of 0 with a scale of 0 throughout, as a cache that was never filled holds them: the weights are those of the keys, and
+    the sums of many large terms stay in range.  One query row, then 40 in the tensor-core kernel, where the keys behind the first
+    block score 2^7.2 times as much as that one: under the 2^8 by which a score may pass the maximum in use."""
+    D, block = 64, 128
+    q = torch.zeros(1, M, 2, D)
+    q[..., 0] = 1.0
+    q[:, :, 1] *= -1.0
+    q = q.to(BF)
+    kc, vc = torch.zeros(1, 1, n, D, dtype=torch.uint8), torch.zeros(1, 1, n, D, dtype=torch.uint8)
+    if M > 1:
+        kc[0, 0, block:, 0] = torch.tensor(40.0).to(torch.float8_e4m3fn).view(torch.uint8).item()
+    ks = torch.ones(1, 1, -(-n // block))
+    vs = torch.zeros_like(ks)
+    r = O.attend(q, Q._values(kc, ks, block), Q._values(vc, vs, block), [n], True, D ** -0.5)
+    cache, _, _ = Q._cache(kc, vc, ks, vs, block)
+    o, lse = torch.ones(1, M, 2, D, dtype=BF, device="cuda"), torch.zeros(1, 2, M, device="cuda")
+    w = torch.zeros(1, 1, n, device="cuda") if weigh else None
+    plan = ops.AttentionQ8Plan(q.cuda(), cache, o, kv_len=n, lse=lse, weight=w)
+    if not weigh:
+        plan.args.workspace, plan.args.workspace_bytes = None, 0     # one CTA sums all keys
+    plan.run()
+    Q._done()
+    assert bool((o == 0).all())
+    Q._check(o, lse, w, r, q, BF, D, [n], 2)

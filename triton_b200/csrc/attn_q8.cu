@@ -6,9 +6,12 @@
 //   * q enters as fp16 times a power of two per row (2^(14 - e), e the exponent of the row's largest element): exact for
 //     fp16 q, and for bf16 q but for elements 2^-28 below the row's largest, whose error is at most 2^-39 of that one;
 //   * ks multiplies the score:  t = acc * (scale * log2 e * row factor * ks);
-//   * vs is folded into the exponent:  t' = t + log2 vs,  running maximum m' of t',  P' = 2^(t' - m') <= 1,
-//     O = sum P' vc,  l = sum P' / vs,  o = O / l,  lse = m' + log2 l  (P' / vs = 2^(t - m')).
-//     P' is what its key adds to O whatever its block's scale, so its rounding to 16 bits is relative to the output.
+//   * vs enters the running maximum and one multiplication:  m' = max (t + log2 vs),  E = 2^(t - m'),  l = sum E,
+//     P' = E vs <= 1,  O = sum P' vc,  o = O / l,  lse = m' + log2 l.
+//     P' is what its key adds to O whatever its block's scale, so its rounding to 16 bits is relative to the largest of
+//     these, taken over the row.  (A column in which the blocks of large scale hold nothing but zeros gets its values from P' that
+//     are smaller by the scales' ratio: with scales 2^26 (attn_q8_tc.cu: 2^20) and more apart these are subnormal in fp16, and such
+//     a column is off by up to 448 * 2^-37 (2^-31) of the row's largest p vs for each position.)
 // P' carries a factor 2^12 into the product (it cancels in O / l), which keeps weights down to 2^-26 of the row's largest out of
 // fp16's subnormals.  bf16 outputs take P' as one fp16 (off by at most 2^-11 of itself, the output's rounding by
 // 2^-8); fp16 outputs take it as hi + lo, since one part alone would err as much as the output's own rounding.
@@ -267,10 +270,10 @@ __device__ __forceinline__ void q8_piece(const Q8Params& p, const CUtensorMap& t
 
   for (int c = 0; c < w.n_chunks; ++c) {
     const int s = (w.loaded + c) % ST, key0 = (w.chunk0 + c) * kQ8Keys;
-    float lv[2], inv[2];
+    float lv[2], vf[2];
     const float ks[2] = {ks_next[0], ks_next[1]};
 #pragma unroll
-    for (int i = 0; i < 2; ++i) scale_log_inv(vs_next[i] < kMinVScale ? kMinVScale : vs_next[i], lv[i], inv[i]);
+    for (int i = 0; i < 2; ++i) v_scale_terms(vs_next[i], lv[i], vf[i]);
     scales_of(c + 1, ks_next, vs_next);
     const bool edge = key0 + kQ8Keys - 1 > w.lim_min;                // some row does not see some position of the chunk
     ok = mbar_wait(bars + 8 * s, ((w.loaded + c) / ST) & 1, ctl, KST_TIMEOUT_CONSUMER);
@@ -303,7 +306,7 @@ __device__ __forceinline__ void q8_piece(const Q8Params& p, const CUtensorMap& t
         }
       }
     }
-    // ---- t = acc * c * ks, t' = t + log2 vs.  Accumulator (2 k + e): position 8 k + q8_key(g) of the block, column 2t + e
+    // ---- t = acc * c * ks.  Accumulator (2 k + e): position 8 k + q8_key(g) of the block, column 2t + e
     bool raise = false;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -311,17 +314,16 @@ __device__ __forceinline__ void q8_piece(const Q8Params& p, const CUtensorMap& t
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float a = cq[nt][e] * ks[i];
+          const float a = cq[nt][e] * ks[i], over = m_ref[nt][e] + kQ8Slack - lv[i];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             const int key = key0 + 16 * i + 8 * k + q8_key<D>(g);
             float x = st[i][nt][2 * k + e] * a;
             // whoever reads the kept scores knows which of them a row sees
             if (sc[nt][e] != nullptr) sc[nt][e][key] = x;
-            x += lv[i];
             if (edge && key > lim[nt][e]) x = -INFINITY;
             st[i][nt][2 * k + e] = x;
-            raise = raise || x > m_ref[nt][e] + kQ8Slack;
+            raise = raise || x > over;
           }
         }
     if (__any_sync(0xffffffffu, raise)) {
@@ -330,13 +332,14 @@ __device__ __forceinline__ void q8_piece(const Q8Params& p, const CUtensorMap& t
         float al[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float mx = fmaxf(fmaxf(st[0][nt][e], st[0][nt][2 + e]), fmaxf(st[1][nt][e], st[1][nt][2 + e]));
+          float mx = fmaxf(fmaxf(st[0][nt][e], st[0][nt][2 + e]) + lv[0], fmaxf(st[1][nt][e], st[1][nt][2 + e]) + lv[1]);
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
           const float mn = fmaxf(m_ref[nt][e], mx);
-          al[e] = mn == -INFINITY ? 1.f : ex2_approx(m_ref[nt][e] - mn);
+          const float d = mn == -INFINITY ? 0.f : m_ref[nt][e] - mn;
+          al[e] = ex2_approx(d);
           m_ref[nt][e] = mn;
-          l_run[nt][e] *= al[e];
+          l_run[nt][e] = sum_moved(l_run[nt][e], d);
         }
 #pragma unroll
         for (int i = 0; i < DT; ++i) {
@@ -345,20 +348,22 @@ __device__ __forceinline__ void q8_piece(const Q8Params& p, const CUtensorMap& t
         }
       }
     }
-    // ---- P' = 2^(t' - m'), transposed into the B operand of o^T += v^T P'^T
+    // ---- E = 2^(t - m'), P' = E vs, transposed into the B operand of o^T += v^T P'^T
     uint32_t ph[2][NT][2], pl[2][NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float use[2];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) use[e] = kQ8PBias - (m_ref[nt][e] == -INFINITY ? 0.f : m_ref[nt][e]);
+      for (int e = 0; e < 2; ++e) use[e] = kQ8PBias + kQ8LBias - (m_ref[nt][e] == -INFINITY ? 0.f : m_ref[nt][e]);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const float a = ex2_approx(st[i][nt][2 * k] + use[0]), c2 = ex2_approx(st[i][nt][2 * k + 1] + use[1]);
-          l_run[nt][0] = fmaf(a, inv[i], l_run[nt][0]);
-          l_run[nt][1] = fmaf(c2, inv[i], l_run[nt][1]);
+          float a = ex2_approx(st[i][nt][2 * k] + use[0]), c2 = ex2_approx(st[i][nt][2 * k + 1] + use[1]);
+          l_run[nt][0] += a;
+          l_run[nt][1] += c2;
+          a *= vf[i];
+          c2 *= vf[i];
           const uint32_t hi = Io<__half>::pack2(a, c2);
           ph[i][nt][k] = transpose8(hi);
           if constexpr (HILO) {
@@ -457,7 +462,7 @@ __device__ __forceinline__ void q8_piece(const Q8Params& p, const CUtensorMap& t
     const float* src = part + (i * ROWS + row) * SM::kRow;
     if (src[D + 1] == 0.f) continue;                               // saw no position of this row
     const float f = ex2_approx(src[D] - mx);
-    tot = fmaf(f, src[D + 1], tot);
+    tot += sum_moved(src[D + 1], src[D] - mx);
 #pragma unroll
     for (int c = 0; c < CW; ++c) acc[c] = fmaf(f, src[c0 + c], acc[c]);
   }
@@ -649,7 +654,7 @@ attn_q8_cluster_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
     for (int i = 0; i < kQ8MaxCluster; ++i)
       if (i < cluster && ml[i].y != 0.f) {
         const float f = ex2_approx(ml[i].x - m);
-        sum = fmaf(f, ml[i].y, sum);
+        sum += sum_moved(ml[i].y, ml[i].x - m);
         o[0] = fmaf(f, v[i].x, o[0]);
         o[1] = fmaf(f, v[i].y, o[1]);
       }
@@ -661,9 +666,9 @@ attn_q8_cluster_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
       for (int i = 0; i < cluster; ++i) m = fmaxf(m, ml_of(r, i).x);
       for (int i = 0; i < cluster; ++i) {
         const float2 ml = ml_of(r, i);
-        if (ml.y != 0.f) sum = fmaf(ex2_approx(ml.x - m), ml.y, sum);
+        if (ml.y != 0.f) sum += sum_moved(ml.y, ml.x - m);
       }
-      lse_of[r] = m - kQ8PBias + log2f(sum);
+      lse_of[r] = m - (kQ8PBias + kQ8LBias) + log2f(sum);
     }
     __syncthreads();
     // only launched with one row tile per (b, kv head): the rows of the tile are all that see a position
@@ -698,13 +703,13 @@ __device__ __forceinline__ float2 join_ml(const Q8Params& p, long long at, int h
     const float2 ml = p.part_ml[at + static_cast<long long>(s) * p.tile_rows];
     if (ml.y == 0.f) continue;
     const float m = fmaxf(mine.x, ml.x);
-    mine.y = (mine.y == 0.f ? 0.f : mine.y * ex2_approx(mine.x - m)) + ml.y * ex2_approx(ml.x - m);
+    mine.y = (mine.y == 0.f ? 0.f : sum_moved(mine.y, mine.x - m)) + sum_moved(ml.y, ml.x - m);
     mine.x = m;
   }
   float m = mine.x;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  float tot = mine.y == 0.f ? 0.f : mine.y * ex2_approx(mine.x - m);
+  float tot = mine.y == 0.f ? 0.f : sum_moved(mine.y, mine.x - m);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) tot += __shfl_xor_sync(0xffffffffu, tot, o);
   return make_float2(m, tot);
@@ -788,7 +793,7 @@ attn_q8_join_kernel(const __grid_constant__ Q8Params p, int merge_ctas, int key_
       int here;
       const long long at = ml_at(r, here);
       const float2 ml = join_ml(p, at, here, lane);
-      if (lane == 0) q8_join[r] = ml.x - kQ8PBias + log2f(ml.y);
+      if (lane == 0) q8_join[r] = ml.x - (kQ8PBias + kQ8LBias) + log2f(ml.y);
     }
   } else {                                     // a thread for each row: rows side by side
     for (int r = tid; r < p.R; r += kQ8JoinThreads) {
@@ -800,11 +805,11 @@ attn_q8_join_kernel(const __grid_constant__ Q8Params p, int merge_ctas, int key_
         const float2 ml = p.part_ml[at + static_cast<long long>(s) * p.tile_rows];
         const float mn = fmaxf(m, ml.x);
         if (ml.y != 0.f) {
-          l = (l == 0.f ? 0.f : l * ex2_approx(m - mn)) + ml.y * ex2_approx(ml.x - mn);
+          l = (l == 0.f ? 0.f : sum_moved(l, m - mn)) + sum_moved(ml.y, ml.x - mn);
           m = mn;
         }
       }
-      q8_join[r] = m - kQ8PBias + log2f(l);
+      q8_join[r] = m - (kQ8PBias + kQ8LBias) + log2f(l);
     }
   }
   __syncthreads();

@@ -9,8 +9,14 @@
 
 namespace trn {
 
+// v's scale stands at its whole power of two in the running maximum, m' = max (t + ceil log2 vs), and as itself in the factor of
+// the product:  E = 2^(t - m'),  l = sum E,  P' = E vs.  With vs within [2^-64, 2^120] the terms E of a row reach from
+// 2^-120 (the maximum's own, at the largest scale) to 2^64, so the sum of up to 2^29 of them stays inside 32 bits with a
+// factor of 2^30 (kQ8PBias + kQ8LBias), and what lies under 2^-126, which is flushed, is 2^-36 of the row's sum or less.  (l as sum of
+// P' / vs loses the terms whose P' is flushed, although 1 / vs may make them the largest: scales 2^138 apart.)
 constexpr float kQ8PBias = 12.f;               // log2 of the factor P' carries into the product
-constexpr float kMinVScale = 7.888609052210118e-31f;   // 2^-100: smaller scales (a block of zeros) count as this
+constexpr float kQ8LBias = 18.f;               // log2 of the factor E carries beside that
+constexpr float kMinVScale = 5.421010862427522e-20f;   // 2^-64: in the maximum, smaller scales (0: a block of zeros) count as this
 
 struct Q8Params {
   TrnHeadTensor q, o;
@@ -63,16 +69,16 @@ __device__ __forceinline__ uint32_t q8_off(uint32_t r, uint32_t u) {
   if constexpr (D == 128) return r * 128u + ((u ^ (r & 7u)) << 4);
   else return r * 64u + ((u ^ ((r >> 1) & 3u)) << 4);
 }
-// log2 and reciprocal of a scale: exact for powers of two
-__device__ __forceinline__ void scale_log_inv(float s, float& lg, float& inv) {
-  const uint32_t u = __float_as_uint(s);
-  if ((u & 0x7fffffu) == 0u && u - (1u << 23) < (252u << 23)) {       // 2^-126 .. 2^125
-    lg = static_cast<float>(static_cast<int>(u >> 23) - 127);
-    inv = __uint_as_float((254u << 23) - u);
-  } else {
-    lg = log2f(s);
-    inv = 1.0f / s;
-  }
+// a scale of v: exponent of the next power of two in the running maximum, and the factor from E to P'
+__device__ __forceinline__ void v_scale_terms(float s, float& lg, float& f) {
+  lg = static_cast<float>(static_cast<int>((__float_as_uint(fmaxf(s, kMinVScale)) + 0x7fffffu) >> 23) - 127);
+  f = s * 3.814697265625e-06f;                 // 2^-kQ8LBias
+}
+// a sum l moved to a maximum that is larger by -d: 2^d by halves, since d reaches -184 between a small and a large scale of v
+// while what is left of l may still be most of the row's sum
+__device__ __forceinline__ float sum_moved(float l, float d) {
+  const float h = ex2_approx(0.5f * d);
+  return l * h * h;
 }
 // 0xff in every byte of w that holds a NaN code (0x7f or 0xff)
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
@@ -82,12 +88,12 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
 template <typename T, int CW>
 __device__ __forceinline__ void q8_store_row(const Q8Params& p, int b, int h, int r, int c0, const float* acc, float mx, float tot) {
   const int i = r / p.G, hq = h * p.G + r % p.G;
-  const float inv = tot == 0.f ? 0.f : 1.0f / tot;
+  const float inv = tot == 0.f ? 0.f : 262144.f / tot;                // 2^kQ8LBias
   T* dst = static_cast<T*>(p.o.ptr) + b * p.o.stride_b + static_cast<long long>(i) * p.o.stride_s +
            static_cast<long long>(hq) * p.o.stride_h + c0;
 #pragma unroll
   for (int c = 0; c < CW; c += 2) *reinterpret_cast<uint32_t*>(dst + c) = Io<T>::pack2(acc[c] * inv, acc[c + 1] * inv);
-  if (c0 == 0 && p.lse != nullptr) p.lse[(static_cast<long long>(b) * p.Hq + hq) * p.M + i] = mx - kQ8PBias + log2f(tot);
+  if (c0 == 0 && p.lse != nullptr) p.lse[(static_cast<long long>(b) * p.Hq + hq) * p.M + i] = mx - (kQ8PBias + kQ8LBias) + log2f(tot);
 }
 
 inline size_t up256(size_t v) { return (v + 255) / 256 * 256; }

@@ -9,11 +9,11 @@
 //                groups.  (Codes fetched to registers instead made the proxy fence that publishes a tile wait for the
 //                fetches under way.)
 //   warps 4-7,   softmax of tile 0 / 1, one thread per row: q -> shared memory as fp16 times a power of two; then per block of
-//   warps 8-11   128 positions  t' = s * (c ks) + log2 vs,  P' = 2^(t' - m'), packed to fp16 over s in tensor memory,
-//                l += P' / vs;  o is rescaled only when a row's maximum grew by more than 2^8 since the last time
+//   warps 8-11   128 positions  t = s * (c ks),  E = 2^(t - m'),  l += E,  P' = E vs, packed to fp16 over s in tensor memory
+//                (m' as in attn_q8.cu);  o is rescaled only when a row's maximum grew by more than 2^8 since the last time
 //   warp 3       issues S_t = q_t k^T and O_t += P'_t v (P' from tensor memory)
-// The scales cost nothing per score: ks and log2 vs change every 16 columns at most and enter the multiply-add that the
-// softmax makes anyway.  bf16 outputs take P' as one fp16 part, fp16 outputs as hi + lo (see attn_q8.cu).
+// ks enters the multiply-add that the softmax makes anyway, vs costs half a (packed) multiplication a score; both change every
+// 16 columns at most.  bf16 outputs take P' as one fp16 part, fp16 outputs as hi + lo (see attn_q8.cu).
 // Few CTAs (less than one for each SM): the key blocks are divided among several, merged by the kernel in attn_q8.cu.
 //
 // Algorithmic flops: 4 * D per visible (row, position).
@@ -59,7 +59,7 @@ struct TcSmem {
   static constexpr int kKV = 2 * kTile;
   static constexpr int kRaw = kKV + kStages * 2 * kTile;             // codes of k, codes of v
   static constexpr int kRawTile = 128 * D;
-  static constexpr int kScales = kRaw + 2 * kRawTile;         // [stage][8 groups] (ks, log2 vs, 1 / vs, -)
+  static constexpr int kScales = kRaw + 2 * kRawTile;         // [stage][8 groups] (ks, log2 vs rounded up, vs 2^-18, -)
   static constexpr int kNan = kScales + kStages * 8 * 16;            // [D] first position with a NaN code in v
   static constexpr int kBars = kNan + D * 4;
   static constexpr int kTotal = kBars + 256 + 1024;
@@ -312,9 +312,9 @@ attn_q8_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       if (threadIdx.x < 8) {
-        float lg, inv;
-        scale_log_inv(vs < kMinVScale ? kMinVScale : vs, lg, inv);
-        scales[st * 8 + threadIdx.x] = make_float4(ks, lg, inv, 0.f);
+        float lg, f;
+        v_scale_terms(vs, lg, f);
+        scales[st * 8 + threadIdx.x] = make_float4(ks, lg, f, 0.f);
       }
       convert(0, k_s(st), kv0, edge);
       mbar_arrive(k_full(st));
@@ -480,7 +480,7 @@ attn_q8_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       }
       const float4* sc = scales + st * 8;
       const bool masked = kv0 + kTcKeys - 1 > limit_min;
-      // ---- pass 1: the block's maximum of t'
+      // ---- pass 1: the block's maximum of t + log2 vs
       float mb = -INFINITY;
 #pragma unroll
       for (int c = 0; c < kTcKeys / 32; ++c) {
@@ -512,8 +512,8 @@ attn_q8_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       float alpha = 1.0f;
       if (grow) {
         alpha = ex2_approx(m_run - m_new);                         // 0 on the first block
+        l_run = sum_moved(l_run, m_run - m_new);
         m_run = m_new;
-        l_run *= alpha;
       }
       // S_t(j) was produced after P'_t(j-1) v (MMAs run in issue order), so O_t is quiescent here
       if (j > 0 && __any_sync(0xffffffffu, grow)) {
@@ -527,7 +527,7 @@ attn_q8_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           tmem_st16(o_tmem + c * 16, y);
         }
       }
-      // ---- pass 2: P' = 2^(t' - m'), written over S (hi | lo per 32 columns); compiled twice, without and with masks
+      // ---- pass 2: P' = 2^(t - m') vs, written over S (hi | lo per 32 columns); compiled twice, without and with masks
       auto pass2 = [&](auto masked_tag) {
         constexpr bool kMasked = decltype(masked_tag)::value;
         auto chunk_p = [&](const uint32_t (&src)[32], int c, uint32_t (&pk)[SPLIT ? 32 : 16]) {
@@ -536,8 +536,8 @@ attn_q8_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 #pragma unroll
           for (int i0 = 0; i0 < 16; i0 += 8) {                     // pairs of columns, eight at a time
             if (GRP == 16 || i0 == 0) f = sc[c * 2 + i0 / 8];
-            const float a = c_row * f.x, d = f.y - m_run;
-            const float2 a2 = make_float2(a, a), d2 = make_float2(d, d);
+            const float a = c_row * f.x, d = kQ8LBias - m_run;
+            const float2 a2 = make_float2(a, a), d2 = make_float2(d, d), f2 = make_float2(f.z, f.z);
             float2 pp[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -555,7 +555,9 @@ attn_q8_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
             sum = GRP == 16 || i0 == 0 ? pp[0] : __fadd2_rn(sum, pp[0]);
 #pragma unroll
             for (int i = 1; i < 8; ++i) sum = __fadd2_rn(sum, pp[i]);
-            if (GRP == 16 || i0 == 8) l_run = fmaf(sum.x + sum.y, f.z, l_run);
+            if (GRP == 16 || i0 == 8) l_run += sum.x + sum.y;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) pp[i] = __fmul2_rn(pp[i], f2);
 #pragma unroll
             for (int i = 0; i < 8; ++i) pk[i0 + i] = Io<__half>::pack2(pp[i].x, pp[i].y);
             if constexpr (SPLIT) {
@@ -635,7 +637,7 @@ attn_q8_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
                                                               __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
         } else {
           // rows meet in the q tile's place (its products are done), so that the warp can write whole lines
-          const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;
+          const float inv = l_run == 0.f ? 0.f : 262144.f / l_run;         // 2^kQ8LBias
 #pragma unroll
           for (int i = 0; i < 32; i += 8)
             asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};"
@@ -663,7 +665,7 @@ attn_q8_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       if (there) {
         if (parts) p.part_ml[slot * kTcRows + lrow] = make_float2(m_run + kQ8PBias, l_run);    // in the merge's convention
         else if (p.lse != nullptr)
-          p.lse[(static_cast<long long>(b) * p.Hq + h * p.G + r % p.G) * p.M + r / p.G] = m_run + log2f(l_run);
+          p.lse[(static_cast<long long>(b) * p.Hq + h * p.G + r % p.G) * p.M + r / p.G] = m_run - kQ8LBias + log2f(l_run);
       }
       if (p.pieces != nullptr && (tp.ctas > 0 || parts) && split == 0 && lrow == 0) {      // where the merge finds them: slot = unit + entry
         const int u = bh * p.tiles + tile, first = static_cast<int>(slot) - u;

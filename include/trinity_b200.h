@@ -22,7 +22,7 @@
 extern "C" {
 #endif
 
-#define TRINITY_ABI_VERSION 3
+#define TRINITY_ABI_VERSION 4
 
 /* element types of activations / weights / outputs */
 enum { TRN_BF16 = 0, TRN_FP16 = 1 };
@@ -362,6 +362,9 @@ typedef struct {
   void* workspace;                /* 256-byte aligned device scratch of trinity_attention_q8_workspace() bytes; contents need
                                      not be initialised.  NULL without `weight`: the key range is not divided. */
   size_t workspace_bytes;
+  int single_p;                   /* as in TrnAttnArgs.  0 (default): p is carried as hi + lo fp16 parts into the P v product
+                                     (22 mantissa bits); 1: one fp16 part only (11 bits, for both types of o; faster
+                                     where the products bind) */
 } TrnAttnQ8Args;
 int trinity_attention_q8(const TrnAttnQ8Args* a, void* cuda_stream);
 /* Scratch for this shape (reads B, M, Hq, Hkv, D, cache.S, causal, and whether `weight` is given). */

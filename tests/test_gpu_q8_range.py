@@ -105,3 +105,35 @@ def test_a_cache_of_zeros_with_scale_zero(M, n, weigh):
     Q._done()
     assert bool((o == 0).all())
     Q._check(o, lse, w, r, q, BF, D, [n], 2)
+
+
+# ---------------------------------------------------------------------------------- probabilities in one part or in two
+
+@pytest.mark.parametrize("single_p", [False, True])
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("M,Hq,Hkv,D,S,block", [
+    (1, 32, 2, 128, 16, 16),                     # a cluster for each unit
+    (3, 16, 1, 64, 64, 32),
+    (8, 16, 2, 128, 9100, 64),                   # pieces
+    (40, 8, 2, 128, 16, 16),                     # tensor-core kernel
+    (40, 8, 2, 64, 700, 64),                     # ... divided
+])
+def test_probabilities_are_two_parts_unless_one_is_asked_for(M, Hq, Hkv, D, S, block, dt, single_p):
+    """Five positions of nearly equal weight whose values cancel in many columns: what the rounding of p leaves there is not
+    hidden by the output's own rounding.  Queries are small, so that the scores' errors are."""
+    n = 5
+    q, kc, vc, ks, vs = Q._attend_inputs(1, M, Hq, Hkv, D, S, block, dt, 83)
+    q = (q.float() * 2.0 ** -7).to(dt)
+    vs[:] = 2.0 ** -6
+    r = O.attend(q, Q._values(kc, ks, block), Q._values(vc, vs, block), [n], False, D ** -0.5)
+    cache, _, _ = Q._cache(kc, vc, ks, vs, block)
+    o = torch.zeros(1, M, Hq, D, dtype=dt, device="cuda")
+    ops.attention_q8(q.cuda(), cache, o, kv_len=torch.tensor([n], dtype=torch.int32).cuda(), causal=False, single_p=single_p)
+    Q._done()
+    # as Q._tolerance, with the rounding of p that was asked for
+    ds = (D + 8) * 2.0 ** -23 * r["T"].transpose(1, 2)[..., None] + 2.0 ** -21
+    e = (o.double().cpu() - r["o"]).abs()
+    near = lambda pe: torch.finfo(dt).eps / 2 * r["o"].abs() + (pe + 2 * ds) * r["A"] + 2.0 ** -25
+    assert bool((e <= near(2.0 ** -11 if single_p else 2.0 ** -19)).all()), (e / near(2.0 ** -19)).max().item()
+    if single_p:
+        assert bool((e > near(2.0 ** -19)).any())          # one part it is

@@ -14,7 +14,7 @@ LIB_NAME = "libtrinity_b200.so"
 # TRINITY_B200_LIB points at another build of the same library (e.g. one compiled with extra -D flags)
 LIB_PATH = Path(os.environ.get("TRINITY_B200_LIB") or (Path(__file__).resolve().parent / LIB_NAME))
 
-ABI_VERSION = 3
+ABI_VERSION = 4
 
 TRN_BF16, TRN_FP16 = 0, 1
 TRN_VANILLA, TRN_PRENORM, TRN_QKNORM, TRN_KEYFORMER, TRN_ROCO = range(5)
@@ -134,7 +134,7 @@ class TrnAttnQ8Args(C.Structure):
         ("weight_stride_b", C.c_int64), ("weight_stride_h", C.c_int64), ("weight_add", C.c_int),
         ("kv_len", C.c_void_p), ("kv_len_all", C.c_int), ("B", C.c_int), ("M", C.c_int), ("Hq", C.c_int),
         ("Hkv", C.c_int), ("D", C.c_int), ("dtype", C.c_int), ("causal", C.c_int), ("scale", C.c_float),
-        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("single_p", C.c_int),
     ]
 
 

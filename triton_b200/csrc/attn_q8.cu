@@ -13,8 +13,8 @@
 //     are smaller by the scales' ratio: with scales 2^26 (attn_q8_tc.cu: 2^20) and more apart these are subnormal in fp16, and such
 //     a column is off by up to 448 * 2^-37 (2^-31) of the row's largest p vs for each position.)
 // P' carries a factor 2^12 into the product (it cancels in O / l), which keeps weights down to 2^-26 of the row's largest out of
-// fp16's subnormals.  bf16 outputs take P' as one fp16 (off by at most 2^-11 of itself, the output's rounding by
-// 2^-8); fp16 outputs take it as hi + lo, since one part alone would err as much as the output's own rounding.
+// fp16's subnormals.  P' goes into the product as two fp16 parts, hi + lo, off by 2^-22 of itself; with single_p as one, off by
+// 2^-11 (the outputs' own rounding: bf16 2^-8, fp16 2^-11).
 //
 // This kernel is for few query rows per kv head: a CTA of four warps owns up to 8 NT of the M * Hq / Hkv rows of a (b, kv head)
 // and a share of its positions; each warp walks its quarter in chunks of 32 positions through its own ring of TMA
@@ -910,11 +910,11 @@ Q8Plan plan_of(const TrnAttnQ8Args& a, int sm_count, bool divide) {
   return w;
 }
 
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, bool HILO>
 int launch_cluster(const TrnAttnQ8Args& a, const Q8Plan& w, const CUtensorMap& tm_k, const CUtensorMap& tm_v, const Q8Params& p,
                    cudaStream_t st, const DeviceState& ds) {
   using SM = Q8Smem<D, NT, 2>;
-  auto kern = attn_q8_cluster_kernel<T, D, NT, Io<T>::kFmt == 0, 2>;
+  auto kern = attn_q8_cluster_kernel<T, D, NT, HILO, 2>;
   const int rc = ensure_dyn_smem(reinterpret_cast<const void*>(kern), SM::kTotalKept, ds.device);
   if (rc != TRN_OK) return rc;
   cudaLaunchConfig_t cfg{};
@@ -935,10 +935,9 @@ int launch_cluster(const TrnAttnQ8Args& a, const Q8Plan& w, const CUtensorMap& t
   return TRN_OK;
 }
 
-template <typename T, int D, int NT, int ST>
-int launch_tiles(const TrnAttnQ8Args& a, const Q8Plan& w, cudaStream_t st, const DeviceState& ds) {
+template <typename T, int D, int NT, int ST, bool HILO>
+int launch_parts(const TrnAttnQ8Args& a, const Q8Plan& w, cudaStream_t st, const DeviceState& ds) {
   using SM = Q8Smem<D, NT, ST>;
-  constexpr bool HILO = Io<T>::kFmt == 0;
   Q8Params p = q8_params(a, ds);
   CUtensorMap tm_k, tm_v;
   int rc = make_code_tmap(&tm_k, &p.ki, a.cache.k, a.cache.S, a.Hkv, a.B, D, kQ8Keys);
@@ -954,7 +953,7 @@ int launch_tiles(const TrnAttnQ8Args& a, const Q8Plan& w, cudaStream_t st, const
   }
   p.pitch = w.pitch;
   if (w.units * max(w.cluster, 1) + w.ctas > 0x7fffffffLL) return TRN_E_SHAPE;
-  if (w.cluster > 0) return launch_cluster<T, D, NT>(a, w, tm_k, tm_v, p, st, ds);
+  if (w.cluster > 0) return launch_cluster<T, D, NT, HILO>(a, w, tm_k, tm_v, p, st, ds);
   auto kern = attn_q8_kernel<T, D, NT, HILO, ST>;
   rc = ensure_dyn_smem(reinterpret_cast<const void*>(kern), SM::kTotal, ds.device);
   if (rc != TRN_OK) return rc;
@@ -962,6 +961,11 @@ int launch_tiles(const TrnAttnQ8Args& a, const Q8Plan& w, cudaStream_t st, const
   TRN_CUDA_TRY(launch_pdl(kern, dim3(grid), dim3(kQ8Threads), SM::kTotal, st, tm_k, tm_v, p));
   if (w.ctas > 0 || a.weight != nullptr) return launch_q8_join(p, a, w.ctas > 0, st);
   return TRN_OK;
+}
+
+template <typename T, int D, int NT, int ST>
+int launch_tiles(const TrnAttnQ8Args& a, const Q8Plan& w, cudaStream_t st, const DeviceState& ds) {
+  return a.single_p != 0 ? launch_parts<T, D, NT, ST, false>(a, w, st, ds) : launch_parts<T, D, NT, ST, true>(a, w, st, ds);
 }
 
 template <typename T, int D>

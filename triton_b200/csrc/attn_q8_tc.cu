@@ -13,7 +13,7 @@
 //                (m' as in attn_q8.cu);  o is rescaled only when a row's maximum grew by more than 2^8 since the last time
 //   warp 3       issues S_t = q_t k^T and O_t += P'_t v (P' from tensor memory)
 // ks enters the multiply-add that the softmax makes anyway, vs costs half a (packed) multiplication a score; both change every
-// 16 columns at most.  bf16 outputs take P' as one fp16 part, fp16 outputs as hi + lo (see attn_q8.cu).
+// 16 columns at most.  P' enters as hi + lo, with single_p as one fp16 part (see attn_q8.cu).
 // Few CTAs (less than one for each SM): the key blocks are divided among several, merged by the kernel in attn_q8.cu.
 //
 // Algorithmic flops: 4 * D per visible (row, position).
@@ -96,13 +96,13 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
 }
 
 // GRP: positions that share a scale within the kernel, 16 or (blocks of 32 and more) 32
-template <typename T, int D, int GRP>
+// SPLIT: P' enters the product as two fp16 parts
+template <typename T, int D, int GRP, bool SPLIT>
 __global__ void __launch_bounds__(kTcThreads, 1)
 attn_q8_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                   const __grid_constant__ TcParams tp) {
   using SM = TcSmem<D>;
   constexpr int KS = SM::kStages;
-  constexpr bool SPLIT = Io<T>::kFmt == 0;
   const Q8Params& p = tp.c;
   extern __shared__ uint8_t tc_smem_raw[];
   const uint32_t base = (smem_u32(tc_smem_raw) + 1023u) & ~1023u;
@@ -726,7 +726,7 @@ TcPlan tc_plan(const TrnAttnQ8Args& a) {
   return w;
 }
 
-template <typename T, int D, int GRP>
+template <typename T, int D, int GRP, bool SPLIT>
 int launch_grp(const TrnAttnQ8Args& a, cudaStream_t st, const DeviceState& ds) {
   using SM = TcSmem<D>;
   TcPlan w = tc_plan(a);
@@ -761,7 +761,7 @@ int launch_grp(const TrnAttnQ8Args& a, cudaStream_t st, const DeviceState& ds) {
   int rc = make_code_tmap(&tm_k, &tp.c.ki, a.cache.k, a.cache.S, a.Hkv, a.B, D, kTcKeys);
   if (rc == TRN_OK) rc = make_code_tmap(&tm_v, &tp.c.vi, a.cache.v, a.cache.S, a.Hkv, a.B, D, kTcKeys);
   if (rc != TRN_OK) return rc;
-  auto kern = attn_q8_tc_kernel<T, D, GRP>;
+  auto kern = attn_q8_tc_kernel<T, D, GRP, SPLIT>;
   rc = ensure_dyn_smem(reinterpret_cast<const void*>(kern), SM::kTotal, ds.device);
   if (rc != TRN_OK) return rc;
   TRN_CUDA_TRY(launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(kTcThreads), SM::kTotal, st, tm_k, tm_v, tp));
@@ -770,7 +770,8 @@ int launch_grp(const TrnAttnQ8Args& a, cudaStream_t st, const DeviceState& ds) {
 
 template <typename T, int D>
 int launch_typed(const TrnAttnQ8Args& a, cudaStream_t st, const DeviceState& ds) {
-  return a.cache.block == 16 ? launch_grp<T, D, 16>(a, st, ds) : launch_grp<T, D, 32>(a, st, ds);
+  if (a.single_p != 0) return a.cache.block == 16 ? launch_grp<T, D, 16, false>(a, st, ds) : launch_grp<T, D, 32, false>(a, st, ds);
+  return a.cache.block == 16 ? launch_grp<T, D, 16, true>(a, st, ds) : launch_grp<T, D, 32, true>(a, st, ds);
 }
 
 }  // namespace

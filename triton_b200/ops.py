@@ -452,11 +452,12 @@ class AttentionQ8Plan(_BoundCall):
     up to kv_len - M + i; a row that sees nothing is 0.  q, o: (b, s, h, d) views.  ``lse`` [B, Hq, M] fp32 (base 2).
     ``weight`` [B, Hkv, S or more] fp32 receives every position's attention weight, summed over the queries (at most 16) and
     the query heads of the kv head (``weight_add``: is increased by it): what CacheEvictPlan selects by.
+    ``single_p``: p enters the product with v as one fp16 part instead of two, as in attention().
     ``workspace``: a uint8 tensor of attention_q8_workspace_bytes(...) bytes; allocated here when not given."""
 
     def __init__(self, q: torch.Tensor, cache: CacheQ8, o: torch.Tensor, *, kv_len, causal: bool = True,
                  scale: Optional[float] = None, lse: Optional[torch.Tensor] = None, weight: Optional[torch.Tensor] = None,
-                 weight_add: bool = False, workspace: Optional[torch.Tensor] = None):
+                 weight_add: bool = False, single_p: bool = False, workspace: Optional[torch.Tensor] = None):
         if q.dim() != 4 or q.shape != o.shape or q.dtype != o.dtype or q.stride(3) != 1 or o.stride(3) != 1:
             raise ValueError("q and o must be (b, s, h, d) views of one shape and dtype with contiguous head_dim")
         B, M, Hq, D = q.shape
@@ -466,6 +467,7 @@ class AttentionQ8Plan(_BoundCall):
         a.q, a.cache, a.o = _head_tensor(q), cache.c(), _head_tensor(o)
         a.B, a.M, a.Hq, a.Hkv, a.D, a.dtype = B, M, Hq, cache.Hkv, D, _dtype_code(q)
         a.causal, a.scale = int(causal), default_scale(D) if scale is None else float(scale)
+        a.single_p = int(single_p)
         if lse is not None:
             if lse.dtype != torch.float32 or lse.shape != (B, Hq, M) or not lse.is_contiguous():
                 raise ValueError("lse must be a contiguous float32 [B, Hq, M] tensor")

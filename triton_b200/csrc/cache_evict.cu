@@ -60,6 +60,9 @@ __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
 // clock: two clusters of 8 CTAs took 30 us for 71 heads of 32768 positions.)  A CTA takes kEvSumKeys positions, each by
 // kEvSumParts threads that share its heads, so that a position's loads are under way together.
 constexpr int kEvSumKeys = 64, kEvSumParts = 4;
+// First head of part q: a position's sum is that of its kEvSumParts parts in order, whichever kernel takes it, so that the result
+// does not depend on whether there is scratch.
+__device__ __forceinline__ int part_begin(int group, int q) { return static_cast<int>(static_cast<long long>(group) * q / kEvSumParts); }
 __global__ void __launch_bounds__(kEvSumKeys * kEvSumParts)
 evict_sum_kernel(const float* __restrict__ scores, long long sc_sb, long long sc_sh, int group, KvLen len, int Hkv, int S, float* __restrict__ out) {
   __shared__ double part[kEvSumParts][kEvSumKeys];
@@ -72,7 +75,7 @@ evict_sum_kernel(const float* __restrict__ scores, long long sc_sb, long long sc
   const bool there = j < len(b);
   double acc = 0.0;
   if (there) {
-    const int g0 = group * q / kEvSumParts, g1 = group * (q + 1) / kEvSumParts;
+    const int g0 = part_begin(group, q), g1 = part_begin(group, q + 1);
     const float* src = scores + b * sc_sb + static_cast<long long>(h) * group * sc_sh + j;
 #pragma unroll 10
     for (int g = g0; g < g1; ++g) acc += static_cast<double>(src[g * sc_sh]);
@@ -118,19 +121,29 @@ evict_select_kernel(const __grid_constant__ EvictParams p, int cluster) {
   if (p.group == 1) {
     for (int j = tid; j < cnt; j += kEvThreads) ev_keys[j] = order_key(sc[j]);
   } else {
-    // kEvAhead positions at a time, so that enough loads are under way: a row's sum is one chain of Hs / Hkv adds
+    // kEvAhead positions at a time, so that enough loads are under way: a row's sum is one chain of Hs / Hkv adds.  (With less
+    // heads than parts no part holds two, and the chain alone has the parts' order.)
+    static_assert(kEvSumParts == 4, "three inner borders");
+    const int e1 = part_begin(p.group, 1), e2 = part_begin(p.group, 2), e3 = part_begin(p.group, 3);
     for (int j0 = tid; j0 < cnt; j0 += kEvAhead * kEvThreads) {
-      double acc[kEvAhead] = {};
+      double acc[kEvAhead] = {}, done[kEvAhead] = {};
 #pragma unroll 6
       for (int g = 0; g < p.group; ++g) {
         const float* src = sc + g * p.sc_sh + j0;
+        if (g == e1 || g == e2 || g == e3) {                     // the part before is complete
+#pragma unroll
+          for (int i = 0; i < kEvAhead; ++i) {
+            done[i] += acc[i];
+            acc[i] = 0.0;
+          }
+        }
 #pragma unroll
         for (int i = 0; i < kEvAhead; ++i)
           if (j0 + i * kEvThreads < cnt) acc[i] += static_cast<double>(src[i * kEvThreads]);
       }
 #pragma unroll
       for (int i = 0; i < kEvAhead; ++i)
-        if (j0 + i * kEvThreads < cnt) ev_keys[j0 + i * kEvThreads] = order_key(static_cast<float>(acc[i]));
+        if (j0 + i * kEvThreads < cnt) ev_keys[j0 + i * kEvThreads] = order_key(static_cast<float>(done[i] + acc[i]));
     }
   }
   if (tid < 256) hist[0][tid] = 0u;

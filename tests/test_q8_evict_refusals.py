@@ -1,0 +1,41 @@
+"""What eviction refuses beside what test_q8_refusals.py holds: no GPU needed."""
+import ctypes as C
+
+import pytest
+
+import test_q8_refusals as R
+from test_q8_refusals import lib  # noqa: F401  (fixture)
+
+# scores of _evict: 2 items x 8 heads x 256 positions of 4 bytes from 3 << 32; idx: 2 x 2 x 100 from 4 << 32
+SCORES, END = 3 << 32, (3 << 32) + 2 * 8 * 256 * 4
+
+
+@pytest.mark.parametrize("change", [
+    dict(scores_out=SCORES),                                       # compaction in place
+    dict(scores_out=END - 4),
+    dict(scores_out=SCORES - 2 * 2 * 100 * 4 + 4),
+    dict(idx=SCORES + 4096),
+    dict(kv_len_out=SCORES + 8),
+    dict(idx=7 << 32, kv_len=(7 << 32) + 16),
+    dict(scores_out=(4 << 32) + 400),                              # over idx
+    dict(scores_out=5 << 32, kv_len_out=(5 << 32) + 4),
+    dict(Hs=258, score_stride_b=258 * 256, workspace=SCORES + 256, workspace_bytes=1 << 30),
+    dict(Hs=258, score_stride_b=258 * 256, workspace=(4 << 32) - 256, workspace_bytes=1 << 30),
+])
+def test_results_over_what_is_read_or_over_one_another(lib, change):  # noqa: F811
+    assert lib.trinity_cache_evict(C.byref(R._evict(**change)), None) == R.VARIANT
+
+
+@pytest.mark.parametrize("change", [
+    dict(scores_out=END, kv_len=5 << 32, kv_len_out=6 << 32),      # side by side
+    dict(idx=SCORES - 2 * 2 * 100 * 4),
+    dict(kv_len=7 << 32, kv_len_out=(7 << 32) + 8),
+    dict(scores_out=(4 << 32) + 1600),
+    dict(workspace=SCORES + 256, workspace_bytes=1 << 30),         # this shape uses none
+])
+def test_neighbours_are_not_refused(lib, change):  # noqa: F811
+    """Judged as fit: what answers then is the missing GPU."""
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("the pointers are not memory")
+    assert lib.trinity_cache_evict(C.byref(R._evict(**change)), None) in (-7, -8)

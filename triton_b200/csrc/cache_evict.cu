@@ -394,10 +394,17 @@ int check_cache_evict(const TrnCacheEvictArgs& a) {
     if (rc == TRN_OK) rc = check_scales(a.dst.v_scale, a.B, (a.keep - 1) / a.src.block + 1, a.Hkv);
     if (rc != TRN_OK) return rc;
   }
-  // rows move in parallel: a destination inside the source's range could be overwritten before it is read.  The lengths
-  // are read throughout both launches.
-  if (a.kv_len != nullptr && a.kv_len_out != nullptr && a.kv_len_out < a.kv_len + a.B && a.kv_len < a.kv_len_out + a.B)
-    return TRN_E_VARIANT;
+  // rows move in parallel: a destination inside the source's range could be overwritten before it is read.
+  // Positions, scores and lengths of the result, and the scratch, are written while other rows' scores and lengths are read.
+  const int64_t kept = static_cast<int64_t>(a.B) * a.Hkv * a.keep;
+  const struct { const void* ptr; int64_t bytes; } area[6] = {
+      {a.scores, ((a.B - 1) * a.score_stride_b + (a.Hs - 1) * a.score_stride_h + a.src.S) * 4}, {a.kv_len, a.B * 4LL}, {a.idx, kept * 4},
+      {a.scores_out, kept * 4}, {a.kv_len_out, a.B * 4LL}, {a.workspace, static_cast<int64_t>(cache_evict_workspace(a))}};
+  for (int i = 0; i < 6; ++i)
+    for (int j = max(i + 1, 2); j < 6; ++j) {
+      const uintptr_t l0 = reinterpret_cast<uintptr_t>(area[i].ptr), l1 = reinterpret_cast<uintptr_t>(area[j].ptr);
+      if (l0 != 0 && l1 != 0 && area[j].bytes > 0 && l0 < l1 + area[j].bytes && l1 < l0 + area[i].bytes) return TRN_E_VARIANT;
+    }
   for (int i = 0; i < 2; ++i)
     for (int j = 2; j < 4; ++j) {
       uintptr_t l0, h0, l1, h1;

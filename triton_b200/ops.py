@@ -507,7 +507,8 @@ class CacheEvictPlan(_BoundCall):
     block size, or (k, v) pairs of 16-bit (b, s, h, d) views of one dtype; they must not overlap.
     ``idx`` [B, Hkv, keep] int32: the positions kept, ascending, then -1.  ``scores_out`` [B, Hkv, keep] fp32: their scores,
     then 0 (the accumulators of the cache they moved to).  ``kv_len_out`` [B] int32: min(kv_len, keep).  ``workspace``: a uint8
-    tensor for the sums of long rows with several score heads (see trinity_cache_evict_workspace); allocated when not given."""
+    tensor for the sums of long rows with several score heads (see trinity_cache_evict_workspace); allocated when not given.
+    ``idx``, ``scores_out`` and ``kv_len_out`` overlap neither ``scores`` and ``kv_len`` nor one another."""
 
     def __init__(self, src, dst, scores: torch.Tensor, *, kv_len, keep: int, recent: int = 0, first: int = 0,
                  idx: Optional[torch.Tensor] = None, scores_out: Optional[torch.Tensor] = None,

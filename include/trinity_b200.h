@@ -380,7 +380,8 @@ size_t trinity_attention_q8_workspace(const TrnAttnQ8Args* a);
  * 16-bit elements and rows are copied.  src.block must equal dst.block.
  * idx [B, Hkv, keep] receives the positions, ascending, -1 behind the last; scores_out (optional) their fp32 scores, 0
  * behind the last; kv_len_out (optional) [B] min(n, keep).  These three and the scratch overlap neither scores and kv_len nor one
- * another (accumulators are compacted to another array, not in place).  recent + first <= keep; src.S <= 262144; D is 64 or 128. */
+ * another (accumulators are compacted to another array, not in place).  recent + first <= keep <= 2^29; src.S <= 262144; D is 64 or
+ * 128. */
 typedef struct {
   TrnCacheQ8 src, dst;
   const float* scores;            /* fp32 (b, hs, j), j contiguous */

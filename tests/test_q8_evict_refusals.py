@@ -39,3 +39,11 @@ def test_neighbours_are_not_refused(lib, change):  # noqa: F811
     if torch.cuda.is_available():
         pytest.skip("the pointers are not memory")
     assert lib.trinity_cache_evict(C.byref(R._evict(**change)), None) in (-7, -8)
+
+
+@pytest.mark.parametrize("keep", [2 ** 29 + 1, 2 ** 31 - 1000, 2 ** 31 - 1])
+def test_more_rows_to_keep_than_32_bit_steps_reach(lib, keep):  # noqa: F811
+    """A destination with room for 2^31 rows: the loop that marks the unused ones steps past the largest int."""
+    assert lib.trinity_cache_evict(C.byref(R._evict(keep=keep, dst__S=keep, dst__k__stride_b=2 ** 40, dst__v__stride_b=2 ** 40, dst__k__stride_h=2 ** 38,
+                                                    dst__v__stride_h=2 ** 38, dst__k__ptr=1 << 48, dst__v__ptr=1 << 49, dst__k_scale__ptr=1 << 50,
+                                                    dst__v_scale__ptr=1 << 51, idx=1 << 52)), None) == R.SHAPE

@@ -376,7 +376,7 @@ int check_cache_evict(const TrnCacheEvictArgs& a) {
   if (a.B <= 0 || a.Hkv <= 0 || a.Hs <= 0 || a.Hs % a.Hkv != 0) return TRN_E_SHAPE;
   if (a.D != 64 && a.D != 128) return TRN_E_SHAPE;
   if (a.keep <= 0 || a.recent < 0 || a.first < 0 || a.recent > a.keep || a.first > a.keep - a.recent) return TRN_E_SHAPE;
-  if (a.src.S <= 0 || a.src.S > kEvMaxN || a.dst.S < a.keep) return TRN_E_SHAPE;
+  if (a.src.S <= 0 || a.src.S > kEvMaxN || a.dst.S < a.keep || a.keep > kMaxPositions) return TRN_E_SHAPE;
   if (a.score_stride_b < 0 || a.score_stride_h < 0) return TRN_E_SHAPE;
   const bool q8 = a.src.block != 0;
   const TrnHeadTensor* t[4] = {&a.src.k, &a.src.v, &a.dst.k, &a.dst.v};

@@ -389,9 +389,11 @@ class _BoundCall:
     """Arguments of one C-ABI call bound once (pointers, strides, workspace), launched many times on the current stream of
     the tensors' device.  Construction validates and allocates; ``run()`` only launches, so it can be captured in a CUDA graph.
     The tensors (lengths included) are read and written in place at every run; two runs of ONE plan that overlap on the GPU
-    (different streams) share its workspace and outputs and must be ordered by the caller."""
+    (different streams) share its workspace and outputs and must be ordered by the caller.  What the plan allocated itself stays
+    until the work on it is done, on whichever stream it ran, also if the plan is dropped before; a captured graph needs its plan
+    for as long as it is replayed."""
 
-    def _bind(self, name: str, args, keep) -> None:
+    def _bind(self, name: str, args, keep, own=()) -> None:
         self._keep = [t for t in keep if t is not None]
         _one_device(*self._keep)
         self._index = self._keep[0].device.index
@@ -400,13 +402,21 @@ class _BoundCall:
         self._fn = getattr(L.load(), name)
         # the raw-handle forms of current_device() and current_stream(): a decode step is a few microseconds of work
         self._get_device, self._get_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+        # tensors allocated here belong to the stream that is current now; others that run the plan are made known to the allocator
+        self._own = [t for t in own if t is not None]
+        self._streams = {self._get_stream(self._index)}
 
     def run(self) -> None:
+        stream = self._get_stream(self._index)
+        if stream not in self._streams:
+            for t in self._own:
+                t.record_stream(torch.cuda.current_stream(self._index))
+            self._streams.add(stream)
         if self._get_device() == self._index:
-            rc = self._fn(self._ref, self._get_stream(self._index))
+            rc = self._fn(self._ref, stream)
         else:
             with torch.cuda.device(self._index):
-                rc = self._fn(self._ref, self._get_stream(self._index))
+                rc = self._fn(self._ref, stream)
         if rc != 0:
             L.check(rc)
 
@@ -481,14 +491,16 @@ class AttentionQ8Plan(_BoundCall):
             a.weight, a.weight_stride_b, a.weight_stride_h = weight.data_ptr(), weight.stride(0), weight.stride(1)
             a.weight_add = int(weight_add)
         keep = _set_kv_len(a, kv_len, B, cache.S)
+        own = []
         if workspace is None:
             nbytes = L.load().trinity_attention_q8_workspace(C.byref(a))
             workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+            own.append(workspace)
         if workspace is not None:
             if not workspace.is_contiguous():
                 raise ValueError("workspace must be contiguous")
             a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-        self._bind("trinity_attention_q8", a, keep + cache.tensors() + [q, o, lse, weight, workspace])
+        self._bind("trinity_attention_q8", a, keep + cache.tensors() + [q, o, lse, weight, workspace], own)
 
 
 def attention_q8_workspace_bytes(B: int, M: int, Hq: int, Hkv: int, D: int, S: int, *, causal: bool = True,
@@ -538,7 +550,10 @@ class CacheEvictPlan(_BoundCall):
         if scores.dtype != torch.float32 or scores.dim() != 3 or scores.shape[0] != B or scores.shape[1] % Hkv != 0 or \
                 scores.shape[1] == 0 or scores.shape[2] < S or (scores.shape[2] > 1 and scores.stride(2) != 1):
             raise ValueError("scores must be float32 [B, a multiple of Hkv heads, positions of src], positions contiguous")
-        idx = torch.empty(B, Hkv, keep, dtype=torch.int32, device=k.device) if idx is None else idx
+        own = []
+        if idx is None:
+            idx = torch.empty(B, Hkv, keep, dtype=torch.int32, device=k.device)
+            own.append(idx)
         for t, dt, shape in ((idx, torch.int32, (B, Hkv, keep)), (scores_out, torch.float32, (B, Hkv, keep)),
                              (kv_len_out, torch.int32, (B,))):
             if t is not None and (t.dtype != dt or t.shape != shape or not t.is_contiguous()):
@@ -553,11 +568,12 @@ class CacheEvictPlan(_BoundCall):
         if workspace is None:
             nbytes = L.load().trinity_cache_evict_workspace(C.byref(a))
             workspace = torch.empty(nbytes, dtype=torch.uint8, device=k.device) if nbytes else None
+            own.append(workspace)
         if workspace is not None:
             if not workspace.is_contiguous():
                 raise ValueError("workspace must be contiguous")
             a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-        self._bind("trinity_cache_evict", a, keep_alive + [scores, idx, scores_out, kv_len_out, workspace])
+        self._bind("trinity_cache_evict", a, keep_alive + [scores, idx, scores_out, kv_len_out, workspace], own)
 
 
 def cache_append(cache: CacheQ8, k: torch.Tensor, v: torch.Tensor, *, kv_len) -> None:

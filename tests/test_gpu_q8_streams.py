@@ -1,4 +1,4 @@
-"""Plans of the 8-bit cache on streams other than the one they were made on."""
+"""Plans (of the 8-bit cache, and of the block) on streams other than the one they were made on."""
 import pytest
 import torch
 
@@ -23,7 +23,14 @@ def _evict():
     return lambda: ops.CacheEvictPlan((k, k), (to, to.clone()), scores, kv_len=9000, keep=500)
 
 
-@pytest.mark.parametrize("make", [_attend, _evict])
+def _block():
+    B, M, P, H, D = 1, 64, 2000, 8, 128
+    q, o = (torch.randn(B, M, H, D, device="cuda").to(BF) for _ in range(2))
+    k, v = (torch.randn(B, P + M, H, D, device="cuda").to(BF) for _ in range(2))
+    return lambda: ops.BlockPlan("vanilla", B=B, M=M, P=P, Hq=H, Hkv=H, D=D, q=q, k_cache=k, v_cache=v, o=o, scale=D ** -0.5)
+
+
+@pytest.mark.parametrize("make", [_attend, _evict, _block])
 def test_scratch_of_a_dropped_plan_waits_for_the_stream_that_used_it(make):
     """Made on one stream, run on another that is still busy, dropped: the scratch is not handed out again meanwhile."""
     build = make()

@@ -299,9 +299,17 @@ class BlockPlan:
         a.workspace, a.workspace_bytes = self._ws.data_ptr(), self._ws.numel()
         self.args = a
         self._lib = lib
+        # streams that the allocator knows to use what was allocated here: the one current now, and those that ran the plan
+        self._streams = {torch.cuda.current_stream(q.device).cuda_stream}
 
     def run(self) -> None:
-        L.check(self._lib.trinity_attn_block(C.byref(self.args), _stream()))
+        stream = torch.cuda.current_stream()
+        if stream.cuda_stream not in self._streams:
+            for t in (self._ws, getattr(self, "_x_norm", None)):
+                if t is not None:
+                    t.record_stream(stream)
+            self._streams.add(stream.cuda_stream)
+        L.check(self._lib.trinity_attn_block(C.byref(self.args), stream.cuda_stream))
 
     def run_host(self, x_host: torch.Tensor, o_host: torch.Tensor, sum_p_host: Optional[torch.Tensor] = None,
                  sum_p2_host: Optional[torch.Tensor] = None) -> None:

@@ -137,3 +137,72 @@ def test_probabilities_are_two_parts_unless_one_is_asked_for(M, Hq, Hkv, D, S, b
     assert bool((e <= near(2.0 ** -11 if single_p else 2.0 ** -19)).all()), (e / near(2.0 ** -19)).max().item()
     if single_p:
         assert bool((e > near(2.0 ** -19)).any())          # one part it is
+
+
+# ------------------------------------------------------------------------------------------------- queries and variants
+
+@pytest.mark.parametrize("M,Hq,D,n,block,dt", [(6, 2, 64, 100, 16, HF), (40, 2, 128, 100, 16, BF), (40, 2, 64, 333, 32, HF), (200, 1, 128, 513, 32, BF),
+                                               (200, 2, 64, 2100, 16, HF), (40, 3, 64, 140, 64, BF)])
+def test_queries_that_are_not_finite_or_extreme(M, Hq, D, n, block, dt):
+    """A row of q with an infinite or NaN element is NaN throughout and leaves its neighbours alone; tiny rows, rows of zeros, elements
+    far below their row's largest: one head's rows 1 to 5, and rows near the end of a call of many."""
+    q, kc, vc, ks, vs = Q._attend_inputs(1, M, Hq, 1, D, n, block, dt, 6)
+    bad = torch.zeros(M, Hq, dtype=torch.bool)
+    for r0 in {0, M - 6}:
+        q[0, r0 + 1, 0, 3] = math.inf
+        q[0, r0 + 2, Hq - 1, 7] = math.nan
+        q[0, r0 + 3, 0] *= 2.0 ** (-120 if dt == BF else -20)
+        q[0, r0 + 4, 0] = 0.0
+        q[0, r0 + 5, Hq - 1, 0] = 2.0 ** (-60 if dt == BF else -22)
+        bad[r0 + 1, 0] = bad[r0 + 2, Hq - 1] = True
+    clean = torch.where(q.isfinite(), q, torch.zeros_like(q))
+    r = O.attend(clean, Q._values(kc, ks, block), Q._values(vc, vs, block), [n], True, D ** -0.5)
+    r["o"][0][bad] = math.nan
+    r["lse"][0][bad.T] = math.nan
+    cache, _, _ = Q._cache(kc, vc, ks, vs, block)
+    o, lse = torch.zeros(1, M, Hq, D, dtype=dt, device="cuda"), torch.zeros(1, Hq, M, device="cuda")
+    ops.attention_q8(q.cuda(), cache, o, kv_len=n, lse=lse)
+    Q._done()
+    Q._check(o, lse, None, r, clean, dt, D, [n], Hq)
+
+
+VARIANTS = [
+    # B, M, Hq, Hkv, D, S, lens, block, causal: one line for each form of the kernels
+    (2, 2, 4, 1, 128, 300, [300, 77], 64, True),            # clusters: 8 rows, 16 rows, at head_dim 64 also 32
+    (2, 4, 4, 1, 128, 300, [299, 3], 16, True),
+    (2, 2, 4, 1, 64, 300, [300, 77], 64, True),
+    (2, 4, 4, 1, 64, 300, [299, 3], 16, True),
+    (2, 8, 4, 1, 64, 300, [299, 5], 32, True),
+    (40, 1, 4, 4, 128, 1200, None, 32, True),               # shares, many units: two stages
+    (2, 1, 4, 1, 128, 9100, [9100, 2], 128, True),          # few units: three
+    (1, 3, 4, 1, 128, 9100, [9000], 16, True),
+    (1, 2, 4, 1, 64, 9100, [9000], 16, True),
+    (1, 3, 4, 1, 64, 9100, [9000], 16, True),
+    (1, 8, 4, 1, 64, 9100, [9000], 16, True),
+    (2, 40, 4, 2, 128, 300, [300, 41], 16, True),           # tensor-core kernel, scales of 16 and of 32 positions
+    (2, 40, 4, 2, 128, 300, [300, 41], 32, True),
+    (2, 40, 4, 2, 64, 300, [300, 41], 16, False),
+    (2, 40, 4, 2, 64, 300, [300, 41], 128, True),
+    (1, 40, 4, 2, 128, 2000, [1999], 16, True),             # ... divided
+    (4, 257, 40, 8, 64, 5200, [0, 300, 257, 5200], 16, True),       # ... the last round in pieces
+    (3, 257, 34, 17, 128, 5130, [5129, 258, 1], 32, True),
+]
+
+
+@pytest.mark.parametrize("single_p", [False, True])
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("B,M,Hq,Hkv,D,S,lens,block,causal", VARIANTS)
+def test_every_form_of_the_kernels(B, M, Hq, Hkv, D, S, lens, block, causal, dt, single_p):
+    lens = [(i * 997) % (S + 1) for i in range(B)] if lens is None else lens
+    q, kc, vc, ks, vs = Q._attend_inputs(B, M, Hq, Hkv, D, S, block, dt, 91)
+    Q._spoil_behind(kc, vc, ks, vs, lens, block)
+    o, lse, w, r = _call(q, kc, vc, ks, vs, lens, block, causal=causal, weigh=False, single_p=single_p)
+    tol, ds = Q._tolerance(r, q, dt, D)
+    if single_p:                                 # one part of p: off by 2^-11 of itself
+        tol = tol + 2.0 ** -11 * r["A"]
+    e = (o.double().cpu() - r["o"]).abs()
+    assert bool((e <= tol).all()), (e / tol).max().item()
+    far = r["lse"].isfinite()
+    e = (lse.double().cpu() - r["lse"]).abs()
+    assert torch.equal(lse.cpu() == -math.inf, ~far)
+    assert bool((e <= ds[..., 0].transpose(1, 2) * 1.5 + 2.0 ** -21 * (1 + r["lse"].abs()))[far].all())

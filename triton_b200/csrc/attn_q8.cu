@@ -695,6 +695,8 @@ constexpr int kQ8JoinWarps = kQ8JoinThreads / 32;
 // rows' sums weighs more (64 rows of 8 x 8 heads, 4096 positions: 133, 103), so there 128, unless those CTAs are fewer than the
 // SMs (142 rows of one head, 2000 positions: 21.2, 26.1); 32 rows and fewer gain nothing there either (20 rows of 8 heads,
 // 2000 positions: 24.1, 21.5).
+// The border between the two forms: 16 rows of 8 heads, 8192 positions 35.5 us with the threads for positions, 31.5 shared; eight such
+// sequences 75.3, 82.2; 12 rows of 2 heads, 40000 positions 28.9, 55.1; 20 and 32 rows of 8 heads, 8192 positions 41.7, 33.4 and 51.2, 35.3.
 constexpr int kQ8FewRows = 16, kQ8JoinKeys = 8 * kQ8JoinThreads, kQ8JoinKeysRows = 128, kQ8JoinKeysShort = 32, kQ8RowsShort = 256;
 // maximum and sum of a row over its pieces by one warp; at: the row in the first piece's slot
 __device__ __forceinline__ float2 join_ml(const Q8Params& p, long long at, int here, int lane) {

@@ -37,10 +37,15 @@ static_assert(kTcConvert == 32 * kTcMmaWarp && kTcThreads == 32 * (kTcMmaWarp + 
 constexpr int kTcTmemCols = 512;              // S0 [0,128) S1 [128,256) O0 [256,256+D) O1 [384,384+D)
 constexpr float kTcRescale = 8.0f;            // log2 units a row's maximum may pass the offset in use
 constexpr float kTcPBias = 6.0f;              // P' <= 2^14 with it
-constexpr int kTcMaxRounds = 8, kTcMaxCut = 8;
+// Pieces of a pair at most.  One round and 4 pairs without a mask, 6144 positions: 153 us with 16, 160 with 8; and 12 pairs 156, 159;
+// more pairs than that leave room for 8 or less
+constexpr int kTcMaxCut = 16;
 // 512 pairs without a mask: 16 key blocks 200 us whole, 213 with the last round in pieces; 32: 359, 357; 64: 677, 647
 constexpr int kTcMinCutBlocks = 40;
-constexpr int kTcMinShare = 2;                // key blocks a CTA takes at least where they are divided
+// Key blocks of a pair from which on few pairs are divided, down to one a CTA.  40 queries of 8 heads of 128 on 8: 3 blocks 17.2 us
+// whole, 18.7 divided; 4 blocks 19.7 and 18.9 (21.9 with two a CTA at least); 8 blocks 26.8 and 18.8 (22.6); 71 heads of 64 x 16
+// queries on one: 3 blocks 15.8, 18.7; 9 blocks 24.9, 19.5 (23.0); from 24 blocks on one and two are alike
+constexpr int kTcMinDivide = 4;
 
 struct TcParams {
   Q8Params c;
@@ -182,7 +187,7 @@ attn_q8_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     unsigned sum = 0u;
     for (int i = lane; i < p.B; i += 32) sum += blocks_of(i);
     const int total = static_cast<int>(__reduce_add_sync(0xffffffffu, sum)) * per;
-    int share = max((total + tp.ctas - 1) / tp.ctas, kTcMinShare);
+    int share = max((total + tp.ctas - 1) / tp.ctas, 1);
     for (;;) {
       unsigned c = 0u;
       for (int i = lane; i < p.B; i += 32) c += (blocks_of(i) + share - 1) / share;
@@ -693,7 +698,7 @@ struct TcPlan {
   size_t ml_off, o_off, piece_off, total;
 };
 
-// key blocks divided among one CTA for each SM where that is at least two CTAs a pair and two blocks a CTA
+// key blocks divided among one CTA for each SM where that is at least two CTAs a pair
 TcPlan tc_plan(const TrnAttnQ8Args& a) {
   TcPlan w{};
   const int R = a.M * (a.Hq / a.Hkv);
@@ -703,17 +708,18 @@ TcPlan tc_plan(const TrnAttnQ8Args& a) {
   const int longest = a.kv_len != nullptr ? a.cache.S : min(max(a.kv_len_all, 1), a.cache.S);
   const int blocks = (longest - 1) / kTcKeys + 1;
   size_t rows;
-  if (2 * pairs <= kAttnNominalSMs && blocks >= 2 * kTcMinShare) {
-    w.ctas = static_cast<int>(min(static_cast<long long>(kAttnNominalSMs), pairs * ((blocks + kTcMinShare - 1) / kTcMinShare)));
+  if (2 * pairs <= kAttnNominalSMs && blocks >= kTcMinDivide) {
+    w.ctas = static_cast<int>(min(static_cast<long long>(kAttnNominalSMs), pairs * blocks));
     rows = 2 * static_cast<size_t>(pairs + w.ctas) * kTcRows;
   } else {
     // Whole rounds of CTAs, and a last one that would leave most SMs idle: its pairs are cut into pieces that fill it (512
-    // pairs: 3 rounds and 68 pairs in two pieces each, instead of 4 rounds)
+    // pairs: 3 rounds and 68 pairs in two pieces each, instead of 4 rounds).  256 queries a pair, 6144 positions, whole / pieces: 1 round
+    // and 20 pairs 246 / 167 us, 8 and 20 1088 / 1029, 12 and 8 1566 / 1499, 12 and 72 1577 / 1578 (causal 1602 / 1614)
     w.whole = static_cast<int>(min(pairs, 0x7fffffffLL));
     w.cut = 1;
     const long long rest = pairs % kAttnNominalSMs, rounds = pairs / kAttnNominalSMs;
-    if (rest == 0 || rounds == 0 || rounds > kTcMaxRounds || blocks < kTcMinCutBlocks) return w;
-    const int cut = static_cast<int>(min(min(kAttnNominalSMs / rest, static_cast<long long>(blocks / kTcMinShare)), static_cast<long long>(kTcMaxCut)));
+    if (rest == 0 || rounds == 0 || blocks < kTcMinCutBlocks) return w;
+    const int cut = static_cast<int>(min(kAttnNominalSMs / rest, static_cast<long long>(kTcMaxCut)));
     if (cut < 2) return w;
     w.cut = cut;
     w.whole = static_cast<int>(pairs - rest);

@@ -326,7 +326,9 @@ typedef struct {
 int trinity_cache_append(const TrnCacheAppendArgs* a, void* cuda_stream);
 
 /* Read: code * scale, rounded to `dtype`, of positions [0, kv_len[b]) into k_out / v_out; the rest of these is left as
- * it is.  Hands an 8-bit cache to the operators that take 16-bit ones (exact in bf16 for power-of-two scales). */
+ * it is.  Hands an 8-bit cache to the operators that take 16-bit ones (exact in bf16 for power-of-two scales).  The largest
+ * elements of a type may have been rounded up past its largest number and come back as infinite: fp16 from 63488 on, bf16 from
+ * 1.9375 * 2^127 on. */
 typedef struct {
   TrnCacheQ8 cache;
   TrnHeadTensor k_out, v_out;     /* s in [0, min(kv_len[b], S_out)) */
@@ -344,7 +346,13 @@ int trinity_cache_read(const TrnCacheReadArgs* a, void* cuda_stream);
  *   weight (optional): weight[b, h, j] = (weight_add ? weight[b, h, j] : 0) + sum over the queries and the query heads
  *   of kv head h of p_j, for j < kv_len[b]; the rest is left as it is.  It is what trinity_cache_evict selects by.
  *   Fixed summation order: results are bitwise reproducible.
- * Any Hq that is a multiple of Hkv, any M >= 1, D 64 or 128; at most 16 queries (M) with `weight`. */
+ * Any Hq that is a multiple of Hkv, any M >= 1, D 64 or 128, scale positive and finite.  With `weight` at most 16 queries (M)
+ * and at most 8192 rows a kv head (M * Hq / Hkv); except for short caches the scores of all rows are then kept in the scratch, which
+ * grows with the room of the cache, whatever its sequences hold: B * Hq * M * S * 4 bytes (537 MB for 2 x 16 queries of 32 heads
+ * on 131072 positions) beside partial results of a few MB.
+ * Accuracy: sums are taken in 32 bits; the products p v in fp16 relative to the row's largest p * v_scale, so a column whose
+ * values all lie in blocks of scales 2^20 and more below that is less accurate than the others (off by up to 2^-22 of that largest
+ * product for each position). */
 typedef struct {
   TrnHeadTensor q;                /* s in [0,M) */
   TrnCacheQ8 cache;

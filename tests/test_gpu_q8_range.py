@@ -206,3 +206,25 @@ def test_every_form_of_the_kernels(B, M, Hq, Hkv, D, S, lens, block, causal, dt,
     e = (lse.double().cpu() - r["lse"]).abs()
     assert torch.equal(lse.cpu() == -math.inf, ~far)
     assert bool((e <= ds[..., 0].transpose(1, 2) * 1.5 + 2.0 ** -21 * (1 + r["lse"].abs()))[far].all())
+
+
+def test_the_largest_numbers_of_a_type_come_back_rounded():
+    """fp16 up to 63487 and bf16 under 1.9375 * 2^127 stay finite through append and read; above, the nearest code is a power of two
+    past the type's largest number."""
+    for dt, below, above in ((HF, 63456.0, 63488.0), (BF, 1.9296875 * 2.0 ** 127, 1.9375 * 2.0 ** 127)):
+        x = torch.zeros(1, 2, 1, 64, dtype=dt)
+        x[0, 0], x[0, 1, 0, ::2] = below, above
+        cache = ops.CacheQ8.empty(1, 16, 1, 64, block=16)
+        out = torch.zeros(1, 2, 1, 64, dtype=dt, device="cuda")
+        ops.cache_append(cache, x.cuda(), x.cuda(), kv_len=0)
+        ops.cache_read(cache, out, out.clone(), kv_len=2)
+        Q._done()
+        assert bool(out[0, 0].isfinite().all()) and bool(out[0, 1, 0, ::2].isinf().all()) and bool((out[0, 1, 0, 1::2] == 0).all())
+
+
+@pytest.mark.parametrize("M", [2, 16])
+def test_weights_where_the_products_are_in_one_part(M):
+    """Weights come from the scores: they do not depend on single_p."""
+    q, kc, vc, ks, vs = Q._attend_inputs(1, M, 8, 2, 128, 2100, 32, BF, 97)
+    ws = [_call(q, kc, vc, ks, vs, [2099], 32, weigh=True, single_p=sp)[2] for sp in (False, True)]
+    assert torch.equal(*ws)

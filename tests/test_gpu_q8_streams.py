@@ -70,3 +70,29 @@ def test_one_plan_on_several_streams_in_turn():
         s.synchronize()
         assert torch.equal(got, alone)
     Q._done()
+
+
+@pytest.mark.parametrize("S", [600, 9000])
+def test_a_captured_plan_with_scratch_of_its_own(S):
+    """Made outside, captured on the capture's stream, replayed on another, graph and plan dropped: what comes after is sound."""
+    q, kc, vc, ks, vs = Q._attend_inputs(2, 1, 8, 2, 64, S, 64, BF, 37)
+    cache, _, _ = Q._cache(kc, vc, ks, vs, 64)
+    qd, o, w = q.cuda(), torch.zeros(q.shape, dtype=BF, device="cuda"), torch.zeros(2, 2, S, device="cuda")
+    want_w = torch.zeros_like(w)
+    want = ops.attention_q8(qd, cache, kv_len=S, weight=want_w)
+    plan = ops.AttentionQ8Plan(qd, cache, o, kv_len=S, weight=w)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan.run()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            graph.replay()
+    Q._done()
+    assert torch.equal(o, want) and torch.equal(w, want_w)
+    del graph, plan
+    other = [torch.full((1 << 20,), 7, dtype=torch.uint8, device="cuda") for _ in range(8)]
+    again = ops.attention_q8(qd, cache, kv_len=S)
+    Q._done()
+    assert torch.equal(again, want) and all(bool((t == 7).all()) for t in other)

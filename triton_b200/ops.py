@@ -469,7 +469,8 @@ class AttentionQ8Plan(_BoundCall):
     """o = softmax(scale * q k^T) v over the first ``kv_len`` positions of an 8-bit cache; causal: query i of M sees positions
     up to kv_len - M + i; a row that sees nothing is 0.  q, o: (b, s, h, d) views.  ``lse`` [B, Hq, M] fp32 (base 2).
     ``weight`` [B, Hkv, S or more] fp32 receives every position's attention weight, summed over the queries (at most 16) and
-    the query heads of the kv head (``weight_add``: is increased by it): what CacheEvictPlan selects by.
+    the query heads of the kv head (at most 8192 rows in all; ``weight_add``: is increased by it): what CacheEvictPlan selects by.
+    Unless the cache is short its scratch then holds every row's scores, 4 * B * M * Hq * S bytes.
     ``single_p``: p enters the product with v as one fp16 part instead of two, as in attention().
     ``workspace``: a uint8 tensor of attention_q8_workspace_bytes(...) bytes; allocated here when not given."""
 

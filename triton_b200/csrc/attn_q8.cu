@@ -29,10 +29,10 @@
 // the pieces and sums the per-position weights from scores kept in the workspace.  Short ones: a cluster per unit meets in
 // shared memory, one launch.  Pieces, rows and sums are taken in a fixed order: bitwise reproducible.
 //
-// Measured: 2 sequences of 100001 and 131071 positions, 32 / 8 heads of 128, fp16 (473 MB): 82 us = 5.7 TB/s, 89 % of the copy
-// rate, 87 us with the merge; 32 of 1000..8192 with weights, bf16 (307 MB): 75 us, 66 without weights (4.5 TB/s: a CTA
-// ends one unit and begins the next with an empty ring); one of 1040: 8.2 us, launch and the chain length -> tile -> scores ->
-// product -> cluster.
+// Measured (calls one behind another on inputs that change; 5 to 10 % more on other machines): 2 sequences of 100001 and 131071
+// positions, 32 / 8 heads of 128, fp16 (473 MB): 88 us = 5.4 TB/s, 83 % of the copy rate, of which the merge 5 us; 32 of 1000..8192
+// with weights, bf16 (307 MB): 79 us, 66 without (4.7 TB/s: a CTA ends one unit and begins the next with an empty ring); one of
+// 1040: 9.1 us, launch and the chain length -> tile -> scores -> product -> cluster.
 //
 // What must not be seen cannot hurt: scores behind a row's last position are replaced, not weighted, and in the
 // chunks where that happens NaN codes of v are taken as 0 in the product (0 * NaN would poison rows that do not see them) and
@@ -51,8 +51,9 @@ constexpr int kQ8MaxCluster = 8;
 constexpr int kQ8Keep = 4;                     // chunks a warp of a cluster takes at most
 // Stages of a warp's ring, and how many CTAs an SM then has room for.  Three CTAs of two stages where units are many (a CTA
 // ends one and begins others, while the rest of the SM keeps loading); two CTAs of three stages where a unit lies on
-// two CTAs and more.  Measured at head_dim 128 (us, bf16): 256 units of 1000..8192 positions 66.0 against 71.2; 16 units of
-// 100001..131071 92.1 against 85.1; 128 units of 16384 100.2 against 94.1.  Head_dim 64 keeps the first (26.9 against 31.9).
+// two CTAs and more.  Measured at head_dim 128 (us, bf16), two stages and three: 256 units of 1000..8192 positions 66.4, 71.4; 16 units
+// of 100001..131071 92.0, 86.6; 128 units of 16384 100.0, 97.0; 152 of these 117, 114, and 256 of them 184, 179: it is units of
+// unequal lengths that gain from the first form.  Head_dim 64 keeps that (26.9 against 31.9, p in one part).
 // Two CTAs also where a lane's 200 and more registers leave no room for a third: 16 rows of head_dim 128, 32 of 64.
 int q8_stages(int D, int tile_rows, long long units, int sm_count) {
   return D == 128 && (tile_rows == 16 || units <= sm_count) ? 3 : 2;
@@ -690,8 +691,8 @@ attn_q8_cluster_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
 constexpr int kQ8JoinThreads = 256;
 constexpr int kQ8JoinWarps = kQ8JoinThreads / 32;
 // Positions of a weight CTA: with few rows per kv head its threads are for positions, with more they share the rows.  From 256
-// rows on 32 positions, so that the rows are shared 32 ways: 568 rows of one head of 64 and 8192 positions 36 us the call, 55
-// with 128 positions, 223 with all rows in a thread; 1136 rows, 8192 positions 54, 94.  Below, every CTA's own pass over the
+// rows on 32 positions, so that the rows are shared 32 ways: 568 rows of one head of 64 and 8192 positions 36 us the call (p in
+// one part here; two: 37), 55 with 128 positions, 223 with all rows in a thread; 1136 rows, 8192 positions 54, 94.  Below, every CTA's own pass over the
 // rows' sums weighs more (64 rows of 8 x 8 heads, 4096 positions: 133, 103), so there 128, unless those CTAs are fewer than the
 // SMs (142 rows of one head, 2000 positions: 21.2, 26.1); 32 rows and fewer gain nothing there either (20 rows of 8 heads,
 // 2000 positions: 24.1, 21.5).

@@ -18,10 +18,11 @@
 //
 // Algorithmic flops: 4 * D per visible (row, position).
 //
-// Measured: 2 x 2048 queries on 8192 positions, 32 / 8 heads of 128, causal, bf16: 593 to 605 us = 800 TFLOP/s, 48 % of the
-// measured product rate.  Bound by the softmax warps' chain (tensor memory -> maximum -> exponential -> tensor memory; ncu: tensor
-// pipe 39 %, XU 36 %, ALU 34 %): without conversion 4 % less, without exponentials 12 % less; per CTA 9 us of set-up, q
-// and output.  The 16-bit attention core of this library takes 466 us (p in one part) and 605 us (two parts) for the shape.
+// Measured: 2 x 2048 queries on 8192 positions, 32 / 8 heads of 128, causal, bf16: 685 to 728 us (at the power cap) = 700 to 660
+// TFLOP/s, 42 to 40 % of the measured product rate; fp16 698; single_p 609 (790 TFLOP/s) and 597.  Bound by the softmax warps' chain
+// (tensor memory -> maximum -> exponential -> tensor memory; ncu: tensor pipe 47 %, ALU 36 %, XU 33 %); with p in one part, without
+// conversion 4 % less, without exponentials 12 % less; per CTA 9 us of set-up, q and output.  The 16-bit attention core of this
+// library takes 605 us for the shape (single_p 524).
 #include <type_traits>
 
 #include "attn_q8.cuh"
@@ -40,7 +41,7 @@ constexpr float kTcPBias = 6.0f;              // P' <= 2^14 with it
 // Pieces of a pair at most.  One round and 4 pairs without a mask, 6144 positions: 153 us with 16, 160 with 8; and 12 pairs 156, 159;
 // more pairs than that leave room for 8 or less
 constexpr int kTcMaxCut = 16;
-// 512 pairs without a mask: 16 key blocks 200 us whole, 213 with the last round in pieces; 32: 359, 357; 64: 677, 647
+// 512 pairs without a mask: 16 key blocks 218 us whole, 234 with the last round in pieces; 32: 393, 394; 40: 481, 472; 64: 744, 711
 constexpr int kTcMinCutBlocks = 40;
 // Key blocks of a pair from which on few pairs are divided, down to one a CTA.  40 queries of 8 heads of 128 on 8: 3 blocks 17.2 us
 // whole, 18.7 divided; 4 blocks 19.7 and 18.9 (21.9 with two a CTA at least); 8 blocks 26.8 and 18.8 (22.6); 71 heads of 64 x 16
@@ -782,10 +783,12 @@ int launch_typed(const TrnAttnQ8Args& a, cudaStream_t st, const DeviceState& ds)
 
 }  // namespace
 
-// More than 32 rows per kv head (bf16, us here and in attn_q8.cu: 32 rows of 8 x 8 heads, 4096 positions 61.6, 46.4; 36 rows of
-// 16 x 8 heads, 2048 positions 48.7, 62.8; 60 rows of 7 x 32 heads, 4674 positions 191, 226; 71 rows of 32 x 1 head of 64, 4096
-// positions 31.2, 40.7), and no weights (those are summed from scores that attn_q8.cu keeps; kept here, by threads with a row
-// each: 36 rows of 8 x 8 heads, 4096 positions 95.8 us, there 78.1; 568 rows of one head of 64, 8192 positions 67.6, 55.8)
+// More than 32 rows per kv head (bf16, us here and in attn_q8.cu: 24 rows of 8 x 8 heads, 4096 positions 65.0, 50.9; 32 rows 65.8, 51.7; 36
+// rows 65.5, 66.2; 36 rows of 16 x 8 heads, 2048 positions 52.9, 74.6; 60 rows of 32 x 1 head, 4674 positions 48.1, 56.3; 71 rows of
+// 32 x 1 head of 64, 4096 positions 32.9, 42.9.  Few units of few positions would still be faster there: 36 rows of 8 heads, 1000
+// positions 18.6, 11.9; 71 rows of one head, 4096 positions 19.5, 15.1), and
+// no weights (those are summed from scores that attn_q8.cu keeps; kept here, by threads with a row each, p in one part: 36 rows of
+// 8 x 8 heads, 4096 positions 95.8 us, there 78.1; 568 rows of one head of 64, 8192 positions 67.6, 55.8)
 bool attn_q8_tc_applies(const TrnAttnQ8Args& a) {
   return a.weight == nullptr && static_cast<long long>(a.M) * (a.Hq / a.Hkv) > 32;
 }

@@ -11,8 +11,10 @@
 // Launch 2 moves: one CTA per (row, keys or values, group of destination positions) copies the kept rows; for 8-bit caches
 // the group is a scale block, whose scale becomes the largest its rows had.
 //
-// Bound by latency: 4 x 8 rows of 4096 positions (4 heads each), 1024 kept: 12.3 us, of which 3.8 are two empty launches; 2 rows
-// of 32768 (71 heads each, summed first): 19.6 us; 262144 positions: 28.6 us.
+// Calls one behind another, and the launches by themselves (cold): 4 x 8 rows of 4096 positions (4 heads each), 1024 kept in 8 bits:
+// 14.6 us; select 12.4, on as many CTAs as there are rows, and move 7.5 (two empty launches: 3.8).  2 rows of 32768 positions (71 heads
+// each), 2048 kept in 16 bits: 20.5 us; sums 14.8 (17.8 MB: bound by the widening to 64 bits), select 12.4, move 4.2.  32 rows of
+// 1040, 520 kept: 10.6 us; 8.8 and 5.5.  One row of 262144, 70001 kept: 38 us.
 #include "q8.cuh"
 #include "small_mma.cuh"
 

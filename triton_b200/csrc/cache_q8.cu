@@ -7,7 +7,8 @@
 // rewriting exact, so growing a scale token by token loses nothing but what falls under the smallest code.
 //
 // Both kernels are bound by memory: append reads 2 and writes 1 byte per new element, read the other way round.  8 x 2048 rows of
-// 8 heads of 128 (100 MB each): 17.5 us (5.8 TB/s, 89 % of the copy rate) and 17 us; a single row 1.7 us.
+// 8 heads of 128 (100 MB each): 17.7 us a call (5.7 TB/s, 88 % of the copy rate) and 17.7; a single row 3.1 to 4.2 us by itself, 1.4 and
+// 1.7 behind other launches of a graph.
 #include "q8.cuh"
 
 namespace trn {

@@ -12,7 +12,8 @@ namespace trn {
 // v's scale stands at its whole power of two in the running maximum, m' = max (t + ceil log2 vs), and as itself in the factor of
 // the product:  E = 2^(t - m'),  l = sum E,  P' = E vs.  With vs within [2^-64, 2^120] the terms E of a row reach from
 // 2^-120 (the maximum's own, at the largest scale) to 2^64, so the sum of up to 2^29 of them stays inside 32 bits with a
-// factor of 2^30 (kQ8PBias + kQ8LBias), and what lies under 2^-126, which is flushed, is 2^-36 of the row's sum or less.  (l as sum of
+// factor of 2^30 (kQ8PBias + kQ8LBias), and what lies under 2^-126, which is flushed, is 2^-36 of the row's sum or less (2^-30 in
+// attn_q8_tc.cu, whose P' carries at least 2^6 in the place of 2^12).  (l as sum of
 // P' / vs loses the terms whose P' is flushed, although 1 / vs may make them the largest: scales 2^138 apart.)
 constexpr float kQ8PBias = 12.f;               // log2 of the factor P' carries into the product
 constexpr float kQ8LBias = 18.f;               // log2 of the factor E carries beside that
